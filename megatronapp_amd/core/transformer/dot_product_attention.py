@@ -22,6 +22,7 @@ from ..enums import AttnMaskType
 from ..fusions.fused_softmax import FusedScaleMaskSoftmax
 from ..tensor_parallel.utils import divide
 from ..transformer_config import TransformerConfig
+from .packed_attention import packed_attention, packed_attention_supported
 from ... import ops as _ops
 
 
@@ -194,8 +195,29 @@ class FlashAttention(nn.Module):
             return False
         return hn in (64, 128) and query.dtype == torch.bfloat16
 
+    def _packed(self, query, key, value, attention_mask, attn_mask_type,
+                attention_bias, packed_seq_params):
+        """A stream of sequences: each attends within itself."""
+        if not packed_attention_supported(query) or \
+                value.shape != key.shape or \
+                (self.dropout_p > 0 and self.training):
+            return self._fallback(query, key, value, attention_mask,
+                                  attn_mask_type, attention_bias,
+                                  packed_seq_params)
+        mask_type = (attn_mask_type if attn_mask_type is not None
+                     else self.attn_mask_type)
+        o = packed_attention(query, key, value, packed_seq_params,
+                             softmax_scale=self.softmax_scale,
+                             causal=mask_type == AttnMaskType.causal)
+        return o.reshape(o.shape[0], o.shape[1], -1)
+
     def forward(self, query, key, value, attention_mask=None,
                 attn_mask_type=None, attention_bias=None, packed_seq_params=None):
+        if packed_seq_params is not None and \
+                packed_seq_params.cu_seqlens_q is not None:
+            return self._packed(query, key, value, attention_mask,
+                                attn_mask_type, attention_bias,
+                                packed_seq_params)
         if not self._supported(query, key):
             return self._fallback(query, key, value, attention_mask,
                                   attn_mask_type, attention_bias, packed_seq_params)

@@ -111,6 +111,17 @@ void launch_attn_bwd(const void*, const void*, const void*, const void*,
                      const void*, const float*, float*, void*, void*, void*,
                      int, int, int, int, int, int, float, bool, hipStream_t);
 
+void launch_packed_attn_fwd(const void*, const void*, const void*, void*,
+                            float*, const int*, const int*, int, int, int, int,
+                            int, int, int, float, bool, bool, const long*,
+                            const long*, const long*, hipStream_t);
+void launch_packed_attn_bwd(const void*, const void*, const void*,
+                            const void*, const void*, const float*, float*,
+                            void*, void*, void*, const int*, const int*, int,
+                            int, int, int, int, int, int, float, bool, bool,
+                            const long*, const long*, const long*, const long*,
+                            hipStream_t);
+
 namespace {
 
 hipStream_t cur_stream() {
@@ -717,6 +728,108 @@ std::vector<torch::Tensor> attn_fwd_ablate(torch::Tensor q, torch::Tensor k,
   return {o, lse};
 }
 
+// --------------------------------------------------------- packed attention
+// [t, b, h, d] in 16 bits; views are read as they are where each row of a
+// head is adjacent and starts on 16 bytes, others are laid out first
+torch::Tensor packed_rows(const torch::Tensor& t, const char* name,
+                          const torch::Tensor& like, long* strides) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name,
+              " must be on the GPU of the query");
+  TORCH_CHECK(t.scalar_type() == like.scalar_type(), name,
+              " must have the query's type");
+  TORCH_CHECK(t.dim() == 4, name, " must be [t, b, h, d]");
+  bool fits = t.stride(3) == 1 &&
+              reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int i = 0; i < 3; ++i)
+    fits = fits && (t.stride(i) % 8 == 0 || t.size(i) <= 1);
+  auto r = fits ? t : t.contiguous();
+  for (int i = 0; i < 3; ++i)  // a single row's stride is never used
+    strides[i] = r.size(i) <= 1 ? 0 : (long)r.stride(i);
+  return r;
+}
+
+struct PackedShape {
+  int tq, tk, b, nh, ng, d, n;
+  bool fp16;
+};
+
+PackedShape packed_shape(const torch::Tensor& q, const torch::Tensor& k,
+                         const torch::Tensor& v, const torch::Tensor& cu_q,
+                         const torch::Tensor& cu_k) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 4 && k.dim() == 4 &&
+                  k.sizes() == v.sizes(),
+              "packed attention: q, k, v must be [t, b, h, d] on the GPU");
+  TORCH_CHECK(q.scalar_type() == torch::kBFloat16 ||
+                  q.scalar_type() == torch::kHalf,
+              "packed attention: bf16 or fp16");
+  TORCH_CHECK(q.size(3) == 64 || q.size(3) == 128,
+              "packed attention: head size 64 or 128");
+  TORCH_CHECK(k.size(1) == q.size(1) && k.size(3) == q.size(3) &&
+                  k.size(2) > 0 && q.size(2) % k.size(2) == 0,
+              "packed attention: shapes of q and k do not fit");
+  TORCH_CHECK(q.size(0) < (1l << 30) && k.size(0) < (1l << 30),
+              "packed attention: too many tokens");
+  for (auto* c : {&cu_q, &cu_k})
+    TORCH_CHECK(c->device() == q.device() && c->dim() == 1 &&
+                    c->scalar_type() == torch::kInt32 && c->is_contiguous() &&
+                    c->numel() == cu_q.numel() && c->numel() > 0,
+                "packed attention: cu_seqlens must be int32 [n + 1] on the "
+                "GPU of the query");
+  return {(int)q.size(0), (int)k.size(0), (int)q.size(1), (int)q.size(2),
+          (int)k.size(2), (int)q.size(3), (int)cu_q.numel() - 1,
+          q.scalar_type() == torch::kHalf};
+}
+
+std::vector<torch::Tensor> packed_attn_fwd(torch::Tensor q, torch::Tensor k,
+                                           torch::Tensor v, torch::Tensor cu_q,
+                                           torch::Tensor cu_k, double scale,
+                                           bool causal) {
+  const PackedShape s = packed_shape(q, k, v, cu_q, cu_k);
+  c10::DeviceGuard guard(q.device());
+  auto o = torch::empty({s.tq, s.b, s.nh, s.d}, q.options());
+  auto lse = torch::empty({s.b, s.nh, s.tq},
+                          q.options().dtype(torch::kFloat32));
+  if (o.numel() == 0) return {o, lse};
+  long qs[3], ks[3], vs[3];
+  auto qr = packed_rows(q, "q", q, qs), kr = packed_rows(k, "k", q, ks),
+       vr = packed_rows(v, "v", q, vs);
+  launch_packed_attn_fwd(qr.data_ptr(), kr.data_ptr(), vr.data_ptr(),
+                         o.data_ptr(), lse.data_ptr<float>(),
+                         cu_q.data_ptr<int>(), cu_k.data_ptr<int>(), s.n, s.tq,
+                         s.tk, s.b, s.nh, s.ng, s.d, (float)scale, causal,
+                         s.fp16, qs, ks, vs, cur_stream());
+  return {o, lse};
+}
+
+std::vector<torch::Tensor> packed_attn_bwd(
+    torch::Tensor dout, torch::Tensor q, torch::Tensor k, torch::Tensor v,
+    torch::Tensor o, torch::Tensor lse, torch::Tensor cu_q, torch::Tensor cu_k,
+    double scale, bool causal) {
+  const PackedShape s = packed_shape(q, k, v, cu_q, cu_k);
+  c10::DeviceGuard guard(q.device());
+  TORCH_CHECK(dout.sizes() == q.sizes() && o.sizes() == q.sizes() &&
+                  o.is_contiguous() && o.scalar_type() == q.scalar_type() &&
+                  lse.numel() == (long)s.b * s.nh * s.tq &&
+                  lse.is_contiguous() &&
+                  lse.scalar_type() == torch::kFloat32,
+              "packed attention: dout, o and lse must be the forward's");
+  auto dq = torch::empty({s.tq, s.b, s.nh, s.d}, q.options());
+  auto dk = torch::empty({s.tk, s.b, s.ng, s.d}, q.options());
+  auto dv = torch::empty({s.tk, s.b, s.ng, s.d}, q.options());
+  if (s.b == 0 || s.nh == 0) return {dq, dk, dv};
+  auto dot = torch::empty_like(lse);
+  long os[3], qs[3], ks[3], vs[3];
+  auto dr = packed_rows(dout, "dout", q, os), qr = packed_rows(q, "q", q, qs),
+       kr = packed_rows(k, "k", q, ks), vr = packed_rows(v, "v", q, vs);
+  launch_packed_attn_bwd(
+      dr.data_ptr(), qr.data_ptr(), kr.data_ptr(), vr.data_ptr(), o.data_ptr(),
+      lse.data_ptr<float>(), dot.data_ptr<float>(), dq.data_ptr(),
+      dk.data_ptr(), dv.data_ptr(), cu_q.data_ptr<int>(), cu_k.data_ptr<int>(),
+      s.n, s.tq, s.tk, s.b, s.nh, s.ng, s.d, (float)scale, causal, s.fp16, os,
+      qs, ks, vs, cur_stream());
+  return {dq, dk, dv};
+}
+
 // --------------------------------------------------------------------- adam
 // states fp32 OR bf16 (precision-aware optimizer); params/grads fp32
 static bool adam_states_bf16(const torch::Tensor& m, const torch::Tensor& v) {
@@ -896,6 +1009,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   mod.def("wgrad_accum_bgrad", &wgrad_accum_bgrad);
   mod.def("attn_fwd", &attn_fwd);
   mod.def("attn_fwd_ablate", &attn_fwd_ablate);
+  mod.def("packed_attn_fwd", &packed_attn_fwd);
+  mod.def("packed_attn_bwd", &packed_attn_bwd);
   mod.def("attn_bwd", &attn_bwd);
   mod.def("colsum_accum", &colsum_accum);
   mod.def("embedding_bwd_accum", &embedding_bwd_accum);

@@ -1,0 +1,615 @@
+// Attention over packed sequences, forward and backward (gfx950).
+//
+//   row p of sequence i (sq queries, sk keys) sees keys [0, hi(p)):
+//     hi(p) = sk, or causal min(sk, p + 1 + sk - sq), none if that is <= 0
+//   S = scale Q K^T, P = softmax(S), O = P V (0 where no key is seen)
+//   lse = log2 sum 2^(S log2 e), kept for the backward
+//   D = sum_d dO O, dV = P^T dO, dS = P (dO V^T - D)
+//   dQ = scale dS K, dK = scale dS^T Q, both sums over the group's heads
+//
+// The stream's sequences are given on the device, so the grid has as many
+// tiles as could be needed and a block finds its own (sequence, tile) by
+// adding up the sequences' tile counts.  No tile holds rows of two
+// sequences: nothing of one request reaches another's sums, NaN included.
+// The places before the first and behind the last sequence are taken as
+// sequences without keys, so they come out as zeros.
+
+#include "attn_tiles.h"
+
+namespace {
+
+constexpr int BM = 128;     // rows of a block: four waves of 32
+constexpr int BN = 64;      // rows of a tile in LDS
+constexpr int BLOCK = 256;
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Strides {
+  long t, b, h;             // elements; the head's elements are adjacent
+};
+
+struct Packing {
+  const int* cu_q;          // [n + 1]
+  const int* cu_k;
+  int n, tq, tk;            // sequences, places of the two streams
+};
+
+struct Span {
+  int q0, sq, k0, sk;       // the sequence's places and lengths
+  int tile;                 // the block's tile of it
+};
+
+__device__ __forceinline__ int bounded(const int* cu, int i, int lo, int hi) {
+  return max(lo, min(cu[i], hi));
+}
+
+// sequence i - 1 of the stream; 0 and n + 1 are what lies before and behind
+__device__ __forceinline__ void span_of(const int* cu, int n, int total, int i,
+                                        int& from, int& len) {
+  from = i == 0 ? 0 : bounded(cu, i - 1, 0, total);
+  const int to = i > n ? total : bounded(cu, i, from, total);
+  len = max(to - from, 0);
+}
+
+// The `slot`-th tile of BM rows of the query (or key) stream.
+template <bool KEYS>
+__device__ __forceinline__ bool find_span(const Packing& pk, int slot,
+                                          int lane, Span& s) {
+  const int* cu = KEYS ? pk.cu_k : pk.cu_q;
+  const int total = KEYS ? pk.tk : pk.tq;
+  for (int base = 0; base < pk.n + 2; base += WAVE) {
+    const int i = base + lane;
+    int from = 0, len = 0;
+    if (i < pk.n + 2) span_of(cu, pk.n, total, i, from, len);
+    const int tiles = (len + BM - 1) / BM;
+    int upto = tiles;
+#pragma unroll
+    for (int off = 1; off < WAVE; off <<= 1) {
+      const int x = __shfl_up(upto, off, WAVE);
+      if (lane >= off) upto += x;
+    }
+    const unsigned long long hit = __ballot(upto > slot);
+    if (hit) {
+      const int w = __ffsll((unsigned long long)hit) - 1;
+      const int seq = base + w;
+      const int f = __builtin_amdgcn_readlane(from, w);
+      const int l = __builtin_amdgcn_readlane(len, w);
+      s.tile = slot - (__builtin_amdgcn_readlane(upto, w) -
+                       __builtin_amdgcn_readlane(tiles, w));
+      int of = 0, ol = 0;   // of the other stream
+      if (seq > 0 && seq <= pk.n) {
+        if (KEYS) span_of(pk.cu_q, pk.n, pk.tq, seq, of, ol);
+        else span_of(pk.cu_k, pk.n, pk.tk, seq, of, ol);
+      }
+      s.q0 = KEYS ? of : f;
+      s.sq = KEYS ? ol : l;
+      s.k0 = KEYS ? f : of;
+      s.sk = KEYS ? l : ol;
+      return true;
+    }
+    slot -= __builtin_amdgcn_readlane(upto, WAVE - 1);
+  }
+  return false;
+}
+
+// keys that row p of the sequence sees
+template <bool CAUSAL>
+__device__ __forceinline__ int keys_of(const Span& s, int p) {
+  return CAUSAL ? max(0, min(s.sk, p + 1 + s.sk - s.sq)) : s.sk;
+}
+
+__device__ __forceinline__ f32x16 zeros16() {
+  f32x16 z;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z[r] = 0.f;
+  return z;
+}
+
+// head h of the block: heads of one group follow each other in steps of ng,
+// so that they run on one XCD (blocks go round the eight) and share its L2
+__device__ __forceinline__ int head_of(int x, int ng, int rep) {
+  return (x % ng) * rep + x / ng;
+}
+
+// ------------------------------------------------------------------ forward
+template <class T, int D, bool CAUSAL>
+__global__ __launch_bounds__(BLOCK, 2) void packed_fwd_kernel(
+    const unsigned short* __restrict__ q, const unsigned short* __restrict__ k,
+    const unsigned short* __restrict__ v, unsigned short* __restrict__ o,
+    float* __restrict__ lse, Packing pk, int b, int nh, int ng, float c,
+    Strides qs, Strides ks, Strides vs) {
+  __shared__ __attribute__((aligned(16))) unsigned short kv0_lds[2 * BN * D];
+  __shared__ __attribute__((aligned(16))) unsigned short kv1_lds[2 * BN * D];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h = lane >> 5, n = lane & 31;
+  Span s;
+  const unsigned x = blockIdx.x % (b * nh), slot = blockIdx.x / (b * nh);
+  // last tiles first: under a causal mask they have the most keys
+  if (!find_span<false>(pk, gridDim.x / (b * nh) - 1 - slot, lane, s)) return;
+  const int bi = x / nh, head = head_of(x % nh, ng, nh / ng);
+  const int hk = head / (nh / ng);
+
+  const int p0 = s.tile * BM + wave * 32;       // the wave's first row
+  const int p = p0 + n;                         // the lane's row
+  const bool mine = p < s.sq;
+  const long row = s.q0 + min(p, s.sq - 1);
+  constexpr int NF = D / 16, ND = D / 32;
+  typename T::x8 qf[NF];
+  {
+    const unsigned short* src = q + row * qs.t + bi * qs.b + head * qs.h;
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+      qf[f] = *(const typename T::x8*)(src + 16 * f + 8 * h);
+  }
+  const int most = keys_of<CAUSAL>(s, min(s.tile * BM + BM, s.sq) - 1);
+  const int wave_most = keys_of<CAUSAL>(s, min(p0 + 31, s.sq - 1));
+  const int wave_least = keys_of<CAUSAL>(s, min(p0, s.sq - 1));
+  const int lane_most = keys_of<CAUSAL>(s, min(p, s.sq - 1));
+  const int tiles = (most + BN - 1) / BN;
+  const unsigned short* kp = k + s.k0 * ks.t + bi * ks.b + hk * ks.h;
+  const unsigned short* vp = v + s.k0 * vs.t + bi * vs.b + hk * vs.h;
+
+  f32x16 acc[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) acc[i] = zeros16();
+  float m = -INFINITY, ms = 0.f, l = 0.f;
+
+  auto fetch = [&](int t, unsigned short* img) {
+    const int last = s.sk - 1 - t * BN;
+    load_tile<D, BN, 4>(img, kp + (long)t * BN * ks.t, ks.t, last, wave, lane);
+    load_tile<D, BN, 4>(img + BN * D, vp + (long)t * BN * vs.t, vs.t, last,
+                        wave, lane);
+  };
+  auto step = [&](int t, const unsigned short* img) {
+    const int at = t * BN;
+    if (p0 >= s.sq || at >= wave_most) return;
+    f32x16 st[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      st[u] = zeros16();
+      const int kr = 32 * u + tile_row(n);
+#pragma unroll
+      for (int f = 0; f < NF; ++f)
+        st[u] = T::mfma32(read_rows<T, D>(img, kr, f, h), qf[f], st[u]);
+    }
+    if (at + BN > wave_least) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (at + 32 * u + 16 * (r >> 3) + 8 * h + (r & 7) >= lane_most)
+            st[u][r] = -INFINITY;
+    }
+    float mt = st[0][0];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mt = fmaxf(mt, st[u][r]);
+    mt = half_max(mt) * c;
+    // the running maximum moves only where it has to: 2^8 times too large
+    // a sum loses nothing in 32 bits
+    if (__any(mt > m + 8.f)) {
+      const float mn = fmaxf(m, mt);
+      const float a = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      ms = mn == -INFINITY ? 0.f : mn;
+      l *= a;
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] *= a;
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        st[u][r] = __builtin_amdgcn_exp2f(fmaf(st[u][r], c, -ms));
+        l += st[u][r];
+      }
+    const unsigned short* vi = img + BN * D;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const typename T::x8 pf = pack8<T>(st[u], 8 * x);
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+          acc[i] = T::mfma32(read_cols<T, D>(vi, 32 * u + 16 * x, i, lane), pf,
+                             acc[i]);
+      }
+  };
+  // one tile is used while the next one comes in
+  auto turn = [&](int t, unsigned short* img, unsigned short* next) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);         // vmcnt(0)
+    __syncthreads();
+    if (t + 1 < tiles) fetch(t + 1, next);
+    const int rows = s.sk - t * BN;
+    if (rows < BN) {
+      clear_rows<D, BN, BLOCK>(img + BN * D, rows, tid);
+      __syncthreads();
+    }
+    step(t, img);
+  };
+  if (tiles > 0) fetch(0, kv0_lds);
+  for (int t = 0; t < tiles; t += 2) {
+    turn(t, kv0_lds, kv1_lds);
+    if (t + 1 < tiles) turn(t + 1, kv1_lds, kv0_lds);
+  }
+  if (!mine) return;
+  l = half_sum(l);
+  const float by = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  if (h == 0)
+    lse[((long)bi * nh + head) * pk.tq + s.q0 + p] =
+        l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+  unsigned short* dst = o + ((row * b + bi) * nh + head) * D;
+#pragma unroll
+  for (int i = 0; i < ND; ++i) store_cols<T>(dst + 32 * i, acc[i], by, h);
+}
+
+// ----------------------------------------------------------------- backward
+// D[b, h, t] = sum_d dO O, one wave a row pair
+template <class T, int D>
+__global__ __launch_bounds__(BLOCK) void packed_bwd_dot_kernel(
+    const unsigned short* __restrict__ dout,
+    const unsigned short* __restrict__ o, float* __restrict__ dot, int tq,
+    int b, int nh, Strides os) {
+  constexpr int LANES = D / 8;                  // of a row
+  const long rows = (long)tq * b * nh;
+  const long i = ((long)blockIdx.x * BLOCK + threadIdx.x) / LANES;
+  const int x = threadIdx.x % LANES;
+  if (i >= rows) return;                        // whole rows leave together
+  const int head = i % nh;
+  const long t = i / nh / b;
+  const int bi = i / nh % b;
+  const s16x8 a = *(const s16x8*)(dout + t * os.t + bi * os.b + head * os.h +
+                                  8 * x);
+  const s16x8 e = *(const s16x8*)(o + i * D + 8 * x);
+  float sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    sum += T::to_float((unsigned short)a[j]) * T::to_float((unsigned short)e[j]);
+#pragma unroll
+  for (int off = LANES / 2; off > 0; off >>= 1)
+    sum += __shfl_xor(sum, off, LANES);
+  if (x == 0) dot[((long)bi * nh + head) * tq + t] = sum;
+}
+
+// dQ: rows of queries, over their keys
+template <class T, int D, bool CAUSAL>
+__global__ __launch_bounds__(BLOCK, 2) void packed_bwd_dq_kernel(
+    const unsigned short* __restrict__ q, const unsigned short* __restrict__ k,
+    const unsigned short* __restrict__ v,
+    const unsigned short* __restrict__ dout, const float* __restrict__ lse,
+    const float* __restrict__ dot, unsigned short* __restrict__ dq, Packing pk,
+    int b, int nh, int ng, float scale, Strides qs, Strides ks, Strides vs,
+    Strides os) {
+  __shared__ __attribute__((aligned(16))) unsigned short kv0_lds[2 * BN * D];
+  __shared__ __attribute__((aligned(16))) unsigned short kv1_lds[2 * BN * D];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h = lane >> 5, n = lane & 31;
+  Span s;
+  const unsigned x = blockIdx.x % (b * nh), slot = blockIdx.x / (b * nh);
+  // last tiles first: under a causal mask they have the most keys
+  if (!find_span<false>(pk, gridDim.x / (b * nh) - 1 - slot, lane, s)) return;
+  const int bi = x / nh, head = head_of(x % nh, ng, nh / ng);
+  const int hk = head / (nh / ng);
+  const float c = scale * LOG2E;
+
+  const int p0 = s.tile * BM + wave * 32;
+  const int p = p0 + n;
+  const long row = s.q0 + min(p, s.sq - 1);
+  constexpr int NF = D / 16, ND = D / 32;
+  typename T::x8 qf[NF], df[NF];
+  {
+    const unsigned short* src = q + row * qs.t + bi * qs.b + head * qs.h;
+    const unsigned short* dsrc = dout + row * os.t + bi * os.b + head * os.h;
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      qf[f] = *(const typename T::x8*)(src + 16 * f + 8 * h);
+      df[f] = *(const typename T::x8*)(dsrc + 16 * f + 8 * h);
+    }
+  }
+  const long stat = ((long)bi * nh + head) * pk.tq + row;
+  const float rl = lse[stat], rd = dot[stat];
+  const int most = keys_of<CAUSAL>(s, min(s.tile * BM + BM, s.sq) - 1);
+  const int wave_most = keys_of<CAUSAL>(s, min(p0 + 31, s.sq - 1));
+  const int wave_least = keys_of<CAUSAL>(s, min(p0, s.sq - 1));
+  const int lane_most = keys_of<CAUSAL>(s, min(p, s.sq - 1));
+  const int tiles = (most + BN - 1) / BN;
+  const unsigned short* kp = k + s.k0 * ks.t + bi * ks.b + hk * ks.h;
+  const unsigned short* vp = v + s.k0 * vs.t + bi * vs.b + hk * vs.h;
+
+  f32x16 acc[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) acc[i] = zeros16();
+
+  auto fetch = [&](int t, unsigned short* img) {
+    const int last = s.sk - 1 - t * BN;
+    load_tile<D, BN, 4>(img, kp + (long)t * BN * ks.t, ks.t, last, wave, lane);
+    load_tile<D, BN, 4>(img + BN * D, vp + (long)t * BN * vs.t, vs.t, last,
+                        wave, lane);
+  };
+  auto step = [&](int t, const unsigned short* img) {
+    const int at = t * BN;
+    if (p0 >= s.sq || at >= wave_most) return;
+    const bool edge = at + BN > wave_least;
+    const unsigned short* vi = img + BN * D;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      f32x16 st = zeros16(), dp = zeros16();
+      const int kr = 32 * u + tile_row(n);
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        st = T::mfma32(read_rows<T, D>(img, kr, f, h), qf[f], st);
+        dp = T::mfma32(read_rows<T, D>(vi, kr, f, h), df[f], dp);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        dp[r] = __builtin_amdgcn_exp2f(fmaf(st[r], c, -rl)) * (dp[r] - rd);
+      if (edge) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (at + 32 * u + 16 * (r >> 3) + 8 * h + (r & 7) >= lane_most)
+            dp[r] = 0.f;
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const typename T::x8 sf = pack8<T>(dp, 8 * x);
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+          acc[i] = T::mfma32(read_cols<T, D>(img, 32 * u + 16 * x, i, lane),
+                             sf, acc[i]);
+      }
+    }
+  };
+  auto turn = [&](int t, unsigned short* img, unsigned short* next) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);         // vmcnt(0)
+    __syncthreads();
+    if (t + 1 < tiles) fetch(t + 1, next);
+    const int rows = s.sk - t * BN;
+    if (rows < BN) {
+      clear_rows<D, BN, BLOCK>(img, rows, tid);
+      __syncthreads();
+    }
+    step(t, img);
+  };
+  if (tiles > 0) fetch(0, kv0_lds);
+  for (int t = 0; t < tiles; t += 2) {
+    turn(t, kv0_lds, kv1_lds);
+    if (t + 1 < tiles) turn(t + 1, kv1_lds, kv0_lds);
+  }
+  if (p >= s.sq) return;
+  unsigned short* dst = dq + ((row * b + bi) * nh + head) * D;
+#pragma unroll
+  for (int i = 0; i < ND; ++i) store_cols<T>(dst + 32 * i, acc[i], scale, h);
+}
+
+// dK and dV: rows of keys, over the queries that see them, for each head of
+// the group in turn (one block sums them all, so no atomics)
+template <class T, int D, bool CAUSAL>
+__global__ __launch_bounds__(BLOCK, 1) void packed_bwd_dkv_kernel(
+    const unsigned short* __restrict__ q, const unsigned short* __restrict__ k,
+    const unsigned short* __restrict__ v,
+    const unsigned short* __restrict__ dout, const float* __restrict__ lse,
+    const float* __restrict__ dot, unsigned short* __restrict__ dk,
+    unsigned short* __restrict__ dv, Packing pk, int b, int nh, int ng,
+    float scale, Strides qs, Strides ks, Strides vs, Strides os) {
+  // Q, dO, then the rows' lse and D
+  constexpr int IMG = 2 * BN * D + 4 * BN;
+  __shared__ __attribute__((aligned(16))) unsigned short qd0_lds[IMG];
+  __shared__ __attribute__((aligned(16))) unsigned short qd1_lds[IMG];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h = lane >> 5, n = lane & 31;
+  Span s;
+  const unsigned x = blockIdx.x % (b * ng);
+  if (!find_span<true>(pk, blockIdx.x / (b * ng), lane, s)) return;
+  const int bi = x / ng, hk = x % ng, rep = nh / ng;
+  const float c = scale * LOG2E;
+
+  const int j0 = s.tile * BM + wave * 32;       // the wave's first key
+  const int j = j0 + n;                         // the lane's key
+  const long row = s.k0 + min(j, s.sk - 1);
+  constexpr int NF = D / 16, ND = D / 32;
+  typename T::x8 kf[NF], vf[NF];
+  {
+    const unsigned short* ksrc = k + row * ks.t + bi * ks.b + hk * ks.h;
+    const unsigned short* vsrc = v + row * vs.t + bi * vs.b + hk * vs.h;
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      kf[f] = *(const typename T::x8*)(ksrc + 16 * f + 8 * h);
+      vf[f] = *(const typename T::x8*)(vsrc + 16 * f + 8 * h);
+    }
+  }
+  // the first query that sees the block's first key
+  const int ahead = CAUSAL ? s.sk - s.sq : 0;
+  const int first = CAUSAL ? max(0, s.tile * BM - ahead) / BN : 0;
+  const int per = max(0, (s.sq + BN - 1) / BN - first);
+  const int turns = per * rep;
+
+  f32x16 ak[ND], av[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) ak[i] = av[i] = zeros16();
+
+  auto fetch = [&](int it, unsigned short* img) {
+    const int head = hk * rep + it / per, at = (first + it % per) * BN;
+    const int last = s.sq - 1 - at;
+    const unsigned short* qp =
+        q + (s.q0 + at) * qs.t + bi * qs.b + head * qs.h;
+    const unsigned short* dp =
+        dout + (s.q0 + at) * os.t + bi * os.b + head * os.h;
+    load_tile<D, BN, 4>(img, qp, qs.t, last, wave, lane);
+    load_tile<D, BN, 4>(img + BN * D, dp, os.t, last, wave, lane);
+    // four bytes a lane: the rows' statistics, by one wave each
+    if (wave < 2) {
+      const float* src = (wave ? dot : lse) +
+                         ((long)bi * nh + head) * pk.tq + s.q0 + at +
+                         min(lane, last);
+      __builtin_amdgcn_global_load_lds(
+          (global_char*)src, (lds_char*)(img + 2 * BN * D + 2 * BN * wave), 4,
+          0, 0);
+    }
+  };
+  auto step = [&](int it, const unsigned short* img) {
+    const int at = (first + it % per) * BN;
+    if (j0 >= s.sk) return;
+    const unsigned short* di = img + BN * D;
+    const float* sl = (const float*)(img + 2 * BN * D);
+    const float* sd = sl + BN;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int a0 = at + 32 * u;
+      // no key of the wave is seen by these rows
+      if (a0 >= s.sq || (CAUSAL && j0 > a0 + 31 + ahead)) continue;
+      f32x16 st = zeros16(), dp = zeros16();
+      const int qr = 32 * u + tile_row(n);
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        st = T::mfma32(read_rows<T, D>(img, qr, f, h), kf[f], st);
+        dp = T::mfma32(read_rows<T, D>(di, qr, f, h), vf[f], dp);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int x = 32 * u + 16 * (r >> 3) + 8 * h + (r & 7);
+        st[r] = __builtin_amdgcn_exp2f(fmaf(st[r], c, -sl[x]));
+        dp[r] = st[r] * (dp[r] - sd[x]);
+      }
+      if (a0 + 32 > s.sq || (CAUSAL && j0 + 31 > a0 + ahead)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int x = at + 32 * u + 16 * (r >> 3) + 8 * h + (r & 7);
+          if (x >= s.sq || (CAUSAL && j > x + ahead)) st[r] = dp[r] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const typename T::x8 pf = pack8<T>(st, 8 * x);
+        const typename T::x8 sf = pack8<T>(dp, 8 * x);
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
+          av[i] = T::mfma32(read_cols<T, D>(di, 32 * u + 16 * x, i, lane), pf,
+                            av[i]);
+          ak[i] = T::mfma32(read_cols<T, D>(img, 32 * u + 16 * x, i, lane), sf,
+                            ak[i]);
+        }
+      }
+    }
+  };
+  auto turn = [&](int it, unsigned short* img, unsigned short* next) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);         // vmcnt(0)
+    __syncthreads();
+    if (it + 1 < turns) fetch(it + 1, next);
+    const int rows = s.sq - (first + it % per) * BN;
+    if (rows < BN) {
+      clear_rows<D, BN, BLOCK>(img, rows, tid);
+      clear_rows<D, BN, BLOCK>(img + BN * D, rows, tid);
+      __syncthreads();
+    }
+    step(it, img);
+  };
+  if (turns > 0) fetch(0, qd0_lds);
+  for (int it = 0; it < turns; it += 2) {
+    turn(it, qd0_lds, qd1_lds);
+    if (it + 1 < turns) turn(it + 1, qd1_lds, qd0_lds);
+  }
+  if (j >= s.sk) return;
+  const long at = ((row * b + bi) * ng + hk) * D;
+#pragma unroll
+  for (int i = 0; i < ND; ++i) {
+    store_cols<T>(dk + at + 32 * i, ak[i], scale, h);
+    store_cols<T>(dv + at + 32 * i, av[i], 1.f, h);
+  }
+}
+
+// each sequence may end in a part of a tile
+dim3 grid_for(long heads, int total, int n) {
+  const long blocks = heads * ((long)total / BM + n + 2);
+  if (blocks * BLOCK >= 1l << 32)
+    throw std::runtime_error("packed attention: too many tiles for one launch");
+  return dim3((unsigned)blocks);
+}
+
+}  // namespace
+
+#define PACKED_DISPATCH(RUN)                                              \
+  do {                                                                    \
+    if (fp16) {                                                           \
+      if (d == 128) { if (causal) RUN(Fp16, 128, true); else RUN(Fp16, 128, false); } \
+      else { if (causal) RUN(Fp16, 64, true); else RUN(Fp16, 64, false); }  \
+    } else {                                                              \
+      if (d == 128) { if (causal) RUN(Bf16, 128, true); else RUN(Bf16, 128, false); } \
+      else { if (causal) RUN(Bf16, 64, true); else RUN(Bf16, 64, false); }  \
+    }                                                                     \
+  } while (0)
+
+void launch_packed_attn_fwd(const void* q, const void* k, const void* v,
+                            void* o, float* lse, const int* cu_q,
+                            const int* cu_k, int n, int tq, int tk, int b,
+                            int nh, int ng, int d, float scale, bool causal,
+                            bool fp16, const long* qs, const long* ks,
+                            const long* vs, hipStream_t stream) {
+  const Packing pk = {cu_q, cu_k, n, tq, tk};
+  const dim3 grid = grid_for((long)b * nh, tq, n);
+#define RUN(T, DD, CC)                                                      \
+  hipLaunchKernelGGL((packed_fwd_kernel<T, DD, CC>), grid, dim3(BLOCK), 0,  \
+                     stream, (const unsigned short*)q,                      \
+                     (const unsigned short*)k, (const unsigned short*)v,    \
+                     (unsigned short*)o, lse, pk, b, nh, ng, scale * LOG2E, \
+                     Strides{qs[0], qs[1], qs[2]},                          \
+                     Strides{ks[0], ks[1], ks[2]},                          \
+                     Strides{vs[0], vs[1], vs[2]})
+  PACKED_DISPATCH(RUN);
+#undef RUN
+  HIP_CHECK_LAUNCH();
+}
+
+void launch_packed_attn_bwd(const void* dout, const void* q, const void* k,
+                            const void* v, const void* o, const float* lse,
+                            float* dot, void* dq, void* dk, void* dv,
+                            const int* cu_q, const int* cu_k, int n, int tq,
+                            int tk, int b, int nh, int ng, int d, float scale,
+                            bool causal, bool fp16, const long* os,
+                            const long* qs, const long* ks, const long* vs,
+                            hipStream_t stream) {
+  const Packing pk = {cu_q, cu_k, n, tq, tk};
+  const Strides so = {os[0], os[1], os[2]}, sq = {qs[0], qs[1], qs[2]},
+                sk = {ks[0], ks[1], ks[2]}, sv = {vs[0], vs[1], vs[2]};
+  if (tq > 0) {
+    const long lanes = (long)tq * b * nh * (d / 8);
+    if (lanes >= 1l << 32)
+      throw std::runtime_error("packed attention: too many rows for one launch");
+    const dim3 grid = grid_for((long)b * nh, tq, n);
+#define RUN(T, DD, CC)                                                     \
+  hipLaunchKernelGGL((packed_bwd_dot_kernel<T, DD>),                       \
+                     dim3((unsigned)((lanes + BLOCK - 1) / BLOCK)),        \
+                     dim3(BLOCK), 0, stream, (const unsigned short*)dout,                  \
+                     (const unsigned short*)o, dot, tq, b, nh, so)
+    PACKED_DISPATCH(RUN);
+#undef RUN
+    HIP_CHECK_LAUNCH();
+#define RUN(T, DD, CC)                                                       \
+  hipLaunchKernelGGL((packed_bwd_dq_kernel<T, DD, CC>),                      \
+                     grid, dim3(BLOCK), 0, stream,                   \
+                     (const unsigned short*)q, (const unsigned short*)k,     \
+                     (const unsigned short*)v, (const unsigned short*)dout,  \
+                     lse, dot, (unsigned short*)dq, pk, b, nh, ng, scale,    \
+                     sq, sk, sv, so)
+    PACKED_DISPATCH(RUN);
+#undef RUN
+    HIP_CHECK_LAUNCH();
+  }
+  if (tk > 0) {
+    const dim3 grid = grid_for((long)b * ng, tk, n);
+#define RUN(T, DD, CC)                                                       \
+  hipLaunchKernelGGL((packed_bwd_dkv_kernel<T, DD, CC>),                     \
+                     grid, dim3(BLOCK), 0, stream,                   \
+                     (const unsigned short*)q, (const unsigned short*)k,     \
+                     (const unsigned short*)v, (const unsigned short*)dout,  \
+                     lse, dot, (unsigned short*)dk, (unsigned short*)dv, pk, \
+                     b, nh, ng, scale, sq, sk, sv, so)
+    PACKED_DISPATCH(RUN);
+#undef RUN
+    HIP_CHECK_LAUNCH();
+  }
+}

@@ -25,7 +25,19 @@ SOURCES = [
     "adam.hip", "scan.hip", "ce.hip", "fp8quant.hip", "moe.hip", "dropout.hip",
     "wgrad.cpp",
     "attention.hip",
+    "packed_attention.hip",
 ]
+
+
+def _drop_stale_objects(build_dir: str) -> None:
+    """The build's rules do not know which headers a source includes: an
+    object older than the newest header is compiled again."""
+    newest = max(os.path.getmtime(os.path.join(CSRC, f))
+                 for f in os.listdir(CSRC) if f.endswith(".h"))
+    for f in os.listdir(build_dir):
+        path = os.path.join(build_dir, f)
+        if f.endswith(".o") and os.path.getmtime(path) < newest:
+            os.remove(path)
 
 
 def build(verbose: bool = True) -> str:
@@ -36,6 +48,7 @@ def build(verbose: bool = True) -> str:
                if os.path.exists(os.path.join(CSRC, s))]
     build_dir = os.path.join(HERE, "build")
     os.makedirs(build_dir, exist_ok=True)
+    _drop_stale_objects(build_dir)
     mod = load(
         name="_C",
         sources=sources,
