@@ -122,6 +122,27 @@ void launch_packed_attn_bwd(const void*, const void*, const void*,
                             const long*, const long*, const long*, const long*,
                             hipStream_t);
 
+void launch_cache_fork(int*, int*, int*, int*, int, int, int, int, void*, int,
+                       int, int, const int*, const int*, int, int*,
+                       hipStream_t);
+void launch_cache_free(int*, int*, int*, int*, int, int, int, int, const int*,
+                       int, hipStream_t);
+void launch_cache_compact(int*, int*, int*, int*, int, int, int, int, void*,
+                          int, long, int*, hipStream_t);
+void launch_cache_copy(const int*, const int*, int, void*, int, int, long,
+                       int*, hipStream_t);
+void launch_cache_extend(int*, int*, int*, int*, int, int, int, int,
+                         const int*, const int*, int, int, int*, hipStream_t);
+void launch_cache_write(int*, int*, int*, int*, int, int, int, int, const int*,
+                        const int*, int, int, void*, void*, const void*,
+                        const void*, int, int, long, long, long, long,
+                        hipStream_t);
+int paged_attn_pieces(int, int, int, int);
+void launch_paged_attn(const void*, long, long, const void*, const void*,
+                       const long*, const long*, const int*, const int*,
+                       const int*, int, int, int, int, int, int, int, int, int,
+                       void*, float*, float*, float, bool, hipStream_t);
+
 namespace {
 
 hipStream_t cur_stream() {
@@ -830,6 +851,227 @@ std::vector<torch::Tensor> packed_attn_bwd(
   return {dq, dk, dv};
 }
 
+// ------------------------------------------------------------- paged cache
+// pages [layers, 2, P, groups, page, d]; refs [P], tables [slots, W], lengths
+// [slots] and status [1] int32, all on one GPU and contiguous
+struct CacheRefs {
+  int *refs, *tables, *lengths, *status;
+  int pages, slots, width, page, planes, groups, token;
+  void* data;
+};
+
+void check_ints(const torch::Tensor& t, const torch::Tensor& like, int dim,
+                const char* name) {
+  TORCH_CHECK(t.device() == like.device() && t.dim() == dim &&
+                  t.scalar_type() == torch::kInt32 && t.is_contiguous(),
+              name, " must be a contiguous int32 tensor on the cache's GPU");
+}
+
+CacheRefs cache_refs(const torch::Tensor& pages, const torch::Tensor& refs,
+                     const torch::Tensor& tables, const torch::Tensor& lengths,
+                     const torch::Tensor& status) {
+  TORCH_CHECK(pages.is_cuda() && pages.dim() == 6 && pages.size(1) == 2 &&
+                  pages.is_contiguous() &&
+                  reinterpret_cast<uintptr_t>(pages.data_ptr()) % 16 == 0,
+              "pages must be [layers, 2, P, groups, page, d], contiguous, on "
+              "the GPU");
+  check_ints(refs, pages, 1, "ref_counts");
+  check_ints(tables, pages, 2, "page_tables");
+  check_ints(lengths, pages, 1, "lengths");
+  check_ints(status, pages, 1, "status");
+  const long token = pages.size(5) * pages.element_size();
+  TORCH_CHECK(refs.numel() == pages.size(2) &&
+                  lengths.numel() == tables.size(0) && status.numel() > 0 &&
+                  token % 16 == 0 && pages.size(2) < (1l << 30) &&
+                  tables.size(0) <= (1l << 18) && tables.size(1) < (1l << 30),
+              "the cache's tensors do not fit each other");
+  return {refs.data_ptr<int>(),    tables.data_ptr<int>(),
+          lengths.data_ptr<int>(), status.data_ptr<int>(),
+          (int)pages.size(2),      (int)tables.size(0),
+          (int)tables.size(1),     (int)pages.size(4),
+          (int)pages.size(0) * 2,  (int)pages.size(3),
+          (int)token,              pages.data_ptr()};
+}
+
+#define CACHE_ARGS                                                       \
+  torch::Tensor pages, torch::Tensor refs, torch::Tensor tables,         \
+      torch::Tensor lengths, torch::Tensor status
+#define CACHE_TABLES c.refs, c.tables, c.lengths, c.status, c.pages, \
+                     c.slots, c.width, c.page
+
+void cache_fork(CACHE_ARGS, torch::Tensor src, torch::Tensor dst) {
+  const CacheRefs c = cache_refs(pages, refs, tables, lengths, status);
+  c10::DeviceGuard guard(pages.device());
+  check_ints(src, pages, 1, "src");
+  check_ints(dst, pages, 1, "dst");
+  const int n = (int)src.numel();
+  TORCH_CHECK(dst.numel() == n && n <= c.slots, "fork: src and dst must name "
+              "as many slots, at most all");
+  if (n == 0) return;
+  auto scratch = torch::empty({4 + 5l * n + (long)n * c.width}, refs.options());
+  launch_cache_fork(CACHE_TABLES, c.data, c.planes, c.groups, c.token,
+                    src.data_ptr<int>(), dst.data_ptr<int>(), n,
+                    scratch.data_ptr<int>(), cur_stream());
+}
+
+void cache_free(CACHE_ARGS, torch::Tensor list) {
+  const CacheRefs c = cache_refs(pages, refs, tables, lengths, status);
+  c10::DeviceGuard guard(pages.device());
+  check_ints(list, pages, 1, "slots");
+  if (list.numel() == 0) return;
+  launch_cache_free(CACHE_TABLES, list.data_ptr<int>(), (int)list.numel(),
+                    cur_stream());
+}
+
+void cache_compact(CACHE_ARGS) {
+  const CacheRefs c = cache_refs(pages, refs, tables, lengths, status);
+  c10::DeviceGuard guard(pages.device());
+  if (c.pages == 0) return;
+  auto scratch = torch::empty({2 + 4l * c.pages}, refs.options());
+  launch_cache_compact(CACHE_TABLES, c.data, c.planes,
+                       (long)c.groups * c.page * c.token,
+                       scratch.data_ptr<int>(), cur_stream());
+}
+
+void cache_copy(CACHE_ARGS, torch::Tensor src, torch::Tensor dst) {
+  const CacheRefs c = cache_refs(pages, refs, tables, lengths, status);
+  c10::DeviceGuard guard(pages.device());
+  check_ints(src, pages, 1, "src");
+  check_ints(dst, pages, 1, "dst");
+  TORCH_CHECK(dst.numel() == src.numel(),
+              "copy_pages: src and dst must name as many pages");
+  if (src.numel() == 0) return;
+  launch_cache_copy(src.data_ptr<int>(), dst.data_ptr<int>(),
+                    (int)src.numel(), c.data, c.planes, c.pages,
+                    (long)c.groups * c.page * c.token, c.status, cur_stream());
+}
+
+void cache_extend(CACHE_ARGS, torch::Tensor list,
+                  c10::optional<torch::Tensor> counts, long each) {
+  const CacheRefs c = cache_refs(pages, refs, tables, lengths, status);
+  c10::DeviceGuard guard(pages.device());
+  check_ints(list, pages, 1, "slots");
+  const int n = (int)list.numel();
+  TORCH_CHECK(n <= c.slots && each >= 0 && each < (1l << 30),
+              "extend: at most all slots, and a number of tokens");
+  if (counts.has_value()) {
+    check_ints(*counts, pages, 1, "num_tokens");
+    TORCH_CHECK(counts->numel() == n, "extend: a count for each slot");
+  }
+  if (n == 0) return;
+  auto scratch = torch::empty({(long)n + c.pages}, refs.options());
+  launch_cache_extend(CACHE_TABLES, list.data_ptr<int>(),
+                      counts.has_value() ? counts->data_ptr<int>() : nullptr,
+                      (int)each, n, scratch.data_ptr<int>(), cur_stream());
+}
+
+void cache_write(CACHE_ARGS, long layer, torch::Tensor k, torch::Tensor v,
+                 torch::Tensor list, c10::optional<torch::Tensor> cu) {
+  const CacheRefs c = cache_refs(pages, refs, tables, lengths, status);
+  c10::DeviceGuard guard(pages.device());
+  check_ints(list, pages, 1, "slots");
+  TORCH_CHECK(layer >= 0 && layer < pages.size(0), "write: no such layer");
+  TORCH_CHECK(k.device() == pages.device() && v.device() == pages.device() &&
+                  k.scalar_type() == pages.scalar_type() &&
+                  v.scalar_type() == pages.scalar_type() && k.dim() == 3 &&
+                  k.sizes() == v.sizes() && k.size(1) == c.groups &&
+                  k.size(2) == pages.size(5),
+              "write: key and value must be [tokens, groups, d] of the "
+              "cache's type, on its GPU");
+  const int n = (int)list.numel();
+  if (cu.has_value()) {
+    check_ints(*cu, pages, 1, "cu_seqlens");
+    TORCH_CHECK(cu->numel() == n + 1, "write: cu_seqlens must be [slots + 1]");
+  } else {
+    TORCH_CHECK(k.size(0) == n, "write: one token for each slot");
+  }
+  TORCH_CHECK(k.size(0) * (long)c.groups < (1l << 31), "write: too many tokens");
+  if (k.size(0) == 0 || c.groups == 0) return;
+  const long es = pages.element_size();
+  auto rows = [&](const torch::Tensor& t) {
+    const bool fits = t.stride(2) == 1 && t.stride(0) * es % 16 == 0 &&
+                      t.stride(1) * es % 16 == 0 &&
+                      reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    return fits ? t : t.contiguous();
+  };
+  auto kr = rows(k), vr = rows(v);
+  const long plane = (long)c.pages * c.groups * c.page * c.token;
+  char* keys = (char*)c.data + 2 * layer * plane;
+  launch_cache_write(CACHE_TABLES, list.data_ptr<int>(),
+                     cu.has_value() ? cu->data_ptr<int>() : nullptr, n,
+                     (int)k.size(0), keys, keys + plane, kr.data_ptr(),
+                     vr.data_ptr(), c.groups, c.token, kr.stride(0) * es,
+                     kr.stride(1) * es, vr.stride(0) * es, vr.stride(1) * es,
+                     cur_stream());
+}
+
+// ---------------------------------------------------------- paged attention
+torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
+                         torch::Tensor tables, torch::Tensor lengths,
+                         c10::optional<torch::Tensor> slots, long max_length,
+                         double scale) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3 && k.dim() == 4 &&
+                  v.sizes() == k.sizes() && k.device() == q.device() &&
+                  v.device() == q.device(),
+              "paged attention: q [b, heads, d], k and v [P, groups, page, d] "
+              "on one GPU");
+  TORCH_CHECK((q.scalar_type() == torch::kBFloat16 ||
+               q.scalar_type() == torch::kHalf) &&
+                  k.scalar_type() == q.scalar_type() &&
+                  v.scalar_type() == q.scalar_type(),
+              "paged attention: bf16 or fp16, one type");
+  const int b = (int)q.size(0), nh = (int)q.size(1), d = (int)q.size(2);
+  const int ng = (int)k.size(1), page = (int)k.size(2);
+  TORCH_CHECK((d == 64 || d == 128) && k.size(3) == d && ng > 0 &&
+                  nh % ng == 0 && page > 0 && page % 16 == 0 &&
+                  k.size(0) > 0 && k.size(0) < (1l << 30),
+              "paged attention: head size 64 or 128, pages of a multiple of "
+              "16 tokens, heads that the groups divide");
+  for (auto* t : {&k, &v})
+    TORCH_CHECK(t->stride(3) == 1 && t->stride(0) % 8 == 0 &&
+                    t->stride(1) % 8 == 0 && t->stride(2) % 8 == 0 &&
+                    reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
+                "paged attention: rows of a page must start on 16 bytes");
+  check_ints(tables, q, 2, "page_tables");
+  check_ints(lengths, q, 1, "lengths");
+  const int count = (int)tables.size(0);
+  TORCH_CHECK(lengths.numel() == count && count > 0 && tables.size(1) > 0 &&
+                  tables.size(1) * (long)page < (1l << 31),
+              "paged attention: a length for each table, and a table");
+  if (slots.has_value()) {
+    check_ints(*slots, q, 1, "slots");
+    TORCH_CHECK(slots->numel() == b, "paged attention: a slot for each row");
+  } else {
+    TORCH_CHECK(count == b, "paged attention: a table for each row");
+  }
+  c10::DeviceGuard guard(q.device());
+  auto o = torch::empty({b, nh, d}, q.options());
+  if (o.numel() == 0) return o;
+  const bool fits = q.stride(2) == 1 && q.stride(0) % 8 == 0 &&
+                    q.stride(1) % 8 == 0 &&
+                    reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0;
+  auto qr = fits ? q : q.contiguous();
+  const long most = std::min(max_length, tables.size(1) * (long)page);
+  const int pieces = paged_attn_pieces(b, nh, ng, (int)std::max(most, 1l));
+  torch::Tensor part;
+  if (pieces > 1)
+    part = torch::empty({(long)b * nh * pieces * (d + 1)},
+                        q.options().dtype(torch::kFloat32));
+  float* po = pieces > 1 ? part.data_ptr<float>() : nullptr;
+  const long ks[3] = {k.stride(0), k.stride(1), k.stride(2)};
+  const long vs[3] = {v.stride(0), v.stride(1), v.stride(2)};
+  launch_paged_attn(qr.data_ptr(), qr.stride(0), qr.stride(1), k.data_ptr(),
+                    v.data_ptr(), ks, vs, tables.data_ptr<int>(),
+                    lengths.data_ptr<int>(),
+                    slots.has_value() ? slots->data_ptr<int>() : nullptr, b,
+                    nh, ng, d, (int)k.size(0), page, (int)tables.size(1),
+                    count, pieces, o.data_ptr(), po,
+                    po ? po + (long)b * nh * pieces * d : nullptr,
+                    (float)scale, q.scalar_type() == torch::kHalf,
+                    cur_stream());
+  return o;
+}
+
 // --------------------------------------------------------------------- adam
 // states fp32 OR bf16 (precision-aware optimizer); params/grads fp32
 static bool adam_states_bf16(const torch::Tensor& m, const torch::Tensor& v) {
@@ -1010,6 +1252,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   mod.def("attn_fwd", &attn_fwd);
   mod.def("attn_fwd_ablate", &attn_fwd_ablate);
   mod.def("packed_attn_fwd", &packed_attn_fwd);
+  mod.def("cache_fork", &cache_fork);
+  mod.def("cache_free", &cache_free);
+  mod.def("cache_compact", &cache_compact);
+  mod.def("cache_copy", &cache_copy);
+  mod.def("cache_extend", &cache_extend);
+  mod.def("cache_write", &cache_write);
+  mod.def("paged_attn", &paged_attn);
   mod.def("packed_attn_bwd", &packed_attn_bwd);
   mod.def("attn_bwd", &attn_bwd);
   mod.def("colsum_accum", &colsum_accum);

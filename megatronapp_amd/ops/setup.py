@@ -26,6 +26,8 @@ SOURCES = [
     "wgrad.cpp",
     "attention.hip",
     "packed_attention.hip",
+    "paged_cache.hip",
+    "paged_attention.hip",
 ]
 
 

@@ -1,0 +1,305 @@
+"""Attention over paged sequences against the formula in 64 bits.
+
+Tolerances.  With h = eps / 2 of the type: P is rounded before the product
+with V and the output at the end, so |o - ref| <= h |ref| + h P|V|; sums,
+exponentials and the joining of pieces are in 32 bits, below 1e-5 of the
+terms, which 5% on top covers.  fp16 values below its normal range are off by
+up to 2^-25."""
+
+import math
+
+import pytest
+import torch
+
+from megatronapp_amd.core.inference.paged_attention import (SharedPrefix,
+                                                            paged_attention)
+
+gpu = pytest.mark.gpu
+
+
+def _state(lens, nh=4, ng=2, d=64, page=16, dtype=torch.bfloat16, spare=3,
+           device="cuda", seed=0, prefix=0):
+    """Rows of these lengths, all with the same `prefix` first tokens, their
+    pages in no order."""
+    g = torch.Generator().manual_seed(seed)
+    shared = prefix // page
+    need = [-(-n // page) for n in lens]
+    pages = shared + sum(max(0, x - shared) for x in need) + spare
+    order = torch.randperm(pages, generator=g).tolist()
+    tables, at = [], shared
+    width = max(need + [1]) + 1
+    for x in need:
+        own = max(0, x - shared)
+        row = order[:min(shared, x)] + order[at:at + own]
+        at += own
+        tables.append(row + [-1] * (width - len(row)))
+
+    def randn(*shape):
+        return torch.randn(*shape, generator=g).to(dtype).to(device)
+    return (randn(len(lens), nh, d) * 2.0, randn(pages, ng, page, d),
+            randn(pages, ng, page, d),
+            torch.tensor(tables, dtype=torch.int32, device=device),
+            torch.tensor(lens, dtype=torch.int32, device=device))
+
+
+def oracle(q, k, v, tables, lengths, scale=None, slots=None):
+    b, nh, d = q.shape
+    pages, ng, page = k.shape[:3]
+    h = torch.finfo(q.dtype).eps / 2
+    tiny = 2.0 ** -25 if q.dtype == torch.float16 else 0.0
+    scale = d ** -0.5 if scale is None else scale
+    out = torch.zeros(b, nh, d, dtype=torch.float64, device=q.device)
+    room = torch.zeros_like(out)
+    for i in range(b):
+        s = i if slots is None else int(slots[i])
+        seen = [(int(tables[s, t // page]), t % page)
+                for t in range(int(lengths[s]))]
+        seen = [x for x in seen if 0 <= x[0] < pages]
+        if not seen:
+            continue
+        p, t = (torch.tensor(x, device=q.device) for x in zip(*seen))
+        kk, vv = k[p, :, t].double(), v[p, :, t].double()   # [n, ng, d]
+        for x in range(nh):
+            z = kk[:, x * ng // nh] @ q[i, x].double() * scale
+            w = torch.softmax(z, 0)
+            y = vv[:, x * ng // nh]
+            out[i, x] = w @ y
+            room[i, x] = h * out[i, x].abs() + (h * w + tiny) @ y.abs() + tiny
+    return out, 1.05 * room
+
+
+def _near(got, want, name=""):
+    assert torch.isfinite(got).all(), name
+    off = ((got.double() - want[0]).abs() - want[1]).max()
+    assert off <= 0, (name, off.item())
+
+
+def _check(lens, scale=None, **kw):
+    s = _state(lens, **kw)
+    got = paged_attention(*s, softmax_scale=scale)
+    _near(got, oracle(*s, scale=scale), (lens, kw))
+    return s, got
+
+
+# ----------------------------------------------------------------- on the CPU
+def test_plain_matches_oracle():
+    s = _state([1, 0, 16, 40, 33], dtype=torch.float32, device="cpu", nh=6,
+               ng=2, d=8)
+    got = paged_attention(*s, softmax_scale=0.4)
+    out, _ = oracle(*s, scale=0.4)
+    # 32 bits: 41 terms and their exponentials, each off by a few 2^-24
+    assert (got.double() - out).abs().max() < 1e-5
+    slots = torch.tensor([3, 0, 9, -1], dtype=torch.int32)
+    got2 = paged_attention(s[0][:4], *s[1:], slots=slots, softmax_scale=0.4)
+    want = oracle(s[0][:2], *s[1:], scale=0.4, slots=[3, 0])[0]
+    assert (got2[:2].double() - want).abs().max() < 1e-5
+    assert (got2[2:] == 0).all()
+
+
+def test_plain_leaves_out_pages_out_of_the_pool():
+    q, k, v, tables, lengths = _state([40, 40, 16], dtype=torch.float32,
+                                      device="cpu", d=8)
+    tables[0, 1] = 999
+    tables[1, 0] = -7
+    tables[2, 0] = k.shape[0]
+    got = paged_attention(q, k, v, tables, lengths)
+    out, _ = oracle(q, k, v, tables, lengths)
+    assert (got.double() - out).abs().max() < 1e-5
+    assert (got[2] == 0).all()
+    lengths[0] = 100000          # longer than the table
+    lengths[1] = -4
+    got = paged_attention(q, k, v, tables, lengths)
+    assert torch.isfinite(got).all() and (got[1] == 0).all()
+
+
+def _refuse(message, device="cpu", **change):
+    q, k, v, tables, lengths = _state([20, 20], device=device)
+    args = dict(query=q, key_pages=k, value_pages=v, page_tables=tables,
+                lengths=lengths)
+    args.update({n: f(args) if callable(f) else f for n, f in change.items()})
+    with pytest.raises(ValueError, match=message):
+        paged_attention(**args)
+
+
+def test_refusals():
+    _refuse("must be", query=lambda a: a["query"][0])
+    _refuse("must be", value_pages=lambda a: a["value_pages"][:1])
+    _refuse("fit", query=lambda a: a["query"][:, :3])
+    _refuse("fit", query=lambda a: a["query"][..., :32])
+    _refuse("type", query=lambda a: a["query"].half())
+    _refuse("int32", lengths=lambda a: a["lengths"].long())
+    _refuse("int32", page_tables=lambda a: a["page_tables"][0])
+    _refuse("one length", lengths=lambda a: a["lengths"][:1])
+    _refuse("slot", slots=lambda a: a["lengths"][:1])
+    _refuse("positive", softmax_scale=0.0)
+    _refuse("16", key_pages=lambda a: a["key_pages"][:, :, :8],
+            value_pages=lambda a: a["value_pages"][:, :, :8])
+    _refuse("longer", shared_prefix=lambda a: SharedPrefix(
+        a["lengths"], a["lengths"], 1, 16))
+    _refuse("int32", shared_prefix=lambda a: SharedPrefix(
+        a["lengths"].long(), a["lengths"][:1], 1, 16))
+    _refuse("gradient", query=lambda a: a["query"].requires_grad_(True))
+
+
+# ----------------------------------------------------------------- on the GPU
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens", [
+    [1], [0], [15, 16, 17], [31, 32, 33, 0, 1], [127, 128, 129, 500]])
+def test_lengths(lens, dtype, d):
+    _check(lens, dtype=dtype, d=d)
+
+
+@gpu
+@pytest.mark.parametrize("page", [16, 32, 48, 64, 256])
+def test_page_sizes(page):
+    _check([1, page - 1, page, page + 1, 5 * page + 3], page=page, d=64)
+    _check([700, 2, 300], page=page, d=128, nh=8, ng=1)
+
+
+@gpu
+@pytest.mark.parametrize("nh,ng", [(1, 1), (3, 3), (16, 1), (24, 1), (40, 2),
+                                   (32, 8)])
+def test_head_layouts(nh, ng):
+    _check([70, 3, 190], nh=nh, ng=ng, d=64)
+    _check([70, 3, 190], nh=nh, ng=ng, d=128, scale=0.2)
+
+
+@gpu
+def test_long_rows_and_many_rows():
+    _check([9000, 31], nh=4, ng=2, d=128, page=64)
+    _check([(i * 37) % 90 for i in range(150)], nh=2, ng=1, d=64)
+
+
+@gpu
+def test_what_lies_behind_the_end_does_not_matter():
+    lens = [21, 40, 3]
+    s, want = _check(lens, d=64, spare=2)
+    k, v = s[1].clone(), s[2].clone()
+    used = torch.zeros(k.shape[0], k.shape[2], dtype=torch.bool)
+    for i, n in enumerate(lens):
+        for t in range(n):
+            used[int(s[3][i, t // 16]), t % 16] = True
+    hide = ~used.cuda()[:, None, :, None]
+    for x, by in ((k, math.nan), (v, math.inf), (v, math.nan)):
+        x.masked_fill_(hide, by)
+        assert torch.equal(paged_attention(s[0], k, v, *s[3:]), want)
+
+
+@gpu
+def test_pages_out_of_the_pool_and_lengths_out_of_range():
+    q, k, v, tables, lengths = _state([40, 40, 16], d=64)
+    tables[0, 1] = 999
+    tables[1, 0] = -7
+    tables[2, 0] = k.shape[0]
+    got = paged_attention(q, k, v, tables, lengths)
+    _near(got, oracle(q, k, v, tables, lengths))
+    assert (got[2] == 0).all()
+    lengths[0] = 1 << 30
+    lengths[1] = -4
+    got = paged_attention(q, k, v, tables, lengths)
+    assert torch.isfinite(got).all() and (got[1] == 0).all()
+    slots = torch.tensor([1, 77, -1], dtype=torch.int32, device="cuda")
+    assert (paged_attention(q, k, v, tables, lengths, slots=slots)
+            == 0).all()
+
+
+@gpu
+def test_slots_strides_and_layouts():
+    q, k, v, tables, lengths = _state([21, 200, 33, 0], d=64, nh=4, ng=2)
+    slots = torch.tensor([2, 2, 0, 3, 1, 1], dtype=torch.int32,
+                         device="cuda")
+    wide = torch.randn(6, 2, 4, 3, 64, device="cuda").bfloat16()
+    qv = wide[:, 1, :, 1]                      # a view
+    got = paged_attention(qv, k, v, tables, lengths, slots=slots)
+    want = oracle(qv, k, v, tables, lengths, slots=slots)
+    _near(got, want)
+    # tokens before heads in a page; a layer of a whole cache
+    kt = k.transpose(1, 2).contiguous().transpose(1, 2)
+    both = torch.stack([k, v])
+    assert torch.equal(paged_attention(qv, kt, both[1], tables, lengths,
+                                       slots=slots), got)
+    odd = torch.empty(6 * 4 * 64 + 1, device="cuda").bfloat16()[1:].view(
+        6, 4, 64)
+    odd.copy_(qv)
+    assert torch.equal(paged_attention(odd, k, v, tables, lengths,
+                                       slots=slots), got)
+    # the longest row that the host knows of only cuts the work
+    for most in (1, 50, 100000):
+        _near(paged_attention(qv, k, v, tables, lengths, slots=slots,
+                              max_length=most), want)
+
+
+@gpu
+def test_pages_far_into_a_large_cache():
+    """Offsets past 2^31 elements."""
+    d, page, ng = 128, 64, 8
+    pages = (1 << 31) // (page * ng * d) + 64
+    k = torch.zeros(pages, ng, page, d, dtype=torch.bfloat16, device="cuda")
+    q, ks, vs, tables, lengths = _state([100, 30], nh=8, ng=ng, d=d,
+                                        page=page, spare=0)
+    n = ks.shape[0]
+    want = paged_attention(q, ks, vs, tables, lengths)
+    for name, x in (("k", ks), ("v", vs)):
+        k[-n:] = x
+        far = torch.where(tables >= 0, tables + pages - n, tables).int()
+        if name == "k":
+            v = torch.zeros_like(k)
+            v[-n:] = vs
+    k[-n:] = ks
+    assert torch.equal(paged_attention(q, k, v, far, lengths), want)
+
+
+@gpu
+def test_another_stream_and_the_same_bits():
+    s, want = _check([900, 17, 260], nh=8, ng=2, d=128)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = paged_attention(*s)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
+@gpu
+def test_two_captured_graphs():
+    """Lengths and queries change between replays; two graphs of one pool
+    and eager calls go in turn."""
+    s = _state([300, 17, 260], nh=8, ng=2, d=64)
+    q, k, v, tables, lengths = s
+    graphs, outs = [], []
+    for most in (320, 40):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            paged_attention(*s, max_length=most)
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=graphs[0].pool() if graphs else None):
+            outs.append(paged_attention(*s, max_length=most))
+        graphs.append(g)
+    for i in range(6):
+        lengths.copy_(torch.tensor([300 - 40 * i, 17, i * 7],
+                                   dtype=torch.int32))
+        q.mul_(0.9)
+        want = oracle(*s)
+        graphs[i % 2].replay()
+        _near(outs[i % 2], want)
+        graphs[1 - i % 2].replay()
+        _near(outs[1 - i % 2], want)
+        _near(paged_attention(*s), want)
+
+
+@gpu
+def test_refusals_on_the_gpu():
+    q, k, v, tables, lengths = _state([20, 20], d=32)
+    with pytest.raises(ValueError, match="head size"):
+        paged_attention(q, k, v, tables, lengths)
+    q, k, v, tables, lengths = _state([20, 20])
+    with pytest.raises(ValueError, match="device"):
+        paged_attention(q, k, v, tables.cpu(), lengths)
+    with pytest.raises(ValueError, match="head size"):
+        paged_attention(q.float(), k.float(), v.float(), tables, lengths)
+    assert paged_attention(q[:0], k, v, tables[:1], lengths[:1],
+                           slots=lengths[:0]).shape == (0, 4, 64)
