@@ -77,6 +77,13 @@ def _paged_attention_plain(q, k, v, tables, lengths, slots, scale):
     return out.to(q.dtype)
 
 
+def _groups(prefix: Optional[SharedPrefix]):
+    if prefix is None or prefix.lengths.numel() == 0:
+        return None, None, 0, 0
+    return (prefix.rows.contiguous(), prefix.lengths.contiguous(),
+            int(prefix.max_rows), int(prefix.max_length))
+
+
 def paged_attention(query: torch.Tensor, key_pages: torch.Tensor,
                     value_pages: torch.Tensor, page_tables: torch.Tensor,
                     lengths: torch.Tensor,
@@ -102,9 +109,10 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor,
         raise ValueError(
             f"paged_attention: query {tuple(query.shape)} and pages "
             f"{tuple(key_pages.shape)} do not fit each other")
-    if key_pages.shape[2] < 16 or key_pages.shape[2] % 16:
+    page = key_pages.shape[2]
+    if page < 16 or page % 16 or (page > 512 and page & (page - 1)):
         raise ValueError("paged_attention: pages must hold a multiple of 16 "
-                         "tokens")
+                         "tokens, above 512 a power of two")
     if key_pages.dtype != query.dtype or value_pages.dtype != query.dtype or \
             not query.is_floating_point():
         raise ValueError("paged_attention: query and pages must share one "
@@ -154,4 +162,4 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor,
     return _ops.get_ops().paged_attn(
         query, key_pages, value_pages, page_tables.contiguous(),
         lengths.contiguous(), None if slots is None else slots.contiguous(),
-        most, scale)
+        most, *_groups(shared_prefix), scale)

@@ -137,11 +137,12 @@ void launch_cache_write(int*, int*, int*, int*, int, int, int, int, const int*,
                         const int*, int, int, void*, void*, const void*,
                         const void*, int, int, long, long, long, long,
                         hipStream_t);
-int paged_attn_pieces(int, int, int, int);
+void paged_attn_pieces(int, int, int, int, int, int, int, int*, int*);
 void launch_paged_attn(const void*, long, long, const void*, const void*,
                        const long*, const long*, const int*, const int*,
-                       const int*, int, int, int, int, int, int, int, int, int,
-                       void*, float*, float*, float, bool, hipStream_t);
+                       const int*, const int*, const int*, int, int, int, int,
+                       int, int, int, int, int, int, int, int, void*, float*,
+                       float*, float, bool, hipStream_t);
 
 namespace {
 
@@ -1009,7 +1010,9 @@ void cache_write(CACHE_ARGS, long layer, torch::Tensor k, torch::Tensor v,
 torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
                          torch::Tensor tables, torch::Tensor lengths,
                          c10::optional<torch::Tensor> slots, long max_length,
-                         double scale) {
+                         c10::optional<torch::Tensor> group_rows,
+                         c10::optional<torch::Tensor> group_lengths,
+                         long max_rows, long max_prefix, double scale) {
   TORCH_CHECK(q.is_cuda() && q.dim() == 3 && k.dim() == 4 &&
                   v.sizes() == k.sizes() && k.device() == q.device() &&
                   v.device() == q.device(),
@@ -1024,9 +1027,11 @@ torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
   const int ng = (int)k.size(1), page = (int)k.size(2);
   TORCH_CHECK((d == 64 || d == 128) && k.size(3) == d && ng > 0 &&
                   nh % ng == 0 && page > 0 && page % 16 == 0 &&
+                  (page <= 512 || (page & (page - 1)) == 0) &&
                   k.size(0) > 0 && k.size(0) < (1l << 30),
               "paged attention: head size 64 or 128, pages of a multiple of "
-              "16 tokens, heads that the groups divide");
+              "16 tokens (above 512 a power of two), heads that the groups "
+              "divide");
   for (auto* t : {&k, &v})
     TORCH_CHECK(t->stride(3) == 1 && t->stride(0) % 8 == 0 &&
                     t->stride(1) % 8 == 0 && t->stride(2) % 8 == 0 &&
@@ -1051,8 +1056,22 @@ torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
                     q.stride(1) % 8 == 0 &&
                     reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0;
   auto qr = fits ? q : q.contiguous();
-  const long most = std::min(max_length, tables.size(1) * (long)page);
-  const int pieces = paged_attn_pieces(b, nh, ng, (int)std::max(most, 1l));
+  const long room = tables.size(1) * (long)page;
+  int groups = 0, own, shared;
+  if (group_rows.has_value()) {
+    check_ints(*group_rows, q, 1, "shared_prefix.rows");
+    check_ints(*group_lengths, q, 1, "shared_prefix.lengths");
+    groups = (int)group_lengths->numel();
+    TORCH_CHECK(group_rows->numel() == groups + 1,
+                "paged attention: shared_prefix.rows must be one longer than "
+                "its lengths");
+  }
+  max_rows = std::max(1l, std::min(max_rows, (long)b));
+  paged_attn_pieces(b, nh, ng, (int)std::max(std::min(max_length, room), 1l),
+                    groups, (int)max_rows,
+                    (int)std::max(std::min(max_prefix, room), 0l), &own,
+                    &shared);
+  const int pieces = own + shared;
   torch::Tensor part;
   if (pieces > 1)
     part = torch::empty({(long)b * nh * pieces * (d + 1)},
@@ -1063,9 +1082,11 @@ torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
   launch_paged_attn(qr.data_ptr(), qr.stride(0), qr.stride(1), k.data_ptr(),
                     v.data_ptr(), ks, vs, tables.data_ptr<int>(),
                     lengths.data_ptr<int>(),
-                    slots.has_value() ? slots->data_ptr<int>() : nullptr, b,
-                    nh, ng, d, (int)k.size(0), page, (int)tables.size(1),
-                    count, pieces, o.data_ptr(), po,
+                    slots.has_value() ? slots->data_ptr<int>() : nullptr,
+                    groups ? group_rows->data_ptr<int>() : nullptr,
+                    groups ? group_lengths->data_ptr<int>() : nullptr, groups,
+                    (int)max_rows, b, nh, ng, d, (int)k.size(0), page,
+                    (int)tables.size(1), count, own, shared, o.data_ptr(), po,
                     po ? po + (long)b * nh * pieces * d : nullptr,
                     (float)scale, q.scalar_type() == torch::kHalf,
                     cur_stream());

@@ -8,6 +8,13 @@
 //   o = sum_i 2^(L_i - M) o_i / sum_i 2^(L_i - M),  M = max L_i
 // A row without tokens gives zeros.  A page number out of the pool leaves its
 // tokens out.
+//
+// Rows of a group begin with the same pages.  Their queries, for all heads of
+// a key head, are the rows of a matrix product over these pages, done once
+// for the group; what each row has of its own follows as above, and the
+// pieces of both are joined.  Both kinds of blocks are one launch: the
+// group's products are bound by the matrix units, the rows' own pages by
+// memory, and each fills what the other leaves.
 
 #include "attn_tiles.h"
 
@@ -20,6 +27,9 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int KEYS = 32;      // of one step of a wave
 constexpr int HEADS = 16;     // query heads of a block, of one key head
 
+constexpr int BM = 128;       // queries of a group's block, 32 a wave
+constexpr int BN = 64;        // keys of its step
+
 struct Cache {
   const unsigned short* k;
   const unsigned short* v;
@@ -28,14 +38,30 @@ struct Cache {
   const int* slots;           // [b], or the rows themselves
   long kp, kh, kt, vp, vh, vt;  // strides of pages, heads, tokens
   int pages, page, width, count;  // pages, tokens of one, table, its rows
+  unsigned long magic;        // 2^32 / (page / 16), rounded up
+};
+
+// Groups of rows that share their first pages; none: groups == 0.
+struct Groups {
+  const int* rows;            // [groups + 1]
+  const int* lengths;         // [groups]
+  int groups, b;
+  int tiles, pieces, blocks;  // blocks of BM queries, cuts of the prefix
 };
 
 struct Out {
   unsigned short* o;          // [b, nh, D], where there is one piece
   float* part;                // [b, nh, pieces, D]
   float* lse;                 // [b, nh, pieces]
-  int pieces;
+  int pieces;                 // of a row, the groups' ones last
 };
+
+// the page and the place in it of a token, at a multiple of 16
+__device__ __forceinline__ int page_of(const Cache& c, int token, int& in) {
+  const int i = (int)(((unsigned long)(token >> 4) * c.magic) >> 32);
+  in = token - i * c.page;
+  return i;
+}
 
 __device__ __forceinline__ int slot_at(const Cache& c, int row) {
   return c.slots ? c.slots[row] : row;
@@ -46,6 +72,48 @@ __device__ __forceinline__ int length_at(const Cache& c, int slot) {
   return (int)min((long)max(c.lengths[slot], 0), (long)c.width * c.page);
 }
 
+// tokens that a group's rows share: whole pages
+__device__ __forceinline__ int shared_of(const Cache& c, const Groups& gr,
+                                         int g) {
+  const int n = max(0, min(gr.lengths[g], c.width * c.page));
+  return n / c.page * c.page;
+}
+
+__device__ __forceinline__ int group_row(const Groups& gr, int g) {
+  return max(0, min(gr.rows[g], gr.b));
+}
+
+// tokens of the row that its group's blocks do: the last group that begins
+// at or before it, if it reaches so far
+__device__ __forceinline__ int shared_at(const Cache& c, const Groups& gr,
+                                         int row) {
+  if (gr.groups == 0) return 0;
+  int lo = 0, hi = gr.groups;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (gr.rows[mid] <= row) lo = mid; else hi = mid;
+  }
+  return row >= gr.rows[lo] && row < gr.rows[lo + 1] ? shared_of(c, gr, lo)
+                                                      : 0;
+}
+
+// A lane's worth of a table: 64 page numbers from `base` on, read ahead so
+// that no step waits for its page's number.
+struct Pages {
+  int id, base;
+};
+
+__device__ __forceinline__ int page_at(const Cache& c, const int* table,
+                                       int i, int lane, Pages& p, bool& ok) {
+  if (i < p.base || i >= p.base + WAVE) {
+    p.base = i;
+    p.id = table[min(i + lane, c.width - 1)];
+  }
+  const int page = __builtin_amdgcn_readlane(p.id, i - p.base);
+  ok = page >= 0 && page < c.pages;
+  return ok ? page : 0;
+}
+
 // An image of [KEYS][D] that only the transposing reads use: 32 lanes read
 // 32 bytes of 8 rows, so the pairs of 16-byte slots are what is permuted.
 template <int D>
@@ -53,30 +121,40 @@ __device__ __forceinline__ int pair_slot(int row, int slot) {
   return D == 128 ? slot ^ ((row & 7) << 1) : slot ^ (((row >> 1) & 3) << 1);
 }
 
+// --------------------------------------------------------- a row's own keys
 template <class T, int D>
-__global__ __launch_bounds__(BLOCK, 2) void paged_rows_kernel(
-    const unsigned short* __restrict__ q, long qb, long qh, Cache c, Out out,
-    int nh, int ng, float scale) {
+struct RowsLds {
+  // each wave's V rows; at the end the waves' sums
+  __attribute__((aligned(16))) unsigned short v[4 * KEYS * D];
+  float m[4][HEADS], l[4][HEADS];
+};
+
+template <class T, int D>
+__device__ __forceinline__ void own_keys(const unsigned short* q, long qb,
+                                         long qh, const Cache& c,
+                                         const Groups& gr, const Out& out,
+                                         int nh, int ng, float scale,
+                                         unsigned block, RowsLds<T, D>& lds) {
   constexpr int NF = D / 32, ND = D / 16;
   constexpr int SLOTS = D / 8, PER = WAVE / SLOTS, NV = KEYS / PER;
-  // each wave's V rows; at the end the waves' sums
-  __shared__ __attribute__((aligned(16))) unsigned short v_lds[4 * KEYS * D];
-  __shared__ float m_lds[4][HEADS], l_lds[4][HEADS];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int rep = nh / ng, tiles = (rep + HEADS - 1) / HEADS;
-  const int hk = blockIdx.x % ng, ht = blockIdx.x / ng % tiles;
-  const int piece = blockIdx.x / ng / tiles % out.pieces;
-  const int row = blockIdx.x / ng / tiles / out.pieces;
+  const int pieces = out.pieces - gr.pieces;
+  const int hk = block % ng, ht = block / ng % tiles;
+  const int piece = block / ng / tiles % pieces;
+  const int row = block / ng / tiles / pieces;
   const int heads = min(HEADS, rep - ht * HEADS);
   const int head = hk * rep + ht * HEADS + min(n, heads - 1);
 
   const int slot = slot_at(c, row);
   const int len = length_at(c, slot);
-  // this piece's keys; pieces begin at pages' sixteenths
-  const int per = ((len + out.pieces - 1) / out.pieces + KEYS - 1) / KEYS * KEYS;
-  const int from = min(piece * per, len), to = min(from + per, len);
+  // this piece's keys
+  const int begin = min(shared_at(c, gr, row), len), own = len - begin;
+  const int per = ((own + pieces - 1) / pieces + KEYS - 1) / KEYS * KEYS;
+  const int from = begin + min(piece * per, own);
+  const int to = min(from + per, len);
   const int* table = c.tables + (long)max(0, min(slot, c.count - 1)) * c.width;
 
   typename T::x8 qf[NF];
@@ -88,7 +166,8 @@ __global__ __launch_bounds__(BLOCK, 2) void paged_rows_kernel(
 #pragma unroll
   for (int i = 0; i < ND; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, ms = 0.f, l = 0.f;
-  unsigned short* img = v_lds + wave * KEYS * D;
+  unsigned short* img = lds.v + wave * KEYS * D;
+  Pages ids = {0, -WAVE};
 
   typename T::x8 kn[2][NF];
   s16x8 vn[NV];
@@ -98,10 +177,10 @@ __global__ __launch_bounds__(BLOCK, 2) void paged_rows_kernel(
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int first = min(at + 16 * i, (to - 1) & ~15);
-      int page = __builtin_amdgcn_readfirstlane(table[first / c.page]);
-      okn[i] = page >= 0 && page < c.pages;
-      page = okn[i] ? page : 0;
-      const int in = first % c.page, last = to - 1 - first;
+      int in;
+      const int index = page_of(c, first, in);
+      const long page = page_at(c, table, index, lane, ids, okn[i]);
+      const int last = to - 1 - first;
       const unsigned short* kp = c.k + page * c.kp + hk * c.kh +
                                  (long)(in + min(n, last)) * c.kt + 8 * g;
 #pragma unroll
@@ -198,17 +277,17 @@ __global__ __launch_bounds__(BLOCK, 2) void paged_rows_kernel(
   l += __shfl_xor(l, 16, WAVE);
   l += __shfl_xor(l, 32, WAVE);
   if (g == 0) {
-    m_lds[wave][n] = m;
-    l_lds[wave][n] = l;
+    lds.m[wave][n] = m;
+    lds.l[wave][n] = l;
   }
   __syncthreads();             // the V rows are done with, too
   float mx = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) mx = fmaxf(mx, m_lds[w][n]);
+  for (int w = 0; w < 4; ++w) mx = fmaxf(mx, lds.m[w][n]);
   const float a =
       m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx);
-  // two waves at a time: [2][HEADS][D + 4] floats fit
-  float* sums = (float*)v_lds;
+  // [HEADS][D] floats, the waves' added one after the other
+  float* sums = (float*)lds.v;
   constexpr int ROW = D;
 #pragma unroll
   for (int turn = 0; turn < 4; ++turn) {
@@ -233,12 +312,12 @@ __global__ __launch_bounds__(BLOCK, 2) void paged_rows_kernel(
     const int hh = x / (D / 4), d = x % (D / 4) * 4;
     float mm = -INFINITY, ll = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, m_lds[w][hh]);
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, lds.m[w][hh]);
 #pragma unroll
     for (int w = 0; w < 4; ++w)
-      ll += m_lds[w][hh] == -INFINITY
+      ll += lds.m[w][hh] == -INFINITY
                 ? 0.f
-                : l_lds[w][hh] * __builtin_amdgcn_exp2f(m_lds[w][hh] - mm);
+                : lds.l[w][hh] * __builtin_amdgcn_exp2f(lds.m[w][hh] - mm);
     const float by = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
     f32x4 y = *(f32x4*)(sums + hh * ROW + (d ^ ((hh & 7) << 2)));
     const long r = (long)row * nh + hk * rep + ht * HEADS + hh;
@@ -255,20 +334,224 @@ __global__ __launch_bounds__(BLOCK, 2) void paged_rows_kernel(
   }
 }
 
-// a wave joins the pieces of two (D = 64: four) heads of a row
+// ------------------------------------------------------ a group's first keys
 template <class T, int D>
-__global__ __launch_bounds__(BLOCK) void paged_join_kernel(Out out,
+__device__ __forceinline__ void shared_keys(
+    const unsigned short* q, long qb, long qh, const Cache& c,
+    const Groups& gr, const Out& out, int nh, int ng, float scale,
+    unsigned block, unsigned short* img0, unsigned short* img1) {
+  constexpr int NF = D / 16, ND = D / 32;
+  constexpr int SLOTS = D / 8, PER = WAVE / SLOTS;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h = lane >> 5, n = lane & 31, rep = nh / ng;
+  const int hk = block % ng, piece = block / ng % gr.pieces;
+  const int g = block / ng / gr.pieces % gr.groups;
+  const int first_row = group_row(gr, g);
+  const int queries = (group_row(gr, g + 1) - first_row) * rep;
+  const int shared = shared_of(c, gr, g);
+  if (queries <= 0 || shared == 0) return;
+  const int per = ((shared + gr.pieces - 1) / gr.pieces + BN - 1) / BN * BN;
+  const int from = min(piece * per, shared), to = min(from + per, shared);
+  const int slot = max(0, min(slot_at(c, first_row), c.count - 1));
+  const int* table = c.tables + (long)slot * c.width;
+  const int turns = (to - from + BN - 1) / BN;
+  Pages ids = {0, -WAVE};
+
+  // as many blocks go round the group's queries as the host expects to need
+  for (int tile = block / ng / gr.pieces / gr.groups; tile * BM < queries;
+       tile += gr.tiles) {
+    const int x0 = tile * BM + wave * 32;
+    const int x = min(x0 + n, queries - 1);
+    const int row = first_row + x / rep, head = hk * rep + x % rep;
+    const int sees = min(length_at(c, slot_at(c, row)), to);
+    typename T::x8 qf[NF];
+    const unsigned short* src = q + row * qb + head * qh;
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+      qf[f] = *(const typename T::x8*)(src + 16 * f + 8 * h);
+    f32x16 acc[ND];
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+    float m = -INFINITY, ms = 0.f, l = 0.f;
+    // rows of a group as a rule see all of it
+    const bool all = __all(sees >= to);
+
+    int fine = 0, fine_next = 0;    // which sixteenths' pages are in the pool
+    auto fetch = [&](int t, unsigned short* img) {
+      long pg[4];
+      int in[4];
+      fine_next = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // keys behind the piece are read as its last sixteen, and masked
+        bool ok;
+        const int index =
+            page_of(c, min(from + t * BN + 16 * i, (to - 1) & ~15), in[i]);
+        pg[i] = page_at(c, table, index, lane, ids, ok);
+        fine_next |= (int)ok << i;
+      }
+#pragma unroll
+      for (int i = 0; i < BN / PER / 4; ++i) {
+        const int r0 = (i * 4 + wave) * PER, x = r0 >> 4;
+        const long page = x < 2 ? (x == 0 ? pg[0] : pg[1])
+                                : (x == 2 ? pg[2] : pg[3]);
+        const int base = x < 2 ? (x == 0 ? in[0] : in[1])
+                               : (x == 2 ? in[2] : in[3]);
+        const int r = r0 + lane / SLOTS;
+        const int col = 8 * slot_of<D>(r, lane % SLOTS);
+        const long at = base + (r & 15);
+        __builtin_amdgcn_global_load_lds(
+            (global_char*)(c.k + page * c.kp + hk * c.kh + at * c.kt + col),
+            (lds_char*)(img + r0 * D), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds(
+            (global_char*)(c.v + page * c.vp + hk * c.vh + at * c.vt + col),
+            (lds_char*)(img + (BN + r0) * D), 16, 0, 0);
+      }
+    };
+    auto step = [&](int t, const unsigned short* img) {
+      const int at = from + t * BN;
+      if (x0 >= queries) return;
+      f32x16 st[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st[u][r] = 0.f;
+        const int kr = 32 * u + tile_row(n);
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+          st[u] = T::mfma32(read_rows<T, D>(img, kr, f, h), qf[f], st[u]);
+      }
+      if (!all || at + BN > to || fine != 15) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (at + 32 * u + 16 * (r >> 3) + 8 * h + (r & 7) >= sees ||
+                !(fine >> (2 * u + (r >> 3)) & 1))
+              st[u][r] = -INFINITY;
+      }
+      float mt = st[0][0];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mt = fmaxf(mt, st[u][r]);
+      mt = half_max(mt) * scale;
+      if (__any(mt > m + 8.f)) {
+        const float mn = fmaxf(m, mt);
+        const float a = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        ms = mn == -INFINITY ? 0.f : mn;
+        l *= a;
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][r] *= a;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          st[u][r] = __builtin_amdgcn_exp2f(fmaf(st[u][r], scale, -ms));
+          l += st[u][r];
+        }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const typename T::x8 pf = pack8<T>(st[u], 8 * y);
+#pragma unroll
+          for (int i = 0; i < ND; ++i)
+            acc[i] = T::mfma32(
+                read_cols<T, D>(img + BN * D, 32 * u + 16 * y, i, lane), pf,
+                acc[i]);
+        }
+    };
+    auto turn = [&](int t, unsigned short* img, unsigned short* next) {
+      __builtin_amdgcn_s_waitcnt(0x0f70);         // vmcnt(0)
+      __syncthreads();
+      fine = fine_next;
+      if (t + 1 < turns) fetch(t + 1, next);
+      if (fine != 15) {       // what stands for a page out of the pool
+        for (int i = 0; i < 4; ++i)
+          if (!(fine >> i & 1))
+            for (int x = tid; x < 2 * D; x += BLOCK)
+              *(s16x8*)(img + (BN + 16 * i) * D + 8 * x) =
+                  s16x8{0, 0, 0, 0, 0, 0, 0, 0};
+        __syncthreads();
+      }
+      step(t, img);
+    };
+    __syncthreads();          // the images of the tile before are done with
+    if (turns > 0) fetch(0, img0);
+    for (int t = 0; t < turns; t += 2) {
+      turn(t, img0, img1);
+      if (t + 1 < turns) turn(t + 1, img1, img0);
+    }
+    if (x0 + n < queries) {
+      l = half_sum(l);
+      const float by = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+      const long r = ((long)row * nh + head) * out.pieces + out.pieces -
+                     gr.pieces + piece;
+      if (h == 0)
+        out.lse[r] = l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l);
+      float* dst = out.part + r * D + 4 * h;
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          f32x4 z = {acc[i][4 * y] * by, acc[i][4 * y + 1] * by,
+                     acc[i][4 * y + 2] * by, acc[i][4 * y + 3] * by};
+          *(f32x4*)(dst + 32 * i + 8 * y) = z;
+        }
+    }
+  }
+}
+
+template <class T, int D>
+__global__ __launch_bounds__(BLOCK, 2) void paged_rows_kernel(
+    const unsigned short* __restrict__ q, long qb, long qh, Cache c, Groups gr,
+    Out out, int nh, int ng, float scale) {
+  __shared__ RowsLds<T, D> lds;
+  own_keys<T, D>(q, qb, qh, c, gr, out, nh, ng, scale, blockIdx.x, lds);
+}
+
+template <class T, int D>
+__global__ __launch_bounds__(BLOCK, 2) void paged_groups_kernel(
+    const unsigned short* __restrict__ q, long qb, long qh, Cache c, Groups gr,
+    Out out, int nh, int ng, float scale) {
+  __shared__ union {
+    RowsLds<T, D> rows;
+    __attribute__((aligned(16))) unsigned short img[2][2 * BN * D];
+  } lds;
+  if (blockIdx.x < gr.blocks)
+    shared_keys<T, D>(q, qb, qh, c, gr, out, nh, ng, scale, blockIdx.x,
+                      lds.img[0], lds.img[1]);
+  else
+    own_keys<T, D>(q, qb, qh, c, gr, out, nh, ng, scale,
+                   blockIdx.x - gr.blocks, lds.rows);
+}
+
+// -------------------------------------------------------------------- joining
+template <class T, int D>
+__global__ __launch_bounds__(BLOCK) void paged_join_kernel(Cache c, Groups gr,
+                                                           Out out, int nh,
                                                            long heads) {
   constexpr int LANES = D / 4;
   const long r = ((long)blockIdx.x * BLOCK + threadIdx.x) / LANES;
   const int d = threadIdx.x % LANES * 4;
   if (r >= heads) return;
+  // a row that shares nothing has no pieces of a group
+  const int pieces =
+      shared_at(c, gr, (int)(r / nh)) ? out.pieces : out.pieces - gr.pieces;
   const float* lse = out.lse + r * out.pieces;
   const float* part = out.part + r * out.pieces * D + d;
   float mx = -INFINITY, l = 0.f;
-  for (int i = 0; i < out.pieces; ++i) mx = fmaxf(mx, lse[i]);
+  for (int i = 0; i < pieces; ++i) mx = fmaxf(mx, lse[i]);
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < out.pieces; ++i) {
+  for (int i = 0; i < pieces; ++i) {
     const float x = lse[i];
     if (x == -INFINITY) continue;
     const float w = __builtin_amdgcn_exp2f(x - mx);
@@ -284,40 +567,64 @@ __global__ __launch_bounds__(BLOCK) void paged_join_kernel(Out out,
 
 }  // namespace
 
-// pieces of a row, so that its blocks and the other rows' fill the card
-int paged_attn_pieces(int b, int nh, int ng, int max_length) {
+// How the work is cut: pieces of a row's own keys and of its group's.
+void paged_attn_pieces(int b, int nh, int ng, int max_length, int groups,
+                       int max_rows, int max_prefix, int* own, int* shared) {
   const long blocks = (long)b * ng * ((nh / ng + HEADS - 1) / HEADS);
+  *shared = 0;
+  long most = max_length;
+  if (groups > 0 && max_prefix > 0) {
+    const long tiles = ((long)max_rows * (nh / ng) + BM - 1) / BM;
+    const long units = (long)groups * tiles * ng;
+    const long cuts = std::min(512 / units, (long)max_prefix / 512);
+    *shared = (int)std::max(1l, std::min(cuts, 64l));
+    if (groups == 1) most = std::max(1l, most - max_prefix);
+  }
   const long fill = (1024 + blocks - 1) / blocks;
-  const long most = (max_length + 4 * KEYS - 1) / (4 * KEYS);
-  return (int)std::max(1l, std::min(std::min(fill, most), 64l));
+  most = (most + 4 * KEYS - 1) / (4 * KEYS);
+  *own = (int)std::max(1l, std::min(std::min(fill, most), 64l));
 }
 
 void launch_paged_attn(const void* q, long qb, long qh, const void* k,
                        const void* v, const long* ks, const long* vs,
                        const int* tables, const int* lengths, const int* slots,
-                       int b, int nh, int ng, int d, int pages, int page,
-                       int width, int count, int pieces, void* o, float* part,
-                       float* lse, float scale, bool fp16,
-                       hipStream_t stream) {
+                       const int* group_rows, const int* group_lengths,
+                       int groups, int max_rows, int b, int nh, int ng, int d,
+                       int pages, int page, int width, int count, int own,
+                       int shared, void* o, float* part, float* lse,
+                       float scale, bool fp16, hipStream_t stream) {
+  const unsigned long p16 = page / 16;
   const Cache c = {(const unsigned short*)k, (const unsigned short*)v, tables,
                    lengths, slots, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-                   pages, page, width, count};
-  const Out out = {(unsigned short*)o, part, lse, pieces};
+                   pages, page, width, count, ((1ul << 32) + p16 - 1) / p16};
+  const Out out = {(unsigned short*)o, part, lse, own + shared};
+  const int tiles =
+      (int)std::max(1l, ((long)max_rows * (nh / ng) + BM - 1) / BM);
+  const long first = shared ? (long)groups * tiles * ng * shared : 0;
   const long blocks =
-      (long)b * pieces * ng * ((nh / ng + HEADS - 1) / HEADS);
+      first + (long)b * own * ng * ((nh / ng + HEADS - 1) / HEADS);
   const long lanes = (long)b * nh * (d / 4);
   if (blocks * BLOCK >= 1l << 32 || lanes >= 1l << 32)
     throw std::runtime_error("paged attention: too many rows for one launch");
+  const Groups gr = {group_rows, group_lengths, shared ? groups : 0, b, tiles,
+                     shared, (int)first};
 #define RUN(T, DD)                                                          \
   do {                                                                      \
-    hipLaunchKernelGGL((paged_rows_kernel<T, DD>), dim3((unsigned)blocks),  \
-                       dim3(BLOCK), 0, stream, (const unsigned short*)q,    \
-                       qb, qh, c, out, nh, ng, scale * LOG2E);              \
+    if (shared)                                                             \
+      hipLaunchKernelGGL((paged_groups_kernel<T, DD>),                      \
+                         dim3((unsigned)blocks), dim3(BLOCK), 0, stream,    \
+                         (const unsigned short*)q, qb, qh, c, gr, out, nh,  \
+                         ng, scale * LOG2E);                                \
+    else                                                                    \
+      hipLaunchKernelGGL((paged_rows_kernel<T, DD>), dim3((unsigned)blocks),\
+                         dim3(BLOCK), 0, stream, (const unsigned short*)q,  \
+                         qb, qh, c, gr, out, nh, ng, scale * LOG2E);        \
     HIP_CHECK_LAUNCH();                                                     \
     if (part) {                                                             \
       hipLaunchKernelGGL((paged_join_kernel<T, DD>),                        \
                          dim3((unsigned)((lanes + BLOCK - 1) / BLOCK)),     \
-                         dim3(BLOCK), 0, stream, out, (long)b * nh);        \
+                         dim3(BLOCK), 0, stream, c, gr, out, nh,            \
+                         (long)b * nh);                                     \
       HIP_CHECK_LAUNCH();                                                   \
     }                                                                       \
   } while (0)

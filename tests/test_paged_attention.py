@@ -291,6 +291,145 @@ def test_two_captured_graphs():
         _near(paged_attention(*s), want)
 
 
+def _groups(rows, lengths, max_rows=None, max_length=None):
+    ends = list(rows)
+    return SharedPrefix(
+        torch.tensor(ends, dtype=torch.int32, device="cuda"),
+        torch.tensor(lengths, dtype=torch.int32, device="cuda"),
+        max_rows if max_rows is not None else
+        max(b - a for a, b in zip(ends[:-1], ends[1:])),
+        max_length if max_length is not None else max(lengths))
+
+
+def _grouped_state(sizes, prefixes, own, **kw):
+    """Rows of several groups, each on a prefix of its own."""
+    parts, at = [], 0
+    for i, (r, p) in enumerate(zip(sizes, prefixes)):
+        if r:
+            parts.append(_state([p + n for n in own[at:at + r]], prefix=p,
+                                seed=i, **kw))
+        at += r
+    width = max(x[3].shape[1] for x in parts)
+    tables, base = [], 0
+    for x in parts:
+        t = torch.where(x[3] >= 0, x[3] + base, x[3])
+        tables.append(torch.nn.functional.pad(t, (0, width - t.shape[1]),
+                                              value=-1))
+        base += x[1].shape[0]
+    return (torch.cat([x[0] for x in parts]), torch.cat([x[1] for x in parts]),
+            torch.cat([x[2] for x in parts]), torch.cat(tables).int(),
+            torch.cat([x[4] for x in parts]))
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_one_shared_prefix(dtype, d):
+    own = [1 + (i * 37) % 90 for i in range(50)]
+    s = _grouped_state([50], [640], own, dtype=dtype, d=d, nh=8, ng=2)
+    want = oracle(*s)
+    for most in (640, 1, 1 << 20):
+        _near(paged_attention(*s, shared_prefix=_groups([0, 50], [640], 50,
+                                                        most)), want)
+    # a host that knows too few rows
+    _near(paged_attention(*s, shared_prefix=_groups([0, 50], [640], 1, 640)),
+          want)
+    # a part of a page does not count
+    _near(paged_attention(*s, shared_prefix=_groups([0, 50], [639])), want)
+    # rows outside the group, one of them among them
+    _near(paged_attention(*s, shared_prefix=_groups([3, 41], [640])), want)
+
+
+@gpu
+@pytest.mark.parametrize("page", [16, 48, 64])
+def test_groups_of_rows(page):
+    sizes = [9, 1, 0, 6, 40]
+    prefixes = [page * 11, 0, page, page * 30, page * 3]
+    own = [(i * 53) % 200 for i in range(sum(sizes))]
+    s = _grouped_state(sizes, prefixes, own, page=page, d=64, nh=12, ng=3)
+    ends = [0, 9, 10, 10, 16, 56]
+    want = oracle(*s)
+    for rows in (40, 3):
+        _near(paged_attention(*s, shared_prefix=_groups(ends, prefixes,
+                                                        rows)), want)
+    s2 = _grouped_state(sizes[:2], prefixes[:2], own[:10], page=page, d=128,
+                        nh=48, ng=2)
+    _near(paged_attention(*s2, shared_prefix=_groups(ends[:3], prefixes[:2])),
+          oracle(*s2))
+
+
+@gpu
+def test_a_long_prefix_for_many_rows():
+    own = [1 + (i * 37) % 90 for i in range(70)]
+    s = _grouped_state([70], [6400], own, d=128, nh=8, ng=2, page=64)
+    _near(paged_attention(*s, shared_prefix=_groups([0, 70], [6400])),
+          oracle(*s))
+
+
+@gpu
+def test_groups_with_short_rows_and_bad_pages():
+    """Rows shorter than their group's prefix see their own length; bad pages
+    of the prefix are left out, whatever the pool's first page holds."""
+    own = [5] * 20
+    q, k, v, tables, lengths = _grouped_state([20], [320], own, d=64, nh=8)
+    lengths[3], lengths[7], lengths[19] = 40, 0, 320
+    tables[:, 4] = 9999
+    tables[:, 9] = -1
+    g = _groups([0, 20], [320])
+    want = oracle(q, k, v, tables, lengths)
+    got = paged_attention(q, k, v, tables, lengths, shared_prefix=g)
+    _near(got, want)
+    used = set(tables[:, :21].flatten().tolist())
+    if 0 not in used:
+        k[0], v[0] = math.nan, math.nan
+    else:       # the sequence's own first page: move it to the last
+        k, v = torch.cat([k, k[:1]]), torch.cat([v, v[:1]])
+        tables[tables == 0] = k.shape[0] - 1
+        k[0], v[0] = math.nan, math.nan
+    # one more page in the pool: numbers out of it stay out of it
+    assert torch.equal(paged_attention(q, k, v, tables, lengths,
+                                       shared_prefix=g), got)
+
+
+@gpu
+def test_groups_by_slots_in_a_graph():
+    """The groups' rows and lengths, and the rows' slots, change between
+    replays."""
+    own = [(i * 37) % 60 for i in range(12)]
+    s = _grouped_state([4, 8], [160, 64], own, d=64, nh=8, ng=2)
+    q, k, v, tables, lengths = s
+    slots = torch.arange(12, dtype=torch.int32, device="cuda")
+    g = _groups([0, 4, 12], [160, 64])
+
+    def run():
+        return paged_attention(q, k, v, tables, lengths, slots=slots,
+                               shared_prefix=g, max_length=224)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for ends, shared, order in (
+            ([0, 4, 12], [160, 64], range(12)),
+            ([0, 4, 12], [32, 16], range(12)),
+            ([0, 8, 12], [64, 160], list(range(4, 12)) + list(range(4))),
+            ([0, 0, 0], [160, 64], range(12))):
+        g.rows.copy_(torch.tensor(ends, dtype=torch.int32))
+        g.lengths.copy_(torch.tensor(shared, dtype=torch.int32))
+        slots.copy_(torch.tensor(list(order), dtype=torch.int32))
+        q.mul_(0.9)
+        want = oracle(*s, slots=slots)
+        graph.replay()
+        _near(out, want)
+        graph.replay()
+        _near(out, want)
+        _near(run(), want)
+
+
 @gpu
 def test_refusals_on_the_gpu():
     q, k, v, tables, lengths = _state([20, 20], d=32)
