@@ -8,6 +8,12 @@ positions + padding masks via DynamicInferenceContext), samples, and
 retires finished rows.  ``generate`` drives steps until a set of
 prompts drains, but ``add_request``/``step`` are the real API —
 requests can be added while others are mid-generation.
+
+With ``kv_page_size`` the cache is paged (PagedInferenceContext): waiting
+prompts that fit are prefilled as one packed stream, a decode step reads the
+pages where they lie, and ``add_parallel_requests`` continues one prompt
+several times over pages that are shared.  A request is admitted when the
+pages that it may come to need are left.
 """
 
 from __future__ import annotations
@@ -19,6 +25,7 @@ import torch
 
 from .sampling_params import SamplingParams
 from .dynamic_context import DynamicInferenceContext
+from .paged_context import PagedInferenceContext
 from .static_engine import InferenceRequest
 from .text_generation_controller import TextGenerationController
 from .. import parallel_state
@@ -34,31 +41,88 @@ class _Running:
     slot: int
     generated: List[int] = field(default_factory=list)
     pending_token: Optional[int] = None   # sampled, not yet decoded
+    family: int = -1                      # requests of one prompt
+
+
+@dataclass
+class _Family:
+    """Requests that continue one prompt, and the pages set aside for them:
+    those that all share, and the most that each may need beside them."""
+    members: int
+    shared_tokens: int
+    shared_pages: int
+    own_pages: int
 
 
 class DynamicInferenceEngine:
     def __init__(self, controller: TextGenerationController,
                  max_batch_size: int = 8,
-                 max_sequence_length: int = 2048):
+                 max_sequence_length: int = 2048,
+                 kv_page_size: Optional[int] = None,
+                 kv_num_pages: Optional[int] = None):
         self.controller = controller
         self.max_sequence_length = max_sequence_length
-        self.context = DynamicInferenceContext(max_batch_size,
-                                               max_sequence_length)
+        self.paged = kv_page_size is not None
+        self._families: Dict[int, _Family] = {}
         self.waiting: List[_Running] = []
         self.running: List[_Running] = []
         self.finished: Dict[int, InferenceRequest] = {}
         self._next_id = 0
         self._device = ("cuda" if torch.cuda.is_available() else "cpu")
+        if self.paged:
+            self.context = PagedInferenceContext.from_config(
+                controller.model.config, max_batch_size, max_sequence_length,
+                kv_page_size, kv_num_pages, self._device)
+            self._pages_left = self.context.cache.num_pages
+        else:
+            self.context = DynamicInferenceContext(max_batch_size,
+                                                   max_sequence_length)
 
     # ------------------------------------------------------------- intake
     def add_request(self, prompt: str,
                     sampling: Optional[SamplingParams] = None) -> int:
+        return self.add_parallel_requests(prompt, sampling, 1)[0]
+
+    def add_parallel_requests(self, prompt: str,
+                              sampling: Optional[SamplingParams] = None,
+                              num_samples: int = 1) -> List[int]:
+        """One prompt, continued ``num_samples`` times; the requests' ids.
+        With a paged cache the prompt is prefilled once and its pages are
+        shared."""
         sampling = sampling or SamplingParams()
+        if num_samples < 1:
+            raise ValueError("num_samples must be positive")
         toks = self.controller.tokenize_prompts([prompt])[0]
-        rid = self._next_id
-        self._next_id += 1
-        self.waiting.append(_Running(rid, prompt, toks, sampling, slot=-1))
-        return rid
+        ids = list(range(self._next_id, self._next_id + num_samples))
+        if self.paged:
+            self._families[ids[0]] = self._family_of(toks, sampling,
+                                                     num_samples)
+        self._next_id += num_samples
+        self.waiting += [_Running(rid, prompt, toks, sampling, slot=-1,
+                                  family=ids[0]) for rid in ids]
+        return ids
+
+    def _family_of(self, toks, sampling, members) -> _Family:
+        if not toks:
+            raise ValueError("a prompt without tokens")
+        # the last token that is generated never gets to the cache
+        longest = len(toks) + max(sampling.num_tokens_to_generate, 1) - 1
+        if longest > self.max_sequence_length:
+            raise ValueError(
+                f"{len(toks)} prompt tokens and "
+                f"{sampling.num_tokens_to_generate} to generate are more "
+                f"than max_sequence_length {self.max_sequence_length}")
+        page = self.context.cache.page_size
+        shared = len(toks) // page
+        family = _Family(members, shared * page, shared,
+                         -(-longest // page) - shared)
+        if members > self.context.max_slots or \
+                shared + members * family.own_pages > \
+                self.context.cache.num_pages:
+            raise ValueError(
+                f"{members} request(s) of {longest} tokens do not fit into "
+                f"the cache at once")
+        return family
 
     def has_unfinished_requests(self) -> bool:
         return bool(self.waiting or self.running)
@@ -70,7 +134,70 @@ class DynamicInferenceEngine:
             last = gather_from_tensor_model_parallel_region(last)
         return last
 
+    def _admit_paged(self):
+        """Prefills the waiting families that slots and pages are left for,
+        in order, as one packed stream; the members of each fork from its
+        first one."""
+        ctx = self.context
+        slots = [s for s in range(ctx.max_slots) if ctx.host_lengths[s] == 0]
+        batch: List[List[_Running]] = []
+        while self.waiting:
+            family = self._families[self.waiting[0].family]
+            pages = family.shared_pages + family.members * family.own_pages
+            if family.members > len(slots) or pages > self._pages_left:
+                break
+            members = self.waiting[:family.members]
+            del self.waiting[:family.members]
+            for req in members:
+                req.slot = slots.pop(0)
+            self._pages_left -= pages
+            batch.append(members)
+        if not batch:
+            return
+        prompts = [members[0].prompt_tokens for members in batch]
+        ctx.begin_prompts([members[0].slot for members in batch],
+                          [len(p) for p in prompts])
+        toks = torch.tensor([[t for p in prompts for t in p]],
+                            dtype=torch.long, device=self._device)
+        with torch.no_grad():
+            logits = self.controller.model(
+                toks, ctx.row_positions().unsqueeze(0), inference_context=ctx)
+        end = 0
+        for members, prompt in zip(batch, prompts):
+            end += len(prompt)
+            if len(members) > 1:
+                ctx.fork(members[0].slot, [r.slot for r in members[1:]])
+            new = self.controller.sample(
+                self._logits_last(logits[:, :end]).expand(len(members), -1),
+                members[0].sampling)
+            for req, tok in zip(members, new.tolist()):
+                req.pending_token = tok
+                self.running.append(req)
+
+    def _shared(self):
+        """How the running rows share pages: (rows, tokens) of each family;
+        members stand next to each other."""
+        groups, last = [], None
+        for req in self.running:
+            if req.family == last:
+                groups[-1][0] += 1
+            else:
+                groups.append([1, self._families[req.family].shared_tokens])
+                last = req.family
+        return [tuple(g) for g in groups]
+
+    def _release_pages(self, req: _Running):
+        family = self._families[req.family]
+        family.members -= 1
+        self._pages_left += family.own_pages
+        if family.members == 0:
+            self._pages_left += family.shared_pages
+            del self._families[req.family]
+
     def _admit(self):
+        if self.paged:
+            self._admit_paged()
+            return
         ctx = self.context
         while self.waiting:
             slot = ctx.free_slot()
@@ -96,6 +223,9 @@ class DynamicInferenceEngine:
         if include_pending and req.pending_token is not None:
             req.generated.append(req.pending_token)
         self.context.release(req.slot)
+        if self.paged:
+            self._release_pages(req)
+            self.context.cache.check()
         gen = torch.tensor(req.generated, dtype=torch.long)
         out = InferenceRequest(
             prompt=req.prompt, prompt_tokens=req.prompt_tokens,
@@ -127,7 +257,11 @@ class DynamicInferenceEngine:
             return
 
         ctx = self.context
-        ctx.set_active([r.slot for r in self.running], prefill=False)
+        slots = [r.slot for r in self.running]
+        if self.paged:
+            ctx.set_active(slots, shared=self._shared())
+        else:
+            ctx.set_active(slots, prefill=False)
         toks = torch.tensor([[r.pending_token] for r in self.running],
                             dtype=torch.long, device=self._device)
         pos = ctx.row_positions().unsqueeze(1)
@@ -152,7 +286,8 @@ class DynamicInferenceEngine:
 
 
 def get_dynamic_inference_engine(model, tokenizer, max_batch_size=8,
-                                 max_sequence_length=2048):
+                                 max_sequence_length=2048, kv_page_size=None,
+                                 kv_num_pages=None):
     return DynamicInferenceEngine(
         TextGenerationController(model, tokenizer, use_hip_graphs=False),
-        max_batch_size, max_sequence_length)
+        max_batch_size, max_sequence_length, kv_page_size, kv_num_pages)

@@ -184,6 +184,14 @@ class SelfAttention(MegatronModule):
                            inference_context._arange[:query.shape[0]])
                     q_pos_emb = q_pos_emb.index_select(0, idx)
                     k_pos_emb = k_pos_emb.index_select(0, idx)
+                elif getattr(inference_context, "is_paged", False):
+                    # a place for each token of packed prompts, or for each
+                    # row of a decode step
+                    idx = inference_context.row_positions()
+                    q_pos_emb = q_pos_emb.index_select(0, idx)
+                    if not inference_context.prefill:
+                        q_pos_emb = q_pos_emb.permute(1, 0, 2, 3)
+                    k_pos_emb = q_pos_emb
                 elif getattr(inference_context, "is_dynamic", False) and \
                         query.shape[0] == 1:
                     # continuous batching: per-ROW positions
@@ -198,6 +206,17 @@ class SelfAttention(MegatronModule):
                                           + key.shape[0]][-key.shape[0]:]
             query = apply_rotary_pos_emb(query, q_pos_emb, config=self.config)
             key = apply_rotary_pos_emb(key, k_pos_emb, config=self.config)
+
+        if getattr(inference_context, "is_paged", False):
+            with trace_scope("attention"):
+                core_attn_out = inference_context.attend(
+                    self.layer_number, query, key, value,
+                    softmax_scale=self.core_attention.effective_scale())
+            if tt is not None and tt.enabled(FlagType.ContextLayer,
+                                             self.layer_number):
+                tt.report(FlagType.ContextLayer, self.layer_number,
+                          core_attn_out)
+            return self.linear_proj(core_attn_out)
 
         attn_mask_type = self.attn_mask_type
         if inference_context is not None:

@@ -65,6 +65,10 @@ class DotProductAttention(nn.Module):
             config.attention_dropout if attention_dropout is None
             else attention_dropout)
 
+    def effective_scale(self) -> float:
+        """What multiplies q k^T before the softmax, all in all."""
+        return (self.scale_mask_softmax.scale or 1.0) / self.norm_factor
+
     def forward(self, query, key, value, attention_mask=None,
                 attn_mask_type=None, attention_bias=None, packed_seq_params=None):
         # q: [sq, b, np, hn]; k/v: [sk, b, ng, hn]
@@ -194,6 +198,9 @@ class FlashAttention(nn.Module):
         if query.shape[0] % 128 != 0 or key.shape[0] % 64 != 0:
             return False
         return hn in (64, 128) and query.dtype == torch.bfloat16
+
+    def effective_scale(self) -> float:
+        return self.softmax_scale
 
     def _packed(self, query, key, value, attention_mask, attn_mask_type,
                 attention_bias, packed_seq_params):
