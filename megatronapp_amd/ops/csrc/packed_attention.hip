@@ -223,11 +223,6 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_fwd_kernel(
     __builtin_amdgcn_s_waitcnt(0x0f70);         // vmcnt(0)
     __syncthreads();
     if (t + 1 < tiles) fetch(t + 1, next);
-    const int rows = s.sk - t * BN;
-    if (rows < BN) {
-      clear_rows<D, BN, BLOCK>(img + BN * D, rows, tid);
-      __syncthreads();
-    }
     step(t, img);
   };
   if (tiles > 0) fetch(0, kv0_lds);
@@ -367,11 +362,6 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_bwd_dq_kernel(
     __builtin_amdgcn_s_waitcnt(0x0f70);         // vmcnt(0)
     __syncthreads();
     if (t + 1 < tiles) fetch(t + 1, next);
-    const int rows = s.sk - t * BN;
-    if (rows < BN) {
-      clear_rows<D, BN, BLOCK>(img, rows, tid);
-      __syncthreads();
-    }
     step(t, img);
   };
   if (tiles > 0) fetch(0, kv0_lds);
@@ -386,21 +376,37 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_bwd_dq_kernel(
 }
 
 // dK and dV: rows of keys, over the queries that see them, for each head of
-// the group in turn (one block sums them all, so no atomics)
+// the group in turn (one block sums them all, so no atomics).
+//
+// At D = 128 a wave's two sums alone take 128 registers.  So that two waves
+// still fit a SIMD, K's and V's fragments stay in LDS, and eight waves work on
+// the 128 keys: four on the first 32 queries of a tile, four on the others,
+// whose sums are added at the end.
+template <int D>
+struct Dkv {
+  static constexpr int HALVES = D == 128 ? 2 : 1;
+  static constexpr int WAVES = 4 * HALVES;
+};
+
 template <class T, int D, bool CAUSAL>
-__global__ __launch_bounds__(BLOCK, 1) void packed_bwd_dkv_kernel(
+__global__ __launch_bounds__(Dkv<D>::WAVES * 64, 2) void packed_bwd_dkv_kernel(
     const unsigned short* __restrict__ q, const unsigned short* __restrict__ k,
     const unsigned short* __restrict__ v,
     const unsigned short* __restrict__ dout, const float* __restrict__ lse,
     const float* __restrict__ dot, unsigned short* __restrict__ dk,
     unsigned short* __restrict__ dv, Packing pk, int b, int nh, int ng,
     float scale, Strides qs, Strides ks, Strides vs, Strides os) {
+  constexpr int HALVES = Dkv<D>::HALVES, WAVES = Dkv<D>::WAVES;
+  constexpr bool KV_LDS = D == 128;
   // Q, dO, then the rows' lse and D
   constexpr int IMG = 2 * BN * D + 4 * BN;
   __shared__ __attribute__((aligned(16))) unsigned short qd0_lds[IMG];
   __shared__ __attribute__((aligned(16))) unsigned short qd1_lds[IMG];
+  __shared__ __attribute__((aligned(16)))
+  unsigned short kv_lds[KV_LDS ? 2 * BM * D : 8];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int part = wave & 3, half = wave >> 2;
   const int h = lane >> 5, n = lane & 31;
   Span s;
   const unsigned x = blockIdx.x % (b * ng);
@@ -408,12 +414,20 @@ __global__ __launch_bounds__(BLOCK, 1) void packed_bwd_dkv_kernel(
   const int bi = x / ng, hk = x % ng, rep = nh / ng;
   const float c = scale * LOG2E;
 
-  const int j0 = s.tile * BM + wave * 32;       // the wave's first key
+  const int j0 = s.tile * BM + part * 32;       // the wave's first key
   const int j = j0 + n;                         // the lane's key
   const long row = s.k0 + min(j, s.sk - 1);
   constexpr int NF = D / 16, ND = D / 32;
-  typename T::x8 kf[NF], vf[NF];
-  {
+  typename T::x8 kf[KV_LDS ? 1 : NF], vf[KV_LDS ? 1 : NF];
+  if constexpr (KV_LDS) {
+    const long from = s.k0 + s.tile * BM;
+    const int last = s.sk - 1 - s.tile * BM;
+    load_tile<D, BM, WAVES>(kv_lds, k + from * ks.t + bi * ks.b + hk * ks.h,
+                            ks.t, last, wave, lane);
+    load_tile<D, BM, WAVES>(kv_lds + BM * D,
+                            v + from * vs.t + bi * vs.b + hk * vs.h, vs.t,
+                            last, wave, lane);
+  } else {
     const unsigned short* ksrc = k + row * ks.t + bi * ks.b + hk * ks.h;
     const unsigned short* vsrc = v + row * vs.t + bi * vs.b + hk * vs.h;
 #pragma unroll
@@ -422,25 +436,33 @@ __global__ __launch_bounds__(BLOCK, 1) void packed_bwd_dkv_kernel(
       vf[f] = *(const typename T::x8*)(vsrc + 16 * f + 8 * h);
     }
   }
+  auto k_frag = [&](int f) __attribute__((always_inline)) {
+    if constexpr (KV_LDS) return read_rows<T, D>(kv_lds, 32 * part + n, f, h);
+    else return kf[f];
+  };
+  auto v_frag = [&](int f) __attribute__((always_inline)) {
+    if constexpr (KV_LDS)
+      return read_rows<T, D>(kv_lds + BM * D, 32 * part + n, f, h);
+    else return vf[f];
+  };
   // the first query that sees the block's first key
   const int ahead = CAUSAL ? s.sk - s.sq : 0;
   const int first = CAUSAL ? max(0, s.tile * BM - ahead) / BN : 0;
   const int per = max(0, (s.sq + BN - 1) / BN - first);
-  const int turns = per * rep;
 
   f32x16 ak[ND], av[ND];
 #pragma unroll
   for (int i = 0; i < ND; ++i) ak[i] = av[i] = zeros16();
 
-  auto fetch = [&](int it, unsigned short* img) {
-    const int head = hk * rep + it / per, at = (first + it % per) * BN;
-    const int last = s.sq - 1 - at;
+  // tile `at` of head hk * rep + r
+  auto fetch = [&](int r, int at, unsigned short* img) {
+    const int head = hk * rep + r, last = s.sq - 1 - at;
     const unsigned short* qp =
         q + (s.q0 + at) * qs.t + bi * qs.b + head * qs.h;
     const unsigned short* dp =
         dout + (s.q0 + at) * os.t + bi * os.b + head * os.h;
-    load_tile<D, BN, 4>(img, qp, qs.t, last, wave, lane);
-    load_tile<D, BN, 4>(img + BN * D, dp, os.t, last, wave, lane);
+    load_tile<D, BN, WAVES>(img, qp, qs.t, last, wave, lane);
+    load_tile<D, BN, WAVES>(img + BN * D, dp, os.t, last, wave, lane);
     // four bytes a lane: the rows' statistics, by one wave each
     if (wave < 2) {
       const float* src = (wave ? dot : lse) +
@@ -451,67 +473,96 @@ __global__ __launch_bounds__(BLOCK, 1) void packed_bwd_dkv_kernel(
           0, 0);
     }
   };
-  auto step = [&](int it, const unsigned short* img) {
-    const int at = (first + it % per) * BN;
-    if (j0 >= s.sk) return;
+  auto part_step = [&](int at, int u, const unsigned short* img)
+                       __attribute__((always_inline)) {
+    const int a0 = at + 32 * u;
+    // no key of the wave is seen by these rows
+    if (a0 >= s.sq || (CAUSAL && j0 > a0 + 31 + ahead)) return;
     const unsigned short* di = img + BN * D;
-    const float* sl = (const float*)(img + 2 * BN * D);
+    const float* sl = (const float*)(img + 2 * BN * D) + 32 * u + 8 * h;
     const float* sd = sl + BN;
+    f32x16 st = zeros16(), dp = zeros16();
+    const int qr = 32 * u + tile_row(n);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int a0 = at + 32 * u;
-      // no key of the wave is seen by these rows
-      if (a0 >= s.sq || (CAUSAL && j0 > a0 + 31 + ahead)) continue;
-      f32x16 st = zeros16(), dp = zeros16();
-      const int qr = 32 * u + tile_row(n);
+    for (int f = 0; f < NF; ++f)
+      st = T::mfma32(read_rows<T, D>(img, qr, f, h), k_frag(f), st);
 #pragma unroll
-      for (int f = 0; f < NF; ++f) {
-        st = T::mfma32(read_rows<T, D>(img, qr, f, h), kf[f], st);
-        dp = T::mfma32(read_rows<T, D>(di, qr, f, h), vf[f], dp);
-      }
+    for (int f = 0; f < NF; ++f)
+      dp = T::mfma32(read_rows<T, D>(di, qr, f, h), v_frag(f), dp);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int y = 16 * (r >> 3) + (r & 7);
+      st[r] = __builtin_amdgcn_exp2f(fmaf(st[r], c, -sl[y]));
+      dp[r] = st[r] * (dp[r] - sd[y]);
+    }
+    if (a0 + 32 > s.sq || (CAUSAL && j0 + 31 > a0 + ahead)) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int x = 32 * u + 16 * (r >> 3) + 8 * h + (r & 7);
-        st[r] = __builtin_amdgcn_exp2f(fmaf(st[r], c, -sl[x]));
-        dp[r] = st[r] * (dp[r] - sd[x]);
+        const int y = a0 + 16 * (r >> 3) + 8 * h + (r & 7);
+        if (y >= s.sq || (CAUSAL && j > y + ahead)) st[r] = dp[r] = 0.f;
       }
-      if (a0 + 32 > s.sq || (CAUSAL && j0 + 31 > a0 + ahead)) {
+    }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int x = at + 32 * u + 16 * (r >> 3) + 8 * h + (r & 7);
-          if (x >= s.sq || (CAUSAL && j > x + ahead)) st[r] = dp[r] = 0.f;
-        }
-      }
+    for (int y = 0; y < 2; ++y) {
+      const typename T::x8 pf = pack8<T>(st, 8 * y);
+      const typename T::x8 sf = pack8<T>(dp, 8 * y);
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const typename T::x8 pf = pack8<T>(st, 8 * x);
-        const typename T::x8 sf = pack8<T>(dp, 8 * x);
-#pragma unroll
-        for (int i = 0; i < ND; ++i) {
-          av[i] = T::mfma32(read_cols<T, D>(di, 32 * u + 16 * x, i, lane), pf,
-                            av[i]);
-          ak[i] = T::mfma32(read_cols<T, D>(img, 32 * u + 16 * x, i, lane), sf,
-                            ak[i]);
-        }
+      for (int i = 0; i < ND; ++i) {
+        av[i] = T::mfma32(read_cols<T, D>(di, 32 * u + 16 * y, i, lane), pf,
+                          av[i]);
+        ak[i] = T::mfma32(read_cols<T, D>(img, 32 * u + 16 * y, i, lane), sf,
+                          ak[i]);
       }
     }
   };
-  auto turn = [&](int it, unsigned short* img, unsigned short* next) {
+  // one tile is used while the next one comes in
+  int r1 = 0, t1 = 0;             // the next tile's head and number
+  auto turn = [&](int at, unsigned short* img, unsigned short* next)
+                  __attribute__((always_inline)) {
     __builtin_amdgcn_s_waitcnt(0x0f70);         // vmcnt(0)
     __syncthreads();
-    if (it + 1 < turns) fetch(it + 1, next);
-    const int rows = s.sq - (first + it % per) * BN;
-    if (rows < BN) {
-      clear_rows<D, BN, BLOCK>(img, rows, tid);
-      clear_rows<D, BN, BLOCK>(img + BN * D, rows, tid);
-      __syncthreads();
+    if (++t1 == per) {
+      t1 = 0;
+      ++r1;
     }
-    step(it, img);
+    if (r1 < rep) fetch(r1, (first + t1) * BN, next);
+    if (j0 >= s.sk) return;
+    if (HALVES == 2) {
+      part_step(at, half, img);
+    } else {
+      part_step(at, 0, img);
+      part_step(at, 1, img);
+    }
   };
-  if (turns > 0) fetch(0, qd0_lds);
-  for (int it = 0; it < turns; it += 2) {
-    turn(it, qd0_lds, qd1_lds);
-    if (it + 1 < turns) turn(it + 1, qd1_lds, qd0_lds);
+  if (per > 0) fetch(0, first * BN, qd0_lds);
+  while (per > 0 && r1 < rep) {
+    turn((first + t1) * BN, qd0_lds, qd1_lds);
+    if (r1 < rep) turn((first + t1) * BN, qd1_lds, qd0_lds);
+  }
+  if constexpr (HALVES == 2) {
+    // the second half's sums, handed over through the images
+    static_assert(sizeof(qd0_lds) >= 2 * 16 * ND * WAVE * 4, "room for them");
+    float* to = (float*)(part < 2 ? qd0_lds : qd1_lds) +
+                (part & 1) * 16 * ND * WAVE + lane;
+    auto hand_over = [&](f32x16(&acc)[ND]) __attribute__((always_inline)) {
+      __syncthreads();
+      if (half) {
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) to[(i * 16 + r) * WAVE] = acc[i][r];
+      }
+      __syncthreads();
+      if (!half) {
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][r] += to[(i * 16 + r) * WAVE];
+      }
+    };
+    hand_over(ak);
+    hand_over(av);
+    if (half) return;
   }
   if (j >= s.sk) return;
   const long at = ((row * b + bi) * ng + hk) * D;
@@ -525,7 +576,7 @@ __global__ __launch_bounds__(BLOCK, 1) void packed_bwd_dkv_kernel(
 // each sequence may end in a part of a tile
 dim3 grid_for(long heads, int total, int n) {
   const long blocks = heads * ((long)total / BM + n + 2);
-  if (blocks * BLOCK >= 1l << 32)
+  if (blocks * 512 >= 1l << 32)
     throw std::runtime_error("packed attention: too many tiles for one launch");
   return dim3((unsigned)blocks);
 }
@@ -603,7 +654,7 @@ void launch_packed_attn_bwd(const void* dout, const void* q, const void* k,
     const dim3 grid = grid_for((long)b * ng, tk, n);
 #define RUN(T, DD, CC)                                                       \
   hipLaunchKernelGGL((packed_bwd_dkv_kernel<T, DD, CC>),                     \
-                     grid, dim3(BLOCK), 0, stream,                   \
+                     grid, dim3(Dkv<DD>::WAVES * 64), 0, stream,             \
                      (const unsigned short*)q, (const unsigned short*)k,     \
                      (const unsigned short*)v, (const unsigned short*)dout,  \
                      lse, dot, (unsigned short*)dk, (unsigned short*)dv, pk, \
