@@ -92,9 +92,29 @@ typedef __attribute__((address_space(3))) char lds_char;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef const __attribute__((address_space(1))) char global_char;
 
-// ROWS rows of D elements from `src` (rows `stride` elements apart) into the
-// image at `dst`, by WAVES waves, straight from memory to LDS; rows behind
-// `last` (>= 0) are read as row `last`.  The caller waits for them.
+// 16 bytes a lane from `base` + `off` straight to LDS: base is the wave's, off
+// the lane's, so the address takes no vector instruction.
+__device__ __forceinline__ void load_lds16(unsigned short* dst,
+                                           const unsigned short* base,
+                                           unsigned off) {
+  __builtin_amdgcn_global_load_lds((global_char*)((const char*)base + off),
+                                   (lds_char*)dst, 16, 0, 0);
+}
+
+// The lane's place in what one instruction of `wave` loads of an image: rows
+// of `stride` elements apart (less than 2^27).
+template <int D>
+__device__ __forceinline__ unsigned lane_offset(long stride, int wave,
+                                                int lane) {
+  constexpr int SLOTS = D / 8, PER = WAVE / SLOTS;
+  const int row = wave * PER + lane / SLOTS;   // only its low bits count
+  return (unsigned)(lane / SLOTS) * (unsigned)stride * 2 +
+         16 * slot_of<D>(row, lane % SLOTS);
+}
+
+// ROWS rows of D elements from `src` into the image at `dst`, by WAVES waves
+// (a multiple of four); rows behind `last` (>= 0) are read as row `last`.
+// The caller waits for them.
 template <int D, int ROWS, int WAVES>
 __device__ __forceinline__ void load_tile(unsigned short* dst,
                                           const unsigned short* src,
@@ -102,7 +122,16 @@ __device__ __forceinline__ void load_tile(unsigned short* dst,
                                           int lane) {
   constexpr int SLOTS = D / 8;             // of a row
   constexpr int PER = WAVE / SLOTS;        // rows of one instruction
+  if (last >= ROWS - 1) {
+    const unsigned off = lane_offset<D>(stride, wave, lane);
 #pragma unroll
+    for (int i = 0; i < ROWS / PER / WAVES; ++i) {
+      const int first = (i * WAVES + wave) * PER;
+      load_lds16(dst + first * D, src + (long)first * stride, off);
+    }
+    return;
+  }
+#pragma unroll 1
   for (int i = 0; i < ROWS / PER / WAVES; ++i) {
     const int first = (i * WAVES + wave) * PER;
     const int row = first + lane / SLOTS;
@@ -111,16 +140,6 @@ __device__ __forceinline__ void load_tile(unsigned short* dst,
     __builtin_amdgcn_global_load_lds(
         (global_char*)p, (lds_char*)(dst + first * D), 16, 0, 0);
   }
-}
-
-// zeros for the image's rows from `from` on (a product's operand may hold
-// anything there, and nothing times NaN is NaN)
-template <int D, int ROWS, int THREADS>
-__device__ __forceinline__ void clear_rows(unsigned short* img, int from,
-                                           int tid) {
-  constexpr int SLOTS = D / 8;
-  for (int i = from * SLOTS + tid; i < ROWS * SLOTS; i += THREADS)
-    *(s16x8*)(img + i * 8) = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
 }
 
 // A operand of 32x32x16: row tile_row(n) + row0, elements 16f + 8h ..

@@ -763,7 +763,8 @@ torch::Tensor packed_rows(const torch::Tensor& t, const char* name,
   bool fits = t.stride(3) == 1 &&
               reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
   for (int i = 0; i < 3; ++i)
-    fits = fits && (t.stride(i) % 8 == 0 || t.size(i) <= 1);
+    fits = fits && (t.size(i) <= 1 ||
+                    (t.stride(i) % 8 == 0 && t.stride(i) < (1l << 27)));
   auto r = fits ? t : t.contiguous();
   for (int i = 0; i < 3; ++i)  // a single row's stride is never used
     strides[i] = r.size(i) <= 1 ? 0 : (long)r.stride(i);
@@ -1035,6 +1036,7 @@ torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
   for (auto* t : {&k, &v})
     TORCH_CHECK(t->stride(3) == 1 && t->stride(0) % 8 == 0 &&
                     t->stride(1) % 8 == 0 && t->stride(2) % 8 == 0 &&
+                    t->stride(2) < (1l << 27) &&
                     reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
                 "paged attention: rows of a page must start on 16 bytes");
   check_ints(tables, q, 2, "page_tables");

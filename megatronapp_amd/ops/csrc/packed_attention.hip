@@ -50,7 +50,30 @@ __device__ __forceinline__ void span_of(const int* cu, int n, int total, int i,
   len = max(to - from, 0);
 }
 
+// The wave's sum, as a scalar.  Moves within the vector unit: through LDS the
+// dozen sums of find_span() took longer than a tile's products.
+__device__ __forceinline__ int wave_sum(int v) {
+#define ADD(CTRL, ROWS) \
+  v += __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false)
+  ADD(0x111, 0xf);      // row_shr 1, 2, 4, 8: sums of 16 in their last lane
+  ADD(0x112, 0xf);
+  ADD(0x114, 0xf);
+  ADD(0x118, 0xf);
+  ADD(0x142, 0xa);      // row_bcast 15 into rows 1 and 3, 31 into 2 and 3
+  ADD(0x143, 0xc);
+#undef ADD
+  return __builtin_amdgcn_readlane(v, WAVE - 1);
+}
+
 // The `slot`-th tile of BM rows of the query (or key) stream.
+//
+// Under a causal mask a tile of queries has the more keys the further back it
+// lies, one of keys the more queries the further in front.  Where the
+// sequences fit a wave's lanes, tiles are handed out by that: level L holds
+// the L-th tile (from the other end for keys) of every sequence that has one,
+// and the highest level goes first, so that the last blocks to start are the
+// shortest.  8 documents of 45 to 2048 tokens, 16 heads of 128: CUs were idle
+// 37% of the forward's time in stream order (94 us).
 template <bool KEYS>
 __device__ __forceinline__ bool find_span(const Packing& pk, int slot,
                                           int lane, Span& s) {
@@ -61,32 +84,51 @@ __device__ __forceinline__ bool find_span(const Packing& pk, int slot,
     int from = 0, len = 0;
     if (i < pk.n + 2) span_of(cu, pk.n, total, i, from, len);
     const int tiles = (len + BM - 1) / BM;
-    int upto = tiles;
+    int w;                    // the lane whose sequence it is
+    if (pk.n + 2 <= WAVE) {
+      if (slot >= wave_sum(tiles)) return false;
+      // the highest level at or above which there are more tiles than `slot`
+      int lo = 0, hi = total / BM + 1;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (wave_sum(max(0, tiles - mid)) > slot) lo = mid; else hi = mid;
+      }
+      slot -= wave_sum(max(0, tiles - lo - 1));
+      const unsigned long long in = __ballot(tiles > lo);
+      const int rank = __popcll(in & ((1ull << lane) - 1));
+      w = __ffsll((unsigned long long)__ballot(tiles > lo && rank == slot)) -
+          1;
+      s.tile = KEYS ? __builtin_amdgcn_readlane(tiles, w) - 1 - lo : lo;
+    } else {
+      int upto = tiles;
 #pragma unroll
-    for (int off = 1; off < WAVE; off <<= 1) {
-      const int x = __shfl_up(upto, off, WAVE);
-      if (lane >= off) upto += x;
-    }
-    const unsigned long long hit = __ballot(upto > slot);
-    if (hit) {
-      const int w = __ffsll((unsigned long long)hit) - 1;
-      const int seq = base + w;
-      const int f = __builtin_amdgcn_readlane(from, w);
-      const int l = __builtin_amdgcn_readlane(len, w);
+      for (int off = 1; off < WAVE; off <<= 1) {
+        const int x = __shfl_up(upto, off, WAVE);
+        if (lane >= off) upto += x;
+      }
+      const unsigned long long hit = __ballot(upto > slot);
+      if (!hit) {
+        slot -= __builtin_amdgcn_readlane(upto, WAVE - 1);
+        continue;
+      }
+      w = __ffsll((unsigned long long)hit) - 1;
       s.tile = slot - (__builtin_amdgcn_readlane(upto, w) -
                        __builtin_amdgcn_readlane(tiles, w));
-      int of = 0, ol = 0;   // of the other stream
-      if (seq > 0 && seq <= pk.n) {
-        if (KEYS) span_of(pk.cu_q, pk.n, pk.tq, seq, of, ol);
-        else span_of(pk.cu_k, pk.n, pk.tk, seq, of, ol);
-      }
-      s.q0 = KEYS ? of : f;
-      s.sq = KEYS ? ol : l;
-      s.k0 = KEYS ? f : of;
-      s.sk = KEYS ? l : ol;
-      return true;
     }
-    slot -= __builtin_amdgcn_readlane(upto, WAVE - 1);
+    const int seq = base + w;
+    const int f = __builtin_amdgcn_readlane(from, w);
+    const int l = __builtin_amdgcn_readlane(len, w);
+    int of = 0, ol = 0;       // of the other stream
+    if (seq > 0 && seq <= pk.n) {
+      if (pk.cu_q == pk.cu_k && pk.tq == pk.tk) of = f, ol = l;
+      else if (KEYS) span_of(pk.cu_q, pk.n, pk.tq, seq, of, ol);
+      else span_of(pk.cu_k, pk.n, pk.tk, seq, of, ol);
+    }
+    s.q0 = KEYS ? of : f;
+    s.sq = KEYS ? ol : l;
+    s.k0 = KEYS ? f : of;
+    s.sk = KEYS ? l : ol;
+    return true;
   }
   return false;
 }
@@ -124,8 +166,7 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_fwd_kernel(
   const int h = lane >> 5, n = lane & 31;
   Span s;
   const unsigned x = blockIdx.x % (b * nh), slot = blockIdx.x / (b * nh);
-  // last tiles first: under a causal mask they have the most keys
-  if (!find_span<false>(pk, gridDim.x / (b * nh) - 1 - slot, lane, s)) return;
+  if (!find_span<false>(pk, slot, lane, s)) return;
   const int bi = x / nh, head = head_of(x % nh, ng, nh / ng);
   const int hk = head / (nh / ng);
 
@@ -285,8 +326,7 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_bwd_dq_kernel(
   const int h = lane >> 5, n = lane & 31;
   Span s;
   const unsigned x = blockIdx.x % (b * nh), slot = blockIdx.x / (b * nh);
-  // last tiles first: under a causal mask they have the most keys
-  if (!find_span<false>(pk, gridDim.x / (b * nh) - 1 - slot, lane, s)) return;
+  if (!find_span<false>(pk, slot, lane, s)) return;
   const int bi = x / nh, head = head_of(x % nh, ng, nh / ng);
   const int hk = head / (nh / ng);
   const float c = scale * LOG2E;
@@ -384,7 +424,8 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_bwd_dq_kernel(
 // whose sums are added at the end.
 template <int D>
 struct Dkv {
-  static constexpr int HALVES = D == 128 ? 2 : 1;
+  static constexpr int HALVES = 2;
+  static constexpr int BQ = D == 128 ? 64 : 128;   // queries of a tile
   static constexpr int WAVES = 4 * HALVES;
 };
 
@@ -397,9 +438,10 @@ __global__ __launch_bounds__(Dkv<D>::WAVES * 64, 2) void packed_bwd_dkv_kernel(
     unsigned short* __restrict__ dv, Packing pk, int b, int nh, int ng,
     float scale, Strides qs, Strides ks, Strides vs, Strides os) {
   constexpr int HALVES = Dkv<D>::HALVES, WAVES = Dkv<D>::WAVES;
+  constexpr int BQ = Dkv<D>::BQ;
   constexpr bool KV_LDS = D == 128;
   // Q, dO, then the rows' lse and D
-  constexpr int IMG = 2 * BN * D + 4 * BN;
+  constexpr int IMG = 2 * BQ * D + 4 * BQ;
   __shared__ __attribute__((aligned(16))) unsigned short qd0_lds[IMG];
   __shared__ __attribute__((aligned(16))) unsigned short qd1_lds[IMG];
   __shared__ __attribute__((aligned(16)))
@@ -447,8 +489,8 @@ __global__ __launch_bounds__(Dkv<D>::WAVES * 64, 2) void packed_bwd_dkv_kernel(
   };
   // the first query that sees the block's first key
   const int ahead = CAUSAL ? s.sk - s.sq : 0;
-  const int first = CAUSAL ? max(0, s.tile * BM - ahead) / BN : 0;
-  const int per = max(0, (s.sq + BN - 1) / BN - first);
+  const int first = CAUSAL ? max(0, s.tile * BM - ahead) / BQ : 0;
+  const int per = max(0, (s.sq + BQ - 1) / BQ - first);
 
   f32x16 ak[ND], av[ND];
 #pragma unroll
@@ -461,16 +503,17 @@ __global__ __launch_bounds__(Dkv<D>::WAVES * 64, 2) void packed_bwd_dkv_kernel(
         q + (s.q0 + at) * qs.t + bi * qs.b + head * qs.h;
     const unsigned short* dp =
         dout + (s.q0 + at) * os.t + bi * os.b + head * os.h;
-    load_tile<D, BN, WAVES>(img, qp, qs.t, last, wave, lane);
-    load_tile<D, BN, WAVES>(img + BN * D, dp, os.t, last, wave, lane);
+    load_tile<D, BQ, WAVES>(img, qp, qs.t, last, wave, lane);
+    load_tile<D, BQ, WAVES>(img + BQ * D, dp, os.t, last, wave, lane);
     // four bytes a lane: the rows' statistics, by one wave each
-    if (wave < 2) {
-      const float* src = (wave ? dot : lse) +
+    constexpr int EACH = BQ / WAVE;
+    if (wave < 2 * EACH) {
+      const float* src = (wave / EACH ? dot : lse) +
                          ((long)bi * nh + head) * pk.tq + s.q0 + at +
-                         min(lane, last);
+                         min(wave % EACH * WAVE + lane, last);
       __builtin_amdgcn_global_load_lds(
-          (global_char*)src, (lds_char*)(img + 2 * BN * D + 2 * BN * wave), 4,
-          0, 0);
+          (global_char*)src,
+          (lds_char*)(img + 2 * BQ * D + 2 * WAVE * wave), 4, 0, 0);
     }
   };
   auto part_step = [&](int at, int u, const unsigned short* img)
@@ -478,9 +521,9 @@ __global__ __launch_bounds__(Dkv<D>::WAVES * 64, 2) void packed_bwd_dkv_kernel(
     const int a0 = at + 32 * u;
     // no key of the wave is seen by these rows
     if (a0 >= s.sq || (CAUSAL && j0 > a0 + 31 + ahead)) return;
-    const unsigned short* di = img + BN * D;
-    const float* sl = (const float*)(img + 2 * BN * D) + 32 * u + 8 * h;
-    const float* sd = sl + BN;
+    const unsigned short* di = img + BQ * D;
+    const float* sl = (const float*)(img + 2 * BQ * D) + 32 * u + 8 * h;
+    const float* sd = sl + BQ;
     f32x16 st = zeros16(), dp = zeros16();
     const int qr = 32 * u + tile_row(n);
 #pragma unroll
@@ -525,19 +568,16 @@ __global__ __launch_bounds__(Dkv<D>::WAVES * 64, 2) void packed_bwd_dkv_kernel(
       t1 = 0;
       ++r1;
     }
-    if (r1 < rep) fetch(r1, (first + t1) * BN, next);
+    if (r1 < rep) fetch(r1, (first + t1) * BQ, next);
     if (j0 >= s.sk) return;
-    if (HALVES == 2) {
-      part_step(at, half, img);
-    } else {
-      part_step(at, 0, img);
-      part_step(at, 1, img);
-    }
+#pragma unroll
+    for (int u = 0; u < BQ / 32 / HALVES; ++u)
+      part_step(at, HALVES * u + half, img);
   };
-  if (per > 0) fetch(0, first * BN, qd0_lds);
+  if (per > 0) fetch(0, first * BQ, qd0_lds);
   while (per > 0 && r1 < rep) {
-    turn((first + t1) * BN, qd0_lds, qd1_lds);
-    if (r1 < rep) turn((first + t1) * BN, qd1_lds, qd0_lds);
+    turn((first + t1) * BQ, qd0_lds, qd1_lds);
+    if (r1 < rep) turn((first + t1) * BQ, qd1_lds, qd0_lds);
   }
   if constexpr (HALVES == 2) {
     // the second half's sums, handed over through the images

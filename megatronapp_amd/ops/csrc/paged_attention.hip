@@ -341,7 +341,7 @@ __device__ __forceinline__ void shared_keys(
     const Groups& gr, const Out& out, int nh, int ng, float scale,
     unsigned block, unsigned short* img0, unsigned short* img1) {
   constexpr int NF = D / 16, ND = D / 32;
-  constexpr int SLOTS = D / 8, PER = WAVE / SLOTS;
+  constexpr int PER = WAVE / (D / 8);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, n = lane & 31, rep = nh / ng;
@@ -356,6 +356,8 @@ __device__ __forceinline__ void shared_keys(
   const int slot = max(0, min(slot_at(c, first_row), c.count - 1));
   const int* table = c.tables + (long)slot * c.width;
   const int turns = (to - from + BN - 1) / BN;
+  const unsigned k_off = lane_offset<D>(c.kt, wave, lane);
+  const unsigned v_off = lane_offset<D>(c.vt, wave, lane);
   Pages ids = {0, -WAVE};
 
   // as many blocks go round the group's queries as the host expects to need
@@ -400,15 +402,11 @@ __device__ __forceinline__ void shared_keys(
                                 : (x == 2 ? pg[2] : pg[3]);
         const int base = x < 2 ? (x == 0 ? in[0] : in[1])
                                : (x == 2 ? in[2] : in[3]);
-        const int r = r0 + lane / SLOTS;
-        const int col = 8 * slot_of<D>(r, lane % SLOTS);
-        const long at = base + (r & 15);
-        __builtin_amdgcn_global_load_lds(
-            (global_char*)(c.k + page * c.kp + hk * c.kh + at * c.kt + col),
-            (lds_char*)(img + r0 * D), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds(
-            (global_char*)(c.v + page * c.vp + hk * c.vh + at * c.vt + col),
-            (lds_char*)(img + (BN + r0) * D), 16, 0, 0);
+        const long at = base + (r0 & 15);
+        load_lds16(img + r0 * D, c.k + page * c.kp + hk * c.kh + at * c.kt,
+                   k_off);
+        load_lds16(img + (BN + r0) * D,
+                   c.v + page * c.vp + hk * c.vh + at * c.vt, v_off);
       }
     };
     auto step = [&](int t, const unsigned short* img) {
