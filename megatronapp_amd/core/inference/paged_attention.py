@@ -77,29 +77,9 @@ def _paged_attention_plain(q, k, v, tables, lengths, slots, scale):
     return out.to(q.dtype)
 
 
-def _groups(prefix: Optional[SharedPrefix]):
-    if prefix is None or prefix.lengths.numel() == 0:
-        return None, None, 0, 0
-    return (prefix.rows.contiguous(), prefix.lengths.contiguous(),
-            int(prefix.max_rows), int(prefix.max_length))
-
-
-def paged_attention(query: torch.Tensor, key_pages: torch.Tensor,
-                    value_pages: torch.Tensor, page_tables: torch.Tensor,
-                    lengths: torch.Tensor,
-                    slots: Optional[torch.Tensor] = None,
-                    shared_prefix: Optional[SharedPrefix] = None,
-                    softmax_scale: Optional[float] = None,
-                    max_length: Optional[int] = None) -> torch.Tensor:
-    """query [b, heads, d] over key_pages and value_pages [P, groups, page,
-    d]; returns [b, heads, d].
-
-    Row i sees the first lengths[s] tokens of the pages page_tables[s], with
-    s = slots[i], or i without slots (int32, all on the query's device).
-    ``max_length`` is what the host knows about the longest row (by default
-    all that a table can hold); it chooses how the work is cut, not what is
-    computed.  A row of no tokens gives zeros; so does a slot out of range,
-    and a page number out of the pool leaves its tokens out."""
+def _check(query, key_pages, value_pages, page_tables, lengths, slots,
+           shared_prefix, scale):
+    """What the GPU's entry checks, for the CPU."""
     if query.dim() != 3 or key_pages.dim() != 4 or \
             value_pages.shape != key_pages.shape:
         raise ValueError("paged_attention: query must be [b, heads, d], key "
@@ -140,26 +120,45 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor,
             query.shape[0]:
         raise ValueError("paged_attention: one length for each table, one "
                          "table or slot for each row")
-    scale = (1.0 / math.sqrt(query.shape[2]) if softmax_scale is None
-             else float(softmax_scale))
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError("paged_attention: softmax_scale must be positive "
                          "and finite")
-    if torch.is_grad_enabled() and any(
-            t.requires_grad for t in (query, key_pages, value_pages)):
+
+
+def paged_attention(query: torch.Tensor, key_pages: torch.Tensor,
+                    value_pages: torch.Tensor, page_tables: torch.Tensor,
+                    lengths: torch.Tensor,
+                    slots: Optional[torch.Tensor] = None,
+                    shared_prefix: Optional[SharedPrefix] = None,
+                    softmax_scale: Optional[float] = None,
+                    max_length: Optional[int] = None) -> torch.Tensor:
+    """query [b, heads, d] over key_pages and value_pages [P, groups, page,
+    d]; returns [b, heads, d].
+
+    Row i sees the first lengths[s] tokens of the pages page_tables[s], with
+    s = slots[i], or i without slots (int32, all on the query's device).
+    ``max_length`` is what the host knows about the longest row (by default
+    all that a table can hold); it chooses how the work is cut, not what is
+    computed.  A row of no tokens gives zeros; so does a slot out of range,
+    and a page number out of the pool leaves its tokens out."""
+    if torch.is_grad_enabled() and (query.requires_grad
+                                    or key_pages.requires_grad
+                                    or value_pages.requires_grad):
         raise ValueError("paged_attention: has no gradient; call it under "
                          "torch.no_grad()")
-    room = page_tables.shape[1] * key_pages.shape[2]
-    most = room if max_length is None else max(1, min(int(max_length), room))
-    if not query.is_cuda:
-        return _paged_attention_plain(query, key_pages, value_pages,
-                                      page_tables, lengths, slots, scale)
-    if not paged_attention_supported(query):
-        _ops.get_ops()          # raises where the extension is missing
-        raise ValueError("paged_attention: on the GPU bf16 or fp16 with head "
-                         f"size 64 or 128, got {query.dtype}, "
-                         f"{query.shape[2]}")
-    return _ops.get_ops().paged_attn(
-        query, key_pages, value_pages, page_tables.contiguous(),
-        lengths.contiguous(), None if slots is None else slots.contiguous(),
-        most, *_groups(shared_prefix), scale)
+    if query.is_cuda:
+        rows = shared = None
+        max_rows = max_prefix = 0
+        if shared_prefix is not None:
+            rows, shared = shared_prefix.rows, shared_prefix.lengths
+            max_rows = shared_prefix.max_rows
+            max_prefix = shared_prefix.max_length
+        return _ops.get_ops().paged_attn(
+            query, key_pages, value_pages, page_tables, lengths, slots,
+            max_length, rows, shared, max_rows, max_prefix, softmax_scale)
+    scale = (1.0 / math.sqrt(query.shape[-1]) if softmax_scale is None
+             else float(softmax_scale))
+    _check(query, key_pages, value_pages, page_tables, lengths, slots,
+           shared_prefix, scale)
+    return _paged_attention_plain(query, key_pages, value_pages, page_tables,
+                                  lengths, slots, scale)

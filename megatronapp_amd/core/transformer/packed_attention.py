@@ -37,7 +37,7 @@ class _PackedAttnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, scale, causal):
         o, lse = _ops.get_ops().packed_attn_fwd(q, k, v, cu_q, cu_k, scale,
-                                                causal)
+                                                causal, True)
         ctx.save_for_backward(q, k, v, o, lse, cu_q, cu_k)
         ctx.scale = scale
         ctx.causal = causal
@@ -50,6 +50,40 @@ class _PackedAttnFn(torch.autograd.Function):
         dq, dk, dv = _ops.get_ops().packed_attn_bwd(
             do, q, k, v, o, lse, cu_q, cu_k, ctx.scale, ctx.causal)
         return dq, dk, dv, None, None, None, None
+
+
+def _check(query, key, value, cu_q, cu_k, scale):
+    """What the GPU's entry checks, for the CPU."""
+    if query.dim() not in (3, 4) or key.dim() != query.dim() \
+            or value.shape != key.shape:
+        raise ValueError(
+            "packed_attention: query, key, value must be [t, heads, hn] or "
+            f"[t, b, heads, hn], got {tuple(query.shape)}, "
+            f"{tuple(key.shape)}, {tuple(value.shape)}")
+    if key.shape[-1] != query.shape[-1] or key.shape[-2] < 1 or \
+            query.shape[-2] % key.shape[-2] or \
+            key.shape[1:-2] != query.shape[1:-2]:
+        raise ValueError(
+            f"packed_attention: query {tuple(query.shape)} and key "
+            f"{tuple(key.shape)} do not fit each other")
+    if key.dtype != query.dtype or value.dtype != query.dtype or \
+            not query.is_floating_point():
+        raise ValueError("packed_attention: query, key and value must share "
+                         "one floating type")
+    if key.device != query.device or value.device != query.device:
+        raise ValueError("packed_attention: query, key and value must be on "
+                         "one device")
+    for cu in (cu_q, cu_k):
+        if cu.dim() != 1 or cu.numel() < 1 or cu.shape != cu_q.shape or \
+                cu.dtype not in (torch.int32, torch.int64):
+            raise ValueError("packed_attention: cu_seqlens must be int32 or "
+                             "int64 [sequences + 1], the same for both")
+        if cu.device != query.device:
+            raise ValueError("packed_attention: cu_seqlens must be on the "
+                             "query's device")
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError("packed_attention: softmax_scale must be positive "
+                         "and finite")
 
 
 def _spans(cu, total):
@@ -99,55 +133,25 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor,
     shape.  ``cu_seqlens_kv`` defaults to ``cu_seqlens_q``; both are given on
     the query's device, and are not read by the host there, so ends that run
     out of the stream are cut off at it rather than refused."""
-    if query.dim() not in (3, 4) or key.dim() != query.dim() \
-            or value.shape != key.shape:
-        raise ValueError(
-            "packed_attention: query, key, value must be [t, heads, hn] or "
-            f"[t, b, heads, hn], got {tuple(query.shape)}, "
-            f"{tuple(key.shape)}, {tuple(value.shape)}")
-    if key.shape[-1] != query.shape[-1] or key.shape[-2] < 1 or \
-            query.shape[-2] % key.shape[-2] or \
-            key.shape[1:-2] != query.shape[1:-2]:
-        raise ValueError(
-            f"packed_attention: query {tuple(query.shape)} and key "
-            f"{tuple(key.shape)} do not fit each other")
-    if key.dtype != query.dtype or value.dtype != query.dtype or \
-            not query.is_floating_point():
-        raise ValueError("packed_attention: query, key and value must share "
-                         "one floating type")
-    if key.device != query.device or value.device != query.device:
-        raise ValueError("packed_attention: query, key and value must be on "
-                         "one device")
     cu_q = packed_seq_params.cu_seqlens_q
     cu_k = packed_seq_params.cu_seqlens_kv
     if cu_q is None:
         raise ValueError("packed_attention: cu_seqlens_q is missing")
+    if query.is_cuda:
+        if torch.is_grad_enabled() and (query.requires_grad
+                                        or key.requires_grad
+                                        or value.requires_grad):
+            return _PackedAttnFn.apply(query, key, value, cu_q, cu_k,
+                                       softmax_scale, causal)
+        return _ops.get_ops().packed_attn_fwd(query, key, value, cu_q, cu_k,
+                                              softmax_scale, causal, False)[0]
     cu_k = cu_q if cu_k is None else cu_k
-    for cu in (cu_q, cu_k):
-        if cu.dim() != 1 or cu.numel() < 1 or cu.shape != cu_q.shape or \
-                cu.dtype not in (torch.int32, torch.int64):
-            raise ValueError("packed_attention: cu_seqlens must be int32 or "
-                             "int64 [sequences + 1], the same for both")
-        if cu.device != query.device:
-            raise ValueError("packed_attention: cu_seqlens must be on the "
-                             "query's device")
     scale = (1.0 / math.sqrt(query.shape[-1]) if softmax_scale is None
              else float(softmax_scale))
-    if not (scale > 0.0 and math.isfinite(scale)):
-        raise ValueError("packed_attention: softmax_scale must be positive "
-                         "and finite")
+    _check(query, key, value, cu_q, cu_k, scale)
     flat = query.dim() == 3
     if flat:
         query, key, value = (x.unsqueeze(1) for x in (query, key, value))
-    if query.is_cuda:
-        if not packed_attention_supported(query):
-            _ops.get_ops()      # raises where the extension is missing
-            raise ValueError(
-                "packed_attention: on the GPU bf16 or fp16 with head size 64 "
-                f"or 128, got {query.dtype}, {query.shape[-1]}")
-        out = _PackedAttnFn.apply(query, key, value, cu_q.int().contiguous(),
-                                  cu_k.int().contiguous(), scale, causal)
-    else:
-        out = _packed_attention_plain(query, key, value, cu_q, cu_k, scale,
-                                      causal)
+    out = _packed_attention_plain(query, key, value, cu_q, cu_k, scale,
+                                  causal)
     return out.squeeze(1) if flat else out

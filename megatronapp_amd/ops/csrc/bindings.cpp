@@ -5,6 +5,8 @@
 
 #include <ATen/hip/HIPContext.h>
 
+#include <cmath>
+
 // launchers (norms.hip / elementwise.hip / rope.hip / softmax.hip / adam.hip /
 // attention.hip)
 void launch_rmsnorm_fwd(const void*, const void*, void*, float*, int, int,
@@ -751,23 +753,21 @@ std::vector<torch::Tensor> attn_fwd_ablate(torch::Tensor q, torch::Tensor k,
 }
 
 // --------------------------------------------------------- packed attention
-// [t, b, h, d] in 16 bits; views are read as they are where each row of a
-// head is adjacent and starts on 16 bytes, others are laid out first
-torch::Tensor packed_rows(const torch::Tensor& t, const char* name,
-                          const torch::Tensor& like, long* strides) {
-  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name,
-              " must be on the GPU of the query");
-  TORCH_CHECK(t.scalar_type() == like.scalar_type(), name,
-              " must have the query's type");
-  TORCH_CHECK(t.dim() == 4, name, " must be [t, b, h, d]");
-  bool fits = t.stride(3) == 1 &&
+// [t, b, h, d] (or [t, h, d], b = 1) in 16 bits; views are read as they are
+// where each row of a head is adjacent and starts on 16 bytes, others are laid
+// out first.  Arguments that cannot be are ValueErrors in Python.
+torch::Tensor packed_rows(const torch::Tensor& t, long* strides) {
+  const int h = (int)t.dim() - 2;
+  bool fits = t.stride(h + 1) == 1 &&
               reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-  for (int i = 0; i < 3; ++i)
+  for (int i = 0; i <= h; ++i)
     fits = fits && (t.size(i) <= 1 ||
                     (t.stride(i) % 8 == 0 && t.stride(i) < (1l << 27)));
   auto r = fits ? t : t.contiguous();
-  for (int i = 0; i < 3; ++i)  // a single row's stride is never used
-    strides[i] = r.size(i) <= 1 ? 0 : (long)r.stride(i);
+  // a single row's stride is never used
+  strides[0] = r.size(0) <= 1 ? 0 : (long)r.stride(0);
+  strides[1] = h == 1 || r.size(1) <= 1 ? 0 : (long)r.stride(1);
+  strides[2] = r.size(h) <= 1 ? 0 : (long)r.stride(h);
   return r;
 }
 
@@ -778,47 +778,82 @@ struct PackedShape {
 
 PackedShape packed_shape(const torch::Tensor& q, const torch::Tensor& k,
                          const torch::Tensor& v, const torch::Tensor& cu_q,
-                         const torch::Tensor& cu_k) {
-  TORCH_CHECK(q.is_cuda() && q.dim() == 4 && k.dim() == 4 &&
-                  k.sizes() == v.sizes(),
-              "packed attention: q, k, v must be [t, b, h, d] on the GPU");
-  TORCH_CHECK(q.scalar_type() == torch::kBFloat16 ||
-                  q.scalar_type() == torch::kHalf,
-              "packed attention: bf16 or fp16");
-  TORCH_CHECK(q.size(3) == 64 || q.size(3) == 128,
-              "packed attention: head size 64 or 128");
-  TORCH_CHECK(k.size(1) == q.size(1) && k.size(3) == q.size(3) &&
-                  k.size(2) > 0 && q.size(2) % k.size(2) == 0,
-              "packed attention: shapes of q and k do not fit");
-  TORCH_CHECK(q.size(0) < (1l << 30) && k.size(0) < (1l << 30),
-              "packed attention: too many tokens");
-  for (auto* c : {&cu_q, &cu_k})
-    TORCH_CHECK(c->device() == q.device() && c->dim() == 1 &&
-                    c->scalar_type() == torch::kInt32 && c->is_contiguous() &&
-                    c->numel() == cu_q.numel() && c->numel() > 0,
-                "packed attention: cu_seqlens must be int32 [n + 1] on the "
-                "GPU of the query");
-  return {(int)q.size(0), (int)k.size(0), (int)q.size(1), (int)q.size(2),
-          (int)k.size(2), (int)q.size(3), (int)cu_q.numel() - 1,
-          q.scalar_type() == torch::kHalf};
+                         const torch::Tensor& cu_k, double scale) {
+  const int dim = (int)q.dim(), h = dim - 2;
+  TORCH_CHECK_VALUE((dim == 3 || dim == 4) && k.dim() == dim &&
+                        k.sizes() == v.sizes(),
+                    "packed_attention: query, key, value must be [t, heads, "
+                    "hn] or [t, b, heads, hn], got ", q.sizes(), ", ",
+                    k.sizes(), ", ", v.sizes());
+  TORCH_CHECK_VALUE(k.size(h + 1) == q.size(h + 1) && k.size(h) > 0 &&
+                        q.size(h) % k.size(h) == 0 &&
+                        (dim == 3 || k.size(1) == q.size(1)),
+                    "packed_attention: query ", q.sizes(), " and key ",
+                    k.sizes(), " do not fit each other");
+  TORCH_CHECK_VALUE(k.scalar_type() == q.scalar_type() &&
+                        v.scalar_type() == q.scalar_type(),
+                    "packed_attention: query, key and value must share one "
+                    "floating type");
+  TORCH_CHECK_VALUE(q.is_cuda() && k.device() == q.device() &&
+                        v.device() == q.device(),
+                    "packed_attention: query, key and value must be on one "
+                    "device");
+  for (auto* c : {&cu_q, &cu_k}) {
+    TORCH_CHECK_VALUE(c->dim() == 1 && c->numel() > 0 &&
+                          c->numel() == cu_q.numel() &&
+                          (c->scalar_type() == torch::kInt32 ||
+                           c->scalar_type() == torch::kInt64),
+                      "packed_attention: cu_seqlens must be int32 or int64 "
+                      "[sequences + 1], the same for both");
+    TORCH_CHECK_VALUE(c->device() == q.device(),
+                      "packed_attention: cu_seqlens must be on the query's "
+                      "device");
+  }
+  TORCH_CHECK_VALUE(scale > 0 && std::isfinite((float)scale),
+                    "packed_attention: softmax_scale must be positive and "
+                    "finite");
+  const bool fp16 = q.scalar_type() == torch::kHalf;
+  TORCH_CHECK_VALUE((fp16 || q.scalar_type() == torch::kBFloat16) &&
+                        (q.size(h + 1) == 64 || q.size(h + 1) == 128),
+                    "packed_attention: on the GPU bf16 or fp16 with head size "
+                    "64 or 128, got ", q.scalar_type(), ", ", q.size(h + 1));
+  TORCH_CHECK_VALUE(q.size(0) < (1l << 30) && k.size(0) < (1l << 30),
+                    "packed_attention: too many tokens");
+  return {(int)q.size(0), (int)k.size(0), dim == 3 ? 1 : (int)q.size(1),
+          (int)q.size(h), (int)k.size(h), (int)q.size(h + 1),
+          (int)cu_q.numel() - 1, fp16};
 }
 
-std::vector<torch::Tensor> packed_attn_fwd(torch::Tensor q, torch::Tensor k,
-                                           torch::Tensor v, torch::Tensor cu_q,
-                                           torch::Tensor cu_k, double scale,
-                                           bool causal) {
-  const PackedShape s = packed_shape(q, k, v, cu_q, cu_k);
+torch::Tensor int32_row(const torch::Tensor& t) {
+  return (t.scalar_type() == torch::kInt32 ? t : t.to(torch::kInt32))
+      .contiguous();
+}
+
+// the output, and where a backward will follow the rows' log-sums
+std::vector<torch::Tensor> packed_attn_fwd(
+    torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor cu_q,
+    c10::optional<torch::Tensor> cu_kv, c10::optional<double> softmax_scale,
+    bool causal, bool want_lse) {
+  const torch::Tensor cu_k = cu_kv.has_value() ? *cu_kv : cu_q;
+  const double scale = softmax_scale.has_value()
+                           ? *softmax_scale
+                           : 1.0 / std::sqrt((double)q.size(-1));
+  const PackedShape s = packed_shape(q, k, v, cu_q, cu_k, scale);
   c10::DeviceGuard guard(q.device());
-  auto o = torch::empty({s.tq, s.b, s.nh, s.d}, q.options());
-  auto lse = torch::empty({s.b, s.nh, s.tq},
-                          q.options().dtype(torch::kFloat32));
+  auto o = torch::empty(q.sizes(), q.options());
+  torch::Tensor lse;
+  if (want_lse)
+    lse = torch::empty({s.b, s.nh, s.tq}, q.options().dtype(torch::kFloat32));
   if (o.numel() == 0) return {o, lse};
   long qs[3], ks[3], vs[3];
-  auto qr = packed_rows(q, "q", q, qs), kr = packed_rows(k, "k", q, ks),
-       vr = packed_rows(v, "v", q, vs);
+  auto qr = packed_rows(q, qs), kr = packed_rows(k, ks),
+       vr = packed_rows(v, vs);
+  const torch::Tensor iq = int32_row(cu_q),
+                      ik = cu_k.is_same(cu_q) ? iq : int32_row(cu_k);
   launch_packed_attn_fwd(qr.data_ptr(), kr.data_ptr(), vr.data_ptr(),
-                         o.data_ptr(), lse.data_ptr<float>(),
-                         cu_q.data_ptr<int>(), cu_k.data_ptr<int>(), s.n, s.tq,
+                         o.data_ptr(),
+                         want_lse ? lse.data_ptr<float>() : nullptr,
+                         iq.data_ptr<int>(), ik.data_ptr<int>(), s.n, s.tq,
                          s.tk, s.b, s.nh, s.ng, s.d, (float)scale, causal,
                          s.fp16, qs, ks, vs, cur_stream());
   return {o, lse};
@@ -826,28 +861,37 @@ std::vector<torch::Tensor> packed_attn_fwd(torch::Tensor q, torch::Tensor k,
 
 std::vector<torch::Tensor> packed_attn_bwd(
     torch::Tensor dout, torch::Tensor q, torch::Tensor k, torch::Tensor v,
-    torch::Tensor o, torch::Tensor lse, torch::Tensor cu_q, torch::Tensor cu_k,
-    double scale, bool causal) {
-  const PackedShape s = packed_shape(q, k, v, cu_q, cu_k);
+    torch::Tensor o, torch::Tensor lse, torch::Tensor cu_q,
+    c10::optional<torch::Tensor> cu_kv, c10::optional<double> softmax_scale,
+    bool causal) {
+  const torch::Tensor cu_k = cu_kv.has_value() ? *cu_kv : cu_q;
+  const double scale = softmax_scale.has_value()
+                           ? *softmax_scale
+                           : 1.0 / std::sqrt((double)q.size(-1));
+  const PackedShape s = packed_shape(q, k, v, cu_q, cu_k, scale);
   c10::DeviceGuard guard(q.device());
-  TORCH_CHECK(dout.sizes() == q.sizes() && o.sizes() == q.sizes() &&
-                  o.is_contiguous() && o.scalar_type() == q.scalar_type() &&
-                  lse.numel() == (long)s.b * s.nh * s.tq &&
-                  lse.is_contiguous() &&
-                  lse.scalar_type() == torch::kFloat32,
-              "packed attention: dout, o and lse must be the forward's");
-  auto dq = torch::empty({s.tq, s.b, s.nh, s.d}, q.options());
-  auto dk = torch::empty({s.tk, s.b, s.ng, s.d}, q.options());
-  auto dv = torch::empty({s.tk, s.b, s.ng, s.d}, q.options());
+  TORCH_CHECK_VALUE(dout.sizes() == q.sizes() && o.sizes() == q.sizes() &&
+                        dout.scalar_type() == q.scalar_type() &&
+                        dout.device() == q.device() && o.is_contiguous() &&
+                        o.scalar_type() == q.scalar_type() &&
+                        lse.numel() == (long)s.b * s.nh * s.tq &&
+                        lse.is_contiguous() &&
+                        lse.scalar_type() == torch::kFloat32,
+                    "packed_attention: dout, o and lse must be the forward's");
+  auto dq = torch::empty(q.sizes(), q.options());
+  auto dk = torch::empty(k.sizes(), q.options());
+  auto dv = torch::empty(k.sizes(), q.options());
   if (s.b == 0 || s.nh == 0) return {dq, dk, dv};
   auto dot = torch::empty_like(lse);
   long os[3], qs[3], ks[3], vs[3];
-  auto dr = packed_rows(dout, "dout", q, os), qr = packed_rows(q, "q", q, qs),
-       kr = packed_rows(k, "k", q, ks), vr = packed_rows(v, "v", q, vs);
+  auto dr = packed_rows(dout, os), qr = packed_rows(q, qs),
+       kr = packed_rows(k, ks), vr = packed_rows(v, vs);
+  const torch::Tensor iq = int32_row(cu_q),
+                      ik = cu_k.is_same(cu_q) ? iq : int32_row(cu_k);
   launch_packed_attn_bwd(
       dr.data_ptr(), qr.data_ptr(), kr.data_ptr(), vr.data_ptr(), o.data_ptr(),
       lse.data_ptr<float>(), dot.data_ptr<float>(), dq.data_ptr(),
-      dk.data_ptr(), dv.data_ptr(), cu_q.data_ptr<int>(), cu_k.data_ptr<int>(),
+      dk.data_ptr(), dv.data_ptr(), iq.data_ptr<int>(), ik.data_ptr<int>(),
       s.n, s.tq, s.tk, s.b, s.nh, s.ng, s.d, (float)scale, causal, s.fp16, os,
       qs, ks, vs, cur_stream());
   return {dq, dk, dv};
@@ -1008,48 +1052,82 @@ void cache_write(CACHE_ARGS, long layer, torch::Tensor k, torch::Tensor v,
 }
 
 // ---------------------------------------------------------- paged attention
+torch::Tensor paged_ints(const torch::Tensor& t, const torch::Tensor& q,
+                         int dim, const char* name) {
+  TORCH_CHECK_VALUE(t.dim() == dim && t.scalar_type() == torch::kInt32,
+                    "paged_attention: ", name, " must be an int32 tensor of ",
+                    dim, " dimension(s)");
+  TORCH_CHECK_VALUE(t.device() == q.device(),
+                    "paged_attention: all tensors must be on the query's "
+                    "device");
+  return t.contiguous();
+}
+
 torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
-                         torch::Tensor tables, torch::Tensor lengths,
-                         c10::optional<torch::Tensor> slots, long max_length,
-                         c10::optional<torch::Tensor> group_rows,
-                         c10::optional<torch::Tensor> group_lengths,
-                         long max_rows, long max_prefix, double scale) {
-  TORCH_CHECK(q.is_cuda() && q.dim() == 3 && k.dim() == 4 &&
-                  v.sizes() == k.sizes() && k.device() == q.device() &&
-                  v.device() == q.device(),
-              "paged attention: q [b, heads, d], k and v [P, groups, page, d] "
-              "on one GPU");
-  TORCH_CHECK((q.scalar_type() == torch::kBFloat16 ||
-               q.scalar_type() == torch::kHalf) &&
-                  k.scalar_type() == q.scalar_type() &&
-                  v.scalar_type() == q.scalar_type(),
-              "paged attention: bf16 or fp16, one type");
+                         torch::Tensor page_tables, torch::Tensor row_lengths,
+                         c10::optional<torch::Tensor> row_slots,
+                         c10::optional<long> max_length,
+                         c10::optional<torch::Tensor> prefix_rows,
+                         c10::optional<torch::Tensor> prefix_lengths,
+                         long max_rows, long max_prefix,
+                         c10::optional<double> softmax_scale) {
+  TORCH_CHECK_VALUE(q.dim() == 3 && k.dim() == 4 && v.sizes() == k.sizes(),
+                    "paged_attention: query must be [b, heads, d], key and "
+                    "value pages [P, groups, page, d]");
   const int b = (int)q.size(0), nh = (int)q.size(1), d = (int)q.size(2);
   const int ng = (int)k.size(1), page = (int)k.size(2);
-  TORCH_CHECK((d == 64 || d == 128) && k.size(3) == d && ng > 0 &&
-                  nh % ng == 0 && page > 0 && page % 16 == 0 &&
-                  (page <= 512 || (page & (page - 1)) == 0) &&
-                  k.size(0) > 0 && k.size(0) < (1l << 30),
-              "paged attention: head size 64 or 128, pages of a multiple of "
-              "16 tokens (above 512 a power of two), heads that the groups "
-              "divide");
+  TORCH_CHECK_VALUE(k.size(3) == d && ng > 0 && nh % ng == 0 &&
+                        k.size(0) > 0 && k.size(0) < (1l << 30),
+                    "paged_attention: query ", q.sizes(), " and pages ",
+                    k.sizes(), " do not fit each other");
+  TORCH_CHECK_VALUE(page >= 16 && page % 16 == 0 &&
+                        (page <= 512 || (page & (page - 1)) == 0),
+                    "paged_attention: pages must hold a multiple of 16 "
+                    "tokens, above 512 a power of two");
+  TORCH_CHECK_VALUE(k.scalar_type() == q.scalar_type() &&
+                        v.scalar_type() == q.scalar_type(),
+                    "paged_attention: query and pages must share one floating "
+                    "type");
+  TORCH_CHECK_VALUE(q.is_cuda() && k.device() == q.device() &&
+                        v.device() == q.device(),
+                    "paged_attention: all tensors must be on the query's "
+                    "device");
+  const bool fp16 = q.scalar_type() == torch::kHalf;
+  TORCH_CHECK_VALUE((fp16 || q.scalar_type() == torch::kBFloat16) &&
+                        (d == 64 || d == 128),
+                    "paged_attention: on the GPU bf16 or fp16 with head size "
+                    "64 or 128, got ", q.scalar_type(), ", ", d);
   for (auto* t : {&k, &v})
-    TORCH_CHECK(t->stride(3) == 1 && t->stride(0) % 8 == 0 &&
-                    t->stride(1) % 8 == 0 && t->stride(2) % 8 == 0 &&
-                    t->stride(2) < (1l << 27) &&
-                    reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
-                "paged attention: rows of a page must start on 16 bytes");
-  check_ints(tables, q, 2, "page_tables");
-  check_ints(lengths, q, 1, "lengths");
+    TORCH_CHECK_VALUE(t->stride(3) == 1 && t->stride(0) % 8 == 0 &&
+                          t->stride(1) % 8 == 0 && t->stride(2) % 8 == 0 &&
+                          t->stride(2) < (1l << 27) &&
+                          reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
+                      "paged_attention: the rows of a page must start on 16 "
+                      "bytes");
+  const auto tables = paged_ints(page_tables, q, 2, "page_tables");
+  const auto lengths = paged_ints(row_lengths, q, 1, "lengths");
   const int count = (int)tables.size(0);
-  TORCH_CHECK(lengths.numel() == count && count > 0 && tables.size(1) > 0 &&
-                  tables.size(1) * (long)page < (1l << 31),
-              "paged attention: a length for each table, and a table");
-  if (slots.has_value()) {
-    check_ints(*slots, q, 1, "slots");
-    TORCH_CHECK(slots->numel() == b, "paged attention: a slot for each row");
-  } else {
-    TORCH_CHECK(count == b, "paged attention: a table for each row");
+  torch::Tensor slots, group_rows, group_lengths;
+  if (row_slots.has_value()) slots = paged_ints(*row_slots, q, 1, "slots");
+  TORCH_CHECK_VALUE(lengths.numel() == count && count > 0 &&
+                        tables.size(1) > 0 &&
+                        tables.size(1) * (long)page < (1l << 31) &&
+                        (slots.defined() ? slots.numel() : count) == b,
+                    "paged_attention: one length for each table, one table or "
+                    "slot for each row");
+  const double scale = softmax_scale.has_value() ? *softmax_scale
+                                                 : 1.0 / std::sqrt((double)d);
+  TORCH_CHECK_VALUE(scale > 0 && std::isfinite((float)scale),
+                    "paged_attention: softmax_scale must be positive and "
+                    "finite");
+  int groups = 0, own, shared;
+  if (prefix_rows.has_value()) {
+    group_rows = paged_ints(*prefix_rows, q, 1, "shared_prefix.rows");
+    group_lengths = paged_ints(*prefix_lengths, q, 1, "shared_prefix.lengths");
+    groups = (int)group_lengths.numel();
+    TORCH_CHECK_VALUE(group_rows.numel() == groups + 1,
+                      "paged_attention: shared_prefix.rows must be one longer "
+                      "than its lengths");
   }
   c10::DeviceGuard guard(q.device());
   auto o = torch::empty({b, nh, d}, q.options());
@@ -1059,17 +1137,9 @@ torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
                     reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0;
   auto qr = fits ? q : q.contiguous();
   const long room = tables.size(1) * (long)page;
-  int groups = 0, own, shared;
-  if (group_rows.has_value()) {
-    check_ints(*group_rows, q, 1, "shared_prefix.rows");
-    check_ints(*group_lengths, q, 1, "shared_prefix.lengths");
-    groups = (int)group_lengths->numel();
-    TORCH_CHECK(group_rows->numel() == groups + 1,
-                "paged attention: shared_prefix.rows must be one longer than "
-                "its lengths");
-  }
+  const long longest = max_length.has_value() ? *max_length : room;
   max_rows = std::max(1l, std::min(max_rows, (long)b));
-  paged_attn_pieces(b, nh, ng, (int)std::max(std::min(max_length, room), 1l),
+  paged_attn_pieces(b, nh, ng, (int)std::max(std::min(longest, room), 1l),
                     groups, (int)max_rows,
                     (int)std::max(std::min(max_prefix, room), 0l), &own,
                     &shared);
@@ -1084,14 +1154,13 @@ torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
   launch_paged_attn(qr.data_ptr(), qr.stride(0), qr.stride(1), k.data_ptr(),
                     v.data_ptr(), ks, vs, tables.data_ptr<int>(),
                     lengths.data_ptr<int>(),
-                    slots.has_value() ? slots->data_ptr<int>() : nullptr,
-                    groups ? group_rows->data_ptr<int>() : nullptr,
-                    groups ? group_lengths->data_ptr<int>() : nullptr, groups,
+                    slots.defined() ? slots.data_ptr<int>() : nullptr,
+                    groups ? group_rows.data_ptr<int>() : nullptr,
+                    groups ? group_lengths.data_ptr<int>() : nullptr, groups,
                     (int)max_rows, b, nh, ng, d, (int)k.size(0), page,
                     (int)tables.size(1), count, own, shared, o.data_ptr(), po,
                     po ? po + (long)b * nh * pieces * d : nullptr,
-                    (float)scale, q.scalar_type() == torch::kHalf,
-                    cur_stream());
+                    (float)scale, fp16, cur_stream());
   return o;
 }
 

@@ -290,7 +290,7 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_fwd_kernel(
   if (!mine) return;
   l = half_sum(l);
   const float by = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  if (h == 0)
+  if (h == 0 && lse)
     lse[((long)bi * nh + head) * pk.tq + s.q0 + p] =
         l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
   unsigned short* dst = o + ((row * b + bi) * nh + head) * D;

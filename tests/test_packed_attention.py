@@ -173,7 +173,8 @@ def test_plain_three_dims_and_empty_places():
     (dict(scale=-1.0), "positive"), (dict(scale=math.inf), "finite"),
     (dict(cuk=torch.zeros(3, dtype=torch.int32)), "the same"),
 ])
-def test_refusals(change, message):
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_refusals(change, message, device):
     q = torch.zeros(change.get("q", (4, 4, 8)))
     k = torch.zeros(change.get("k", (4, 2, 8)),
                     dtype=change.get("kt", torch.float32))
@@ -181,8 +182,11 @@ def test_refusals(change, message):
     if k.shape[1] == 3 and "v" not in change:
         v = torch.zeros(k.shape)
     cu = change["cu"] if "cu" in change else _cu([4])
-    params = PackedSeqParams(cu_seqlens_q=cu,
-                             cu_seqlens_kv=change.get("cuk", cu))
+    cuk = change.get("cuk", cu)
+    if device == "cuda":
+        q, k, v = (x.cuda() for x in (q, k, v))
+        cu, cuk = (x if x is None else x.cuda() for x in (cu, cuk))
+    params = PackedSeqParams(cu_seqlens_q=cu, cu_seqlens_kv=cuk)
     with pytest.raises(ValueError, match=message):
         packed_attention(q, k, v, params, softmax_scale=change.get("scale"))
 

@@ -112,7 +112,7 @@ def test_plain_leaves_out_pages_out_of_the_pool():
     assert torch.isfinite(got).all() and (got[1] == 0).all()
 
 
-def _refuse(message, device="cpu", **change):
+def _refused(message, device, **change):
     q, k, v, tables, lengths = _state([20, 20], device=device)
     args = dict(query=q, key_pages=k, value_pages=v, page_tables=tables,
                 lengths=lengths)
@@ -121,7 +121,11 @@ def _refuse(message, device="cpu", **change):
         paged_attention(**args)
 
 
-def test_refusals():
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_refusals(device):
+    def _refuse(message, **change):
+        _refused(message, device, **change)
+
     _refuse("must be", query=lambda a: a["query"][0])
     _refuse("must be", value_pages=lambda a: a["value_pages"][:1])
     _refuse("fit", query=lambda a: a["query"][:, :3])
