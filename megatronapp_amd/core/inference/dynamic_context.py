@@ -68,10 +68,12 @@ class DynamicInferenceContext:
     # ----------------------------------------------------------- kv cache
     def _cache(self, layer: int, key: torch.Tensor, value: torch.Tensor):
         if layer not in self.key_value_memory_dict:
-            k = torch.empty(self.max_sequence_length, self.max_slots,
+            # zeros: a batch's window covers places that a row has not
+            # written, and no weight makes nothing of NaN there
+            k = torch.zeros(self.max_sequence_length, self.max_slots,
                             key.shape[2], key.shape[3], dtype=key.dtype,
                             device=key.device)
-            v = torch.empty(self.max_sequence_length, self.max_slots,
+            v = torch.zeros(self.max_sequence_length, self.max_slots,
                             value.shape[2], value.shape[3],
                             dtype=value.dtype, device=value.device)
             self.key_value_memory_dict[layer] = (k, v)

@@ -75,6 +75,21 @@ def test_same_tokens_as_without_pages(position, groups, use_flash):
     destroy()
 
 
+def test_places_not_written_do_not_matter_without_pages():
+    """The window of a batch covers places that its shorter rows have not
+    written: the cache's memory must not hold NaN there."""
+    from megatronapp_amd.core.inference.dynamic_context import (
+        DynamicInferenceContext)
+    dirty = [torch.full((64 * 2 * 2 * 8,), float("nan")) for _ in range(8)]
+    del dirty
+    ctx = DynamicInferenceContext(2, 64)
+    kv = torch.randn(5, 1, 2, 8)
+    ctx.set_active([1], prefill=True)
+    ctx.update_kv_cache(0, kv, kv)
+    for x in ctx.key_value_memory_dict[0]:
+        assert torch.isfinite(x).all()
+
+
 def test_samples_share_their_prompt():
     _cpu_only()
     model = _model()
