@@ -139,7 +139,7 @@ void launch_cache_write(int*, int*, int*, int*, int, int, int, int, const int*,
                         const int*, int, int, void*, void*, const void*,
                         const void*, int, int, long, long, long, long,
                         hipStream_t);
-void paged_attn_pieces(int, int, int, int, int, int, int, int*, int*);
+void paged_attn_pieces(int, int, int, int, int, int, int, long, int*, int*);
 void launch_paged_attn(const void*, long, long, const void*, const void*,
                        const long*, const long*, const int*, const int*,
                        const int*, const int*, const int*, int, int, int, int,
@@ -1139,9 +1139,10 @@ torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
   const long room = tables.size(1) * (long)page;
   const long longest = max_length.has_value() ? *max_length : room;
   max_rows = std::max(1l, std::min(max_rows, (long)b));
-  paged_attn_pieces(b, nh, ng, (int)std::max(std::min(longest, room), 1l),
+  paged_attn_pieces(b, nh, ng, d,
+                    (int)std::max(std::min(longest, room), 1l),
                     groups, (int)max_rows,
-                    (int)std::max(std::min(max_prefix, room), 0l), &own,
+                    std::min(std::max(max_prefix, 0l), 1l << 30), &own,
                     &shared);
   const int pieces = own + shared;
   torch::Tensor part;

@@ -146,21 +146,6 @@ __device__ __forceinline__ f32x16 zeros16() {
   return z;
 }
 
-// For the scheduler: N products whose operands take READS reads of LDS each,
-// with those of four products ahead all along (it waits for each read just
-// before the product else; forward of 10 prompts 90 -> 87 us).
-template <int N, int READS>
-__device__ __forceinline__ void reads_ahead() {
-  constexpr int MFMA = 0x008, DS_READ = 0x100;
-  __builtin_amdgcn_sched_group_barrier(DS_READ, 4 * READS, 0);
-#pragma unroll
-  for (int i = 0; i < N - 4; ++i) {
-    __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(DS_READ, READS, 0);
-  }
-  __builtin_amdgcn_sched_group_barrier(MFMA, 4, 0);
-}
-
 // head h of the block: heads of one group follow each other in steps of ng,
 // so that they run on one XCD (blocks go round the eight) and share its L2
 __device__ __forceinline__ int head_of(int x, int ng, int rep) {

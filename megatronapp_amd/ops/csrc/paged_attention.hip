@@ -122,19 +122,20 @@ __device__ __forceinline__ int pair_slot(int row, int slot) {
 }
 
 // --------------------------------------------------------- a row's own keys
-template <class T, int D>
-struct RowsLds {
-  // each wave's V rows; at the end the waves' sums
-  __attribute__((aligned(16))) unsigned short v[4 * KEYS * D];
+// What a block's waves tell each other at the end.
+struct WaveSums {
   float m[4][HEADS], l[4][HEADS];
 };
 
+// `image`: each wave's V rows, [4][KEYS][D]; at the end the waves' sums
 template <class T, int D>
 __device__ __forceinline__ void own_keys(const unsigned short* q, long qb,
                                          long qh, const Cache& c,
                                          const Groups& gr, const Out& out,
                                          int nh, int ng, float scale,
-                                         unsigned block, RowsLds<T, D>& lds) {
+                                         unsigned block,
+                                         unsigned short* image,
+                                         WaveSums& lds) {
   constexpr int NF = D / 32, ND = D / 16;
   constexpr int SLOTS = D / 8, PER = WAVE / SLOTS, NV = KEYS / PER;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -166,7 +167,7 @@ __device__ __forceinline__ void own_keys(const unsigned short* q, long qb,
 #pragma unroll
   for (int i = 0; i < ND; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, ms = 0.f, l = 0.f;
-  unsigned short* img = lds.v + wave * KEYS * D;
+  unsigned short* img = image + wave * KEYS * D;
   Pages ids = {0, -WAVE};
 
   typename T::x8 kn[2][NF];
@@ -287,7 +288,7 @@ __device__ __forceinline__ void own_keys(const unsigned short* q, long qb,
   const float a =
       m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx);
   // [HEADS][D] floats, the waves' added one after the other
-  float* sums = (float*)lds.v;
+  float* sums = (float*)image;
   constexpr int ROW = D;
 #pragma unroll
   for (int turn = 0; turn < 4; ++turn) {
@@ -356,6 +357,10 @@ __device__ __forceinline__ void shared_keys(
   const int slot = max(0, min(slot_at(c, first_row), c.count - 1));
   const int* table = c.tables + (long)slot * c.width;
   const int turns = (to - from + BN - 1) / BN;
+  // no tile lies in two pages: one number is enough
+  const bool whole = c.page % BN == 0;
+  const unsigned short* kb = c.k + hk * c.kh;
+  const unsigned short* vb = c.v + hk * c.vh;
   const unsigned k_off = lane_offset<D>(c.kt, wave, lane);
   const unsigned v_off = lane_offset<D>(c.vt, wave, lane);
   Pages ids = {0, -WAVE};
@@ -383,17 +388,27 @@ __device__ __forceinline__ void shared_keys(
 
     int fine = 0, fine_next = 0;    // which sixteenths' pages are in the pool
     auto fetch = [&](int t, unsigned short* img) {
-      long pg[4];
-      int in[4];
-      fine_next = 0;
+      int pg[4], in[4];
+      bool ok;
+      if (whole) {
+        const int index = page_of(c, from + t * BN, in[0]);
+        pg[0] = page_at(c, table, index, lane, ids, ok);
+        fine_next = ok ? 15 : 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // keys behind the piece are read as its last sixteen, and masked
-        bool ok;
-        const int index =
-            page_of(c, min(from + t * BN + 16 * i, (to - 1) & ~15), in[i]);
-        pg[i] = page_at(c, table, index, lane, ids, ok);
-        fine_next |= (int)ok << i;
+        for (int i = 1; i < 4; ++i) {
+          pg[i] = pg[0];
+          in[i] = in[0] + 16 * i;
+        }
+      } else {
+        fine_next = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // keys behind the piece are read as its last sixteen, and masked
+          const int index =
+              page_of(c, min(from + t * BN + 16 * i, (to - 1) & ~15), in[i]);
+          pg[i] = page_at(c, table, index, lane, ids, ok);
+          fine_next |= (int)ok << i;
+        }
       }
 #pragma unroll
       for (int i = 0; i < BN / PER / 4; ++i) {
@@ -403,10 +418,8 @@ __device__ __forceinline__ void shared_keys(
         const int base = x < 2 ? (x == 0 ? in[0] : in[1])
                                : (x == 2 ? in[2] : in[3]);
         const long at = base + (r0 & 15);
-        load_lds16(img + r0 * D, c.k + page * c.kp + hk * c.kh + at * c.kt,
-                   k_off);
-        load_lds16(img + (BN + r0) * D,
-                   c.v + page * c.vp + hk * c.vh + at * c.vt, v_off);
+        load_lds16(img + r0 * D, kb + page * c.kp + at * c.kt, k_off);
+        load_lds16(img + (BN + r0) * D, vb + page * c.vp + at * c.vt, v_off);
       }
     };
     auto step = [&](int t, const unsigned short* img) {
@@ -422,6 +435,7 @@ __device__ __forceinline__ void shared_keys(
         for (int f = 0; f < NF; ++f)
           st[u] = T::mfma32(read_rows<T, D>(img, kr, f, h), qf[f], st[u]);
       }
+      reads_ahead<2 * NF, 1>();
       if (!all || at + BN > to || fine != 15) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -512,73 +526,119 @@ template <class T, int D>
 __global__ __launch_bounds__(BLOCK, 2) void paged_rows_kernel(
     const unsigned short* __restrict__ q, long qb, long qh, Cache c, Groups gr,
     Out out, int nh, int ng, float scale) {
-  __shared__ RowsLds<T, D> lds;
-  own_keys<T, D>(q, qb, qh, c, gr, out, nh, ng, scale, blockIdx.x, lds);
+  __shared__ __attribute__((aligned(16))) unsigned short image[4 * KEYS * D];
+  __shared__ WaveSums sums;
+  own_keys<T, D>(q, qb, qh, c, gr, out, nh, ng, scale, blockIdx.x, image,
+                 sums);
 }
 
 template <class T, int D>
 __global__ __launch_bounds__(BLOCK, 2) void paged_groups_kernel(
     const unsigned short* __restrict__ q, long qb, long qh, Cache c, Groups gr,
     Out out, int nh, int ng, float scale) {
-  __shared__ union {
-    RowsLds<T, D> rows;
-    __attribute__((aligned(16))) unsigned short img[2][2 * BN * D];
-  } lds;
+  // two arrays, so that reads of one do not wait for what comes into the other
+  __shared__ __attribute__((aligned(16))) unsigned short img0[2 * BN * D];
+  __shared__ __attribute__((aligned(16))) unsigned short img1[2 * BN * D];
+  __shared__ WaveSums sums;
+  static_assert(2 * BN >= 4 * KEYS, "room for the rows' image");
   if (blockIdx.x < gr.blocks)
-    shared_keys<T, D>(q, qb, qh, c, gr, out, nh, ng, scale, blockIdx.x,
-                      lds.img[0], lds.img[1]);
+    shared_keys<T, D>(q, qb, qh, c, gr, out, nh, ng, scale, blockIdx.x, img0,
+                      img1);
   else
     own_keys<T, D>(q, qb, qh, c, gr, out, nh, ng, scale,
-                   blockIdx.x - gr.blocks, lds.rows);
+                   blockIdx.x - gr.blocks, img0, sums);
 }
 
 // -------------------------------------------------------------------- joining
+// A wave for each head of a row.  The pieces' log-sums come in at once, a lane
+// each, and each half-wave adds up every other piece (at D = 64 each quarter
+// every fourth).
 template <class T, int D>
 __global__ __launch_bounds__(BLOCK) void paged_join_kernel(Cache c, Groups gr,
                                                            Out out, int nh,
                                                            long heads) {
-  constexpr int LANES = D / 4;
-  const long r = ((long)blockIdx.x * BLOCK + threadIdx.x) / LANES;
-  const int d = threadIdx.x % LANES * 4;
+  constexpr int LANES = D / 4, PARTS = WAVE / LANES;
+  const int lane = threadIdx.x & 63, d = lane % LANES * 4;
+  const long r = (long)blockIdx.x * (BLOCK / WAVE) +
+                 __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (r >= heads) return;
+  const float* lse = out.lse + r * out.pieces;
+  const float* part = out.part + r * out.pieces * D + d;
   // a row that shares nothing has no pieces of a group
   const int pieces =
       shared_at(c, gr, (int)(r / nh)) ? out.pieces : out.pieces - gr.pieces;
-  const float* lse = out.lse + r * out.pieces;
-  const float* part = out.part + r * out.pieces * D + d;
-  float mx = -INFINITY, l = 0.f;
-  for (int i = 0; i < pieces; ++i) mx = fmaxf(mx, lse[i]);
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < pieces; ++i) {
-    const float x = lse[i];
-    if (x == -INFINITY) continue;
-    const float w = __builtin_amdgcn_exp2f(x - mx);
-    const f32x4 y = *(const f32x4*)(part + (long)i * D);
-    l += w;
+  const float x0 = lane < pieces ? lse[lane] : -INFINITY;
+  const float x1 = lane + WAVE < pieces ? lse[lane + WAVE] : -INFINITY;
+  float mx = fmaxf(x0, x1);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] += w * y[j];
+  for (int off = 32; off > 0; off >>= 1)
+    mx = fmaxf(mx, __shfl_xor(mx, off, WAVE));
+  const float w0 = x0 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x0 - mx);
+  const float w1 = x1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x1 - mx);
+  float l = w0 + w1;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off, WAVE);
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  // all lanes stay in: a lane that left would not hand over its weights
+#pragma unroll 4
+  for (int base = 0; base < pieces; base += PARTS) {
+    const int i = base + lane / LANES, last = pieces - 1;
+    const float a = __shfl(w0, i & 63, WAVE), b = __shfl(w1, i & 63, WAVE);
+    const float w = i < WAVE ? a : b;
+    const f32x4 y = *(const f32x4*)(part + (long)min(i, last) * D);
+    // a piece of no keys adds nothing, nor does one that is not there
+    if (i < pieces && w != 0.f) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] += w * y[j];
+    }
   }
+#pragma unroll
+  for (int off = LANES; off < WAVE; off <<= 1)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] += __shfl_xor(o[j], off, WAVE);
   const float by = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  u32x2 z = {pack2<T>(o[0] * by, o[1] * by), pack2<T>(o[2] * by, o[3] * by)};
-  *(u32x2*)(out.o + r * D + d) = z;
+  if (lane < LANES) {
+    u32x2 z = {pack2<T>(o[0] * by, o[1] * by), pack2<T>(o[2] * by, o[3] * by)};
+    *(u32x2*)(out.o + r * D + d) = z;
+  }
 }
 
 }  // namespace
 
-// How the work is cut: pieces of a row's own keys and of its group's.
-void paged_attn_pieces(int b, int nh, int ng, int max_length, int groups,
-                       int max_rows, int max_prefix, int* own, int* shared) {
+// How the work is cut: pieces of a row's own keys, and of its group's (none:
+// every row reads its shared pages for itself).
+//
+// A group's blocks run beside the rows' ones, one of each on a CU where there
+// are enough; both should end together.  A step of 64 keys of a group's block
+// takes the time in which the card reads some 9 MB of rows' own keys at D = 128
+// (half of that at 64), and rows are taken to have half of the longest one's
+// own keys; four steps are worth a piece.  256 rows on 16384 + 1..1024 tokens: 257, 185, 171, 186, 206
+// us in 2, 3, 4, 6, 8 pieces; 64 rows on 4096 + 33..700: 58, 48, 39, 40, 46 us
+// in 3, 4, 6, 8, 16.  Rows that read little more than SHARE bytes of shared
+// keys in all, mostly out of L2, are done sooner each for itself (24 rows in
+// four groups, 51 MB: 13 us against 16; 16 rows, 134 MB: 24 us against 17).
+void paged_attn_pieces(int b, int nh, int ng, int d, int max_length,
+                       int groups, int max_rows, long max_prefix, int* own,
+                       int* shared) {
+  constexpr long SHARE = 96l << 20;
   const long blocks = (long)b * ng * ((nh / ng + HEADS - 1) / HEADS);
   *shared = 0;
   long most = max_length;
-  if (groups > 0 && max_prefix > 0) {
-    const long tiles = ((long)max_rows * (nh / ng) + BM - 1) / BM;
-    const long units = (long)groups * tiles * ng;
-    const long cuts = std::min(512 / units, (long)max_prefix / 512);
-    *shared = (int)std::max(1l, std::min(cuts, 64l));
-    if (groups == 1) most = std::max(1l, most - max_prefix);
+  const long rows = std::min((long)b, (long)groups * max_rows);
+  if (rows * max_prefix * ng * d * 4 > SHARE) {
+    max_prefix = std::min(max_prefix, most);
+    most = std::max(1l, most - max_prefix);
+    const long units =
+        (long)groups * ng * (((long)max_rows * (nh / ng) + BM - 1) / BM);
+    const long steps = (max_prefix + BN - 1) / BN;
+    const long beside = (long)b * most * ng / 34000;   // in steps
+    // little beside them: two of a group's blocks on a CU
+    const long room = beside * 4 < steps * units / 256 ? 512 : 256;
+    const long per = std::max(4l, beside);
+    *shared = (int)std::max(
+        1l, std::min(std::min((steps + per - 1) / per, room / units), 64l));
   }
-  const long fill = (1024 + blocks - 1) / blocks;
+  const long fill = ((*shared ? 512 : 1024) + blocks - 1) / blocks;
   most = (most + 4 * KEYS - 1) / (4 * KEYS);
   *own = (int)std::max(1l, std::min(std::min(fill, most), 64l));
 }
@@ -601,8 +661,8 @@ void launch_paged_attn(const void* q, long qb, long qh, const void* k,
   const long first = shared ? (long)groups * tiles * ng * shared : 0;
   const long blocks =
       first + (long)b * own * ng * ((nh / ng + HEADS - 1) / HEADS);
-  const long lanes = (long)b * nh * (d / 4);
-  if (blocks * BLOCK >= 1l << 32 || lanes >= 1l << 32)
+  const long heads = (long)b * nh, each = BLOCK / WAVE;
+  if (blocks * BLOCK >= 1l << 32 || heads * WAVE >= 1l << 32)
     throw std::runtime_error("paged attention: too many rows for one launch");
   const Groups gr = {group_rows, group_lengths, shared ? groups : 0, b, tiles,
                      shared, (int)first};
@@ -620,9 +680,8 @@ void launch_paged_attn(const void* q, long qb, long qh, const void* k,
     HIP_CHECK_LAUNCH();                                                     \
     if (part) {                                                             \
       hipLaunchKernelGGL((paged_join_kernel<T, DD>),                        \
-                         dim3((unsigned)((lanes + BLOCK - 1) / BLOCK)),     \
-                         dim3(BLOCK), 0, stream, c, gr, out, nh,            \
-                         (long)b * nh);                                     \
+                         dim3((unsigned)((heads + each - 1) / each)),       \
+                         dim3(BLOCK), 0, stream, c, gr, out, nh, heads);    \
       HIP_CHECK_LAUNCH();                                                   \
     }                                                                       \
   } while (0)

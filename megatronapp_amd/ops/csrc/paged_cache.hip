@@ -64,24 +64,29 @@ __device__ __forceinline__ int pages_for(int tokens, int page) {
   return (int)(((long)tokens + page - 1) / page);
 }
 
+// A thread's four of the counts from `base` on; -1 behind the last.
+__device__ __forceinline__ void four_refs(const Pool& p, int base, int* f) {
+  const int at = base + 4 * threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = at + i < p.pages ? p.refs[at + i] : -1;
+}
+
 // The lowest `need` free pages, in order, to `out`; false if there are fewer.
-__device__ bool lowest_free(const Pool& p, int need, int* out, int* lds) {
+// `f`: the first counts, which the caller read before it knew `need`.
+__device__ bool lowest_free(const Pool& p, int need, int* out, int* lds,
+                            int* f) {
   int found = 0;
   for (int base = 0; base < p.pages && found < need; base += 4 * PLAN) {
-    const int at = base + 4 * threadIdx.x;
+    if (base) four_refs(p, base, f);
     int free = 0;
-    bool f[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[i] = at + i < p.pages && p.refs[at + i] == 0;
-      free += f[i];
-    }
+    for (int i = 0; i < 4; ++i) free += f[i] == 0;
     int total;
     int k = found + block_scan(free, lds, total) - free;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (f[i]) {
-        if (k < need) out[k] = at + i;
+      if (f[i] == 0) {
+        if (k < need) out[k] = base + 4 * threadIdx.x + i;
         ++k;
       }
     found += total;
@@ -110,10 +115,13 @@ __global__ __launch_bounds__(PLAN) void fork_plan_kernel(
   __shared__ int lds[WAVES];
   __shared__ int bad;
   extern __shared__ unsigned named[];   // a bit for each slot
+  int refs[4];
+  four_refs(p, 0, refs);
   if (threadIdx.x == 0) bad = 0;
   for (int i = threadIdx.x; i < (p.slots + 31) / 32; i += PLAN) named[i] = 0;
   __syncthreads();
   int copies = 0;
+  Pair mine = {0, -1, -1, 0};
   for (int base = 0; base < n; base += PLAN) {
     const int i = base + threadIdx.x;
     Pair pr = {0, -1, -1, 0};
@@ -140,14 +148,24 @@ __global__ __launch_bounds__(PLAN) void fork_plan_kernel(
     int total;
     const int k = copies + block_scan(copy, lds, total) - copy;
     if (copy) pr.to = k;      // the k-th free page, below
-    if (i < n) plan[i] = pr;
+    mine = pr;
+    if (i < n && n > PLAN) plan[i] = pr;
     copies += total;
   }
-  const bool enough = lowest_free(p, copies, fresh, lds);
+  __shared__ int few[PLAN];   // the pages, where they are not many
+  int* out = copies <= PLAN ? few : fresh;
+  const bool enough = lowest_free(p, copies, out, lds, refs);
   __threadfence_block();
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += PLAN)
-    if (plan[i].to >= 0) plan[i].to = enough ? fresh[plan[i].to] : -1;
+  if (n <= PLAN) {            // a pair a thread, still in its registers
+    if ((int)threadIdx.x < n) {
+      if (mine.to >= 0) mine.to = enough ? out[mine.to] : -1;
+      plan[threadIdx.x] = mine;
+    }
+  } else {
+    for (int i = threadIdx.x; i < n; i += PLAN)
+      if (plan[i].to >= 0) plan[i].to = enough ? out[plan[i].to] : -1;
+  }
   if (threadIdx.x == 0) {
     const int code = bad | (enough ? 0 : NO_PAGE);
     if (code) atomicOr(p.status, code);
@@ -158,12 +176,13 @@ __global__ __launch_bounds__(PLAN) void fork_plan_kernel(
 __global__ __launch_bounds__(BLOCK) void fork_apply_kernel(
     Pool p, const int* src, const int* dst, const int* go, const Pair* plan,
     const int* rows, char* pages, int planes, int groups, int token) {
-  if (!*go) return;
   const int i = blockIdx.x;
-  const Pair pr = plan[i];
+  const Pair pr = plan[i];      // read at once with whether it holds
+  const int from = src[i], into = dst[i];
+  if (!*go) return;
   if (blockIdx.y == 0) {
-    if (src[i] == dst[i]) return;
-    int* row = p.tables + (long)dst[i] * p.width;
+    if (from == into) return;
+    int* row = p.tables + (long)into * p.width;
     const int full = pr.length / p.page;
     for (int j = threadIdx.x; j < p.width; j += BLOCK) {
       const int old = row[j];
@@ -174,7 +193,7 @@ __global__ __launch_bounds__(BLOCK) void fork_apply_kernel(
       if (page >= 0 && page < p.pages) atomicAdd(p.refs + page, 1);
       row[j] = page;
     }
-    if (threadIdx.x == 0) p.lengths[dst[i]] = pr.length;
+    if (threadIdx.x == 0) p.lengths[into] = pr.length;
     return;
   }
   if (pr.to < 0) return;
@@ -262,10 +281,12 @@ __global__ __launch_bounds__(PLAN) void compact_plan_kernel(Pool p, int* map,
   }
 }
 
+// source and target never overlap, so several loads may be in flight
 __device__ __forceinline__ void copy_page(char* pages, long bytes, int count,
                                           int plane, int from, int to) {
-  const char* a = pages + ((long)plane * count + from) * bytes;
-  char* b = pages + ((long)plane * count + to) * bytes;
+  const char* __restrict__ a = pages + ((long)plane * count + from) * bytes;
+  char* __restrict__ b = pages + ((long)plane * count + to) * bytes;
+#pragma unroll 4
   for (long x = (long)threadIdx.x * 16; x < bytes; x += BLOCK * 16)
     *(float4*)(b + x) = *(const float4*)(a + x);
 }
@@ -315,6 +336,8 @@ __global__ __launch_bounds__(PLAN) void extend_kernel(Pool p, const int* slots,
   __shared__ int lds[WAVES];
   __shared__ int bad;
   extern __shared__ unsigned named[];
+  int refs[4];
+  four_refs(p, 0, refs);
   if (threadIdx.x == 0) bad = 0;
   for (int i = threadIdx.x; i < (p.slots + 31) / 32; i += PLAN) named[i] = 0;
   __syncthreads();
@@ -345,7 +368,7 @@ __global__ __launch_bounds__(PLAN) void extend_kernel(Pool p, const int* slots,
   bool ok = bad == 0;
   const bool enough = !ok || need <= p.pages;
   // `fresh` holds as many as there are pages
-  ok = ok && enough && lowest_free(p, need, fresh, lds);
+  ok = ok && enough && lowest_free(p, need, fresh, lds, refs);
   __threadfence_block();
   __syncthreads();
   if (!ok) {

@@ -171,6 +171,14 @@ def test_head_layouts(nh, ng):
 
 
 @gpu
+@pytest.mark.parametrize("n", [4200, 4300, 4400, 4500])
+@pytest.mark.parametrize("d", [64, 128])
+def test_any_number_of_pieces(n, d):
+    """33 to 36 pieces of one row."""
+    _check([n], nh=2, ng=1, d=d)
+
+
+@gpu
 def test_long_rows_and_many_rows():
     _check([9000, 31], nh=4, ng=2, d=128, page=64)
     _check([(i * 37) % 90 for i in range(150)], nh=2, ng=1, d=64)
@@ -295,14 +303,17 @@ def test_two_captured_graphs():
         _near(paged_attention(*s), want)
 
 
-def _groups(rows, lengths, max_rows=None, max_length=None):
+SURELY = 1 << 20      # a host that expects this much always shares
+
+
+def _groups(rows, lengths, max_rows=None, max_length=SURELY):
     ends = list(rows)
     return SharedPrefix(
         torch.tensor(ends, dtype=torch.int32, device="cuda"),
         torch.tensor(lengths, dtype=torch.int32, device="cuda"),
         max_rows if max_rows is not None else
         max(b - a for a, b in zip(ends[:-1], ends[1:])),
-        max_length if max_length is not None else max(lengths))
+        max_length)
 
 
 def _grouped_state(sizes, prefixes, own, **kw):
@@ -332,11 +343,11 @@ def test_one_shared_prefix(dtype, d):
     own = [1 + (i * 37) % 90 for i in range(50)]
     s = _grouped_state([50], [640], own, dtype=dtype, d=d, nh=8, ng=2)
     want = oracle(*s)
-    for most in (640, 1, 1 << 20):
+    for most in (640, 1, SURELY):
         _near(paged_attention(*s, shared_prefix=_groups([0, 50], [640], 50,
                                                         most)), want)
     # a host that knows too few rows
-    _near(paged_attention(*s, shared_prefix=_groups([0, 50], [640], 1, 640)),
+    _near(paged_attention(*s, shared_prefix=_groups([0, 50], [640], 1)),
           want)
     # a part of a page does not count
     _near(paged_attention(*s, shared_prefix=_groups([0, 50], [639])), want)
@@ -366,8 +377,10 @@ def test_groups_of_rows(page):
 def test_a_long_prefix_for_many_rows():
     own = [1 + (i * 37) % 90 for i in range(70)]
     s = _grouped_state([70], [6400], own, d=128, nh=8, ng=2, page=64)
-    _near(paged_attention(*s, shared_prefix=_groups([0, 70], [6400])),
-          oracle(*s))
+    want = oracle(*s)
+    for most in (6400, SURELY):
+        _near(paged_attention(*s, shared_prefix=_groups([0, 70], [6400], 70,
+                                                        most)), want)
 
 
 @gpu
