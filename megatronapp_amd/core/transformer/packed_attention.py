@@ -36,9 +36,9 @@ def packed_attention_supported(query: torch.Tensor) -> bool:
 class _PackedAttnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, scale, causal):
-        o, lse = _ops.get_ops().packed_attn_fwd(q, k, v, cu_q, cu_k, scale,
-                                                causal, True)
-        ctx.save_for_backward(q, k, v, o, lse, cu_q, cu_k)
+        o, lse, low = _ops.get_ops().packed_attn_fwd(q, k, v, cu_q, cu_k,
+                                                     scale, causal, True)
+        ctx.save_for_backward(q, k, v, o, low, lse, cu_q, cu_k)
         ctx.scale = scale
         ctx.causal = causal
         return o
@@ -46,9 +46,9 @@ class _PackedAttnFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
-        q, k, v, o, lse, cu_q, cu_k = ctx.saved_tensors
+        q, k, v, o, low, lse, cu_q, cu_k = ctx.saved_tensors
         dq, dk, dv = _ops.get_ops().packed_attn_bwd(
-            do, q, k, v, o, lse, cu_q, cu_k, ctx.scale, ctx.causal)
+            do, q, k, v, o, low, lse, cu_q, cu_k, ctx.scale, ctx.causal)
         return dq, dk, dv, None, None, None, None
 
 

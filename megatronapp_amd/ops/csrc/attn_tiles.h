@@ -209,21 +209,38 @@ __device__ __forceinline__ float half_sum(float v) {
 
 // A 32x32 C tile (rows d, columns n) as 16-byte pieces of row n: the two
 // half-waves exchange so that h = 0 gets elements 0..7 and h = 1 8..15 of
-// each sixteen.  `p` points at element 0 of row n, aligned to 16 bytes.
-template <class T>
+// each sixteen.  `p` points at element 0 of row n, aligned to 16 bytes; `low`,
+// where there is one, gets what the rounding left out.
+template <class T, bool LOW = false>
 __device__ __forceinline__ void store_cols(unsigned short* p, const f32x16& c,
-                                           float by, int h) {
+                                           float by, int h,
+                                           unsigned short* low = nullptr) {
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    unsigned a[2], b[2];
+    unsigned a[2], b[2], la[2], lb[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      a[i] = pack2<T>(c[8 * k + 2 * i] * by, c[8 * k + 2 * i + 1] * by);
-      b[i] = pack2<T>(c[8 * k + 4 + 2 * i] * by, c[8 * k + 5 + 2 * i] * by);
+      const float x[4] = {c[8 * k + 2 * i] * by, c[8 * k + 2 * i + 1] * by,
+                          c[8 * k + 4 + 2 * i] * by,
+                          c[8 * k + 5 + 2 * i] * by};
+      a[i] = pack2<T>(x[0], x[1]);
+      b[i] = pack2<T>(x[2], x[3]);
+      if (LOW) {
+        la[i] = pack2<T>(x[0] - T::to_float(a[i] & 0xffff),
+                         x[1] - T::to_float(a[i] >> 16));
+        lb[i] = pack2<T>(x[2] - T::to_float(b[i] & 0xffff),
+                         x[3] - T::to_float(b[i] >> 16));
+      }
     }
     auto s0 = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
     auto s1 = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
     u32x4 w = {s0[0], s1[0], s0[1], s1[1]};
     *(u32x4*)(p + 16 * k + 8 * h) = w;
+    if (LOW) {
+      s0 = __builtin_amdgcn_permlane32_swap(la[0], lb[0], false, false);
+      s1 = __builtin_amdgcn_permlane32_swap(la[1], lb[1], false, false);
+      u32x4 y = {s0[0], s1[0], s0[1], s1[1]};
+      *(u32x4*)(low + 16 * k + 8 * h) = y;
+    }
   }
 }

@@ -114,12 +114,13 @@ void launch_attn_bwd(const void*, const void*, const void*, const void*,
                      int, int, int, int, int, int, float, bool, hipStream_t);
 
 void launch_packed_attn_fwd(const void*, const void*, const void*, void*,
-                            float*, const int*, const int*, int, int, int, int,
+                            void*, float*, const int*, const int*, int, int, int, int,
                             int, int, int, float, bool, bool, const long*,
                             const long*, const long*, hipStream_t);
 void launch_packed_attn_bwd(const void*, const void*, const void*,
-                            const void*, const void*, const float*, float*,
-                            void*, void*, void*, const int*, const int*, int,
+                            const void*, const void*, const void*,
+                            const float*, float*, void*, void*, void*,
+                            const int*, const int*, int,
                             int, int, int, int, int, int, float, bool, bool,
                             const long*, const long*, const long*, const long*,
                             hipStream_t);
@@ -829,11 +830,12 @@ torch::Tensor int32_row(const torch::Tensor& t) {
       .contiguous();
 }
 
-// the output, and where a backward will follow the rows' log-sums
+// the output, and where a backward will follow the rows' log-sums and what
+// the output's rounding left out
 std::vector<torch::Tensor> packed_attn_fwd(
     torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor cu_q,
     c10::optional<torch::Tensor> cu_kv, c10::optional<double> softmax_scale,
-    bool causal, bool want_lse) {
+    bool causal, bool training) {
   const torch::Tensor cu_k = cu_kv.has_value() ? *cu_kv : cu_q;
   const double scale = softmax_scale.has_value()
                            ? *softmax_scale
@@ -841,27 +843,29 @@ std::vector<torch::Tensor> packed_attn_fwd(
   const PackedShape s = packed_shape(q, k, v, cu_q, cu_k, scale);
   c10::DeviceGuard guard(q.device());
   auto o = torch::empty(q.sizes(), q.options());
-  torch::Tensor lse;
-  if (want_lse)
+  torch::Tensor lse, low;
+  if (training) {
     lse = torch::empty({s.b, s.nh, s.tq}, q.options().dtype(torch::kFloat32));
-  if (o.numel() == 0) return {o, lse};
+    low = torch::empty(q.sizes(), q.options());
+  }
+  if (o.numel() == 0) return {o, lse, low};
   long qs[3], ks[3], vs[3];
   auto qr = packed_rows(q, qs), kr = packed_rows(k, ks),
        vr = packed_rows(v, vs);
   const torch::Tensor iq = int32_row(cu_q),
                       ik = cu_k.is_same(cu_q) ? iq : int32_row(cu_k);
   launch_packed_attn_fwd(qr.data_ptr(), kr.data_ptr(), vr.data_ptr(),
-                         o.data_ptr(),
-                         want_lse ? lse.data_ptr<float>() : nullptr,
+                         o.data_ptr(), training ? low.data_ptr() : nullptr,
+                         training ? lse.data_ptr<float>() : nullptr,
                          iq.data_ptr<int>(), ik.data_ptr<int>(), s.n, s.tq,
                          s.tk, s.b, s.nh, s.ng, s.d, (float)scale, causal,
                          s.fp16, qs, ks, vs, cur_stream());
-  return {o, lse};
+  return {o, lse, low};
 }
 
 std::vector<torch::Tensor> packed_attn_bwd(
     torch::Tensor dout, torch::Tensor q, torch::Tensor k, torch::Tensor v,
-    torch::Tensor o, torch::Tensor lse, torch::Tensor cu_q,
+    torch::Tensor o, torch::Tensor low, torch::Tensor lse, torch::Tensor cu_q,
     c10::optional<torch::Tensor> cu_kv, c10::optional<double> softmax_scale,
     bool causal) {
   const torch::Tensor cu_k = cu_kv.has_value() ? *cu_kv : cu_q;
@@ -870,14 +874,20 @@ std::vector<torch::Tensor> packed_attn_bwd(
                            : 1.0 / std::sqrt((double)q.size(-1));
   const PackedShape s = packed_shape(q, k, v, cu_q, cu_k, scale);
   c10::DeviceGuard guard(q.device());
-  TORCH_CHECK_VALUE(dout.sizes() == q.sizes() && o.sizes() == q.sizes() &&
+  for (auto* t : {&o, &low})
+    TORCH_CHECK_VALUE(t->sizes() == q.sizes() && t->is_contiguous() &&
+                          t->scalar_type() == q.scalar_type() &&
+                          t->device() == q.device(),
+                      "packed_attention: o and low must be the forward's");
+  TORCH_CHECK_VALUE(dout.sizes() == q.sizes() &&
                         dout.scalar_type() == q.scalar_type() &&
-                        dout.device() == q.device() && o.is_contiguous() &&
-                        o.scalar_type() == q.scalar_type() &&
+                        dout.device() == q.device() &&
+                        lse.device() == q.device() &&
                         lse.numel() == (long)s.b * s.nh * s.tq &&
                         lse.is_contiguous() &&
                         lse.scalar_type() == torch::kFloat32,
-                    "packed_attention: dout, o and lse must be the forward's");
+                    "packed_attention: dout must be the output's gradient and "
+                    "lse the forward's");
   auto dq = torch::empty(q.sizes(), q.options());
   auto dk = torch::empty(k.sizes(), q.options());
   auto dv = torch::empty(k.sizes(), q.options());
@@ -890,7 +900,7 @@ std::vector<torch::Tensor> packed_attn_bwd(
                       ik = cu_k.is_same(cu_q) ? iq : int32_row(cu_k);
   launch_packed_attn_bwd(
       dr.data_ptr(), qr.data_ptr(), kr.data_ptr(), vr.data_ptr(), o.data_ptr(),
-      lse.data_ptr<float>(), dot.data_ptr<float>(), dq.data_ptr(),
+      low.data_ptr(), lse.data_ptr<float>(), dot.data_ptr<float>(), dq.data_ptr(),
       dk.data_ptr(), dv.data_ptr(), iq.data_ptr<int>(), ik.data_ptr<int>(),
       s.n, s.tq, s.tk, s.b, s.nh, s.ng, s.d, (float)scale, causal, s.fp16, os,
       qs, ks, vs, cur_stream());

@@ -233,7 +233,7 @@ __device__ __forceinline__ void own_keys(const unsigned short* q, long qb,
     }
     mt = fmaxf(mt, __shfl_xor(mt, 16, WAVE));
     mt = fmaxf(mt, __shfl_xor(mt, 32, WAVE)) * scale;
-    if (__any(mt > m + 8.f)) {
+    if (__any(mt > m)) {
       const float mn = fmaxf(m, mt);
       const float a = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
@@ -451,7 +451,7 @@ __device__ __forceinline__ void shared_keys(
 #pragma unroll
         for (int r = 0; r < 16; ++r) mt = fmaxf(mt, st[u][r]);
       mt = half_max(mt) * scale;
-      if (__any(mt > m + 8.f)) {
+      if (__any(mt > m)) {
         const float mn = fmaxf(m, mt);
         const float a = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
         m = mn;
