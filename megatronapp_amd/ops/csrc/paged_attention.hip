@@ -359,8 +359,9 @@ __device__ __forceinline__ void shared_keys(
   const int turns = (to - from + BN - 1) / BN;
   // no tile lies in two pages: one number is enough
   const bool whole = c.page % BN == 0;
-  const unsigned short* kb = c.k + hk * c.kh;
-  const unsigned short* vb = c.v + hk * c.vh;
+  const unsigned short* kb = c.k + hk * c.kh + wave * PER * c.kt;
+  const unsigned short* vb = c.v + hk * c.vh + wave * PER * c.vt;
+  const long k_step = 4 * PER * c.kt, v_step = 4 * PER * c.vt;
   const unsigned k_off = lane_offset<D>(c.kt, wave, lane);
   const unsigned v_off = lane_offset<D>(c.vt, wave, lane);
   Pages ids = {0, -WAVE};
@@ -388,27 +389,33 @@ __device__ __forceinline__ void shared_keys(
 
     int fine = 0, fine_next = 0;    // which sixteenths' pages are in the pool
     auto fetch = [&](int t, unsigned short* img) {
-      int pg[4], in[4];
       bool ok;
       if (whole) {
-        const int index = page_of(c, from + t * BN, in[0]);
-        pg[0] = page_at(c, table, index, lane, ids, ok);
+        int in;
+        const int index = page_of(c, from + t * BN, in);
+        const long page = page_at(c, table, index, lane, ids, ok);
         fine_next = ok ? 15 : 0;
+        const unsigned short* kr = kb + page * c.kp + in * c.kt;
+        const unsigned short* vr = vb + page * c.vp + in * c.vt;
 #pragma unroll
-        for (int i = 1; i < 4; ++i) {
-          pg[i] = pg[0];
-          in[i] = in[0] + 16 * i;
+        for (int i = 0; i < BN / PER / 4; ++i) {
+          const int r0 = (i * 4 + wave) * PER;
+          load_lds16(img + r0 * D, kr, k_off);
+          load_lds16(img + (BN + r0) * D, vr, v_off);
+          kr += k_step;
+          vr += v_step;
         }
-      } else {
-        fine_next = 0;
+        return;
+      }
+      int pg[4], in[4];
+      fine_next = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // keys behind the piece are read as its last sixteen, and masked
-          const int index =
-              page_of(c, min(from + t * BN + 16 * i, (to - 1) & ~15), in[i]);
-          pg[i] = page_at(c, table, index, lane, ids, ok);
-          fine_next |= (int)ok << i;
-        }
+      for (int i = 0; i < 4; ++i) {
+        // keys behind the piece are read as its last sixteen, and masked
+        const int index =
+            page_of(c, min(from + t * BN + 16 * i, (to - 1) & ~15), in[i]);
+        pg[i] = page_at(c, table, index, lane, ids, ok);
+        fine_next |= (int)ok << i;
       }
 #pragma unroll
       for (int i = 0; i < BN / PER / 4; ++i) {
@@ -417,7 +424,8 @@ __device__ __forceinline__ void shared_keys(
                                 : (x == 2 ? pg[2] : pg[3]);
         const int base = x < 2 ? (x == 0 ? in[0] : in[1])
                                : (x == 2 ? in[2] : in[3]);
-        const long at = base + (r0 & 15);
+        // kb and vb begin at the wave's rows of the first sixteenth
+        const long at = base - (r0 & ~15) + i * 4 * PER;
         load_lds16(img + r0 * D, kb + page * c.kp + at * c.kt, k_off);
         load_lds16(img + (BN + r0) * D, vb + page * c.vp + at * c.vt, v_off);
       }
