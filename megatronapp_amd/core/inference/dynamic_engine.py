@@ -141,10 +141,16 @@ class DynamicInferenceEngine:
         ctx = self.context
         slots = [s for s in range(ctx.max_slots) if ctx.host_lengths[s] == 0]
         batch: List[List[_Running]] = []
+        tokens = 0
         while self.waiting:
             family = self._families[self.waiting[0].family]
             pages = family.shared_pages + family.members * family.own_pages
+            tokens += len(self.waiting[0].prompt_tokens)
             if family.members > len(slots) or pages > self._pages_left:
+                break
+            # the stream has logits for all its tokens: no more of them than
+            # one prompt may have, the others go with the next step
+            if batch and tokens > self.max_sequence_length:
                 break
             members = self.waiting[:family.members]
             del self.waiting[:family.members]

@@ -154,6 +154,11 @@ class PagedInferenceContext:
             self.host_lengths[s] += n
 
     # ------------------------------------------------------- for the layers
+    def update_kv_cache(self, layer_number, key, value):
+        raise NotImplementedError(
+            "a paged cache is read through attend(): this layer's attention "
+            "does not know it")
+
     def row_positions(self) -> torch.Tensor:
         """Each new token's place in its sequence."""
         return self._positions

@@ -130,9 +130,9 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor,
                      causal: bool = True) -> torch.Tensor:
     """query [t, np, hn] or [t, b, np, hn], key and value the same with ng
     heads that divide np (and a length of their own); returns the query's
-    shape.  ``cu_seqlens_kv`` defaults to ``cu_seqlens_q``; both are given on
-    the query's device, and are not read by the host there, so ends that run
-    out of the stream are cut off at it rather than refused."""
+    shape.  ``cu_seqlens_kv`` defaults to ``cu_seqlens_q``; both ascend, are
+    given on the query's device, and are not read by the host there, so ends
+    that run out of the stream are cut off at it rather than refused."""
     cu_q = packed_seq_params.cu_seqlens_q
     cu_k = packed_seq_params.cu_seqlens_kv
     if cu_q is None:

@@ -779,7 +779,9 @@ struct PackedShape {
 
 PackedShape packed_shape(const torch::Tensor& q, const torch::Tensor& k,
                          const torch::Tensor& v, const torch::Tensor& cu_q,
-                         const torch::Tensor& cu_k, double scale) {
+                         const torch::Tensor& cu_k,
+                         const c10::optional<double>& softmax_scale,
+                         double& scale) {
   const int dim = (int)q.dim(), h = dim - 2;
   TORCH_CHECK_VALUE((dim == 3 || dim == 4) && k.dim() == dim &&
                         k.sizes() == v.sizes(),
@@ -810,7 +812,9 @@ PackedShape packed_shape(const torch::Tensor& q, const torch::Tensor& k,
                       "packed_attention: cu_seqlens must be on the query's "
                       "device");
   }
-  TORCH_CHECK_VALUE(scale > 0 && std::isfinite((float)scale),
+  scale = softmax_scale.has_value() ? *softmax_scale
+                                    : 1.0 / std::sqrt((double)q.size(h + 1));
+  TORCH_CHECK_VALUE((float)scale > 0 && std::isfinite((float)scale),
                     "packed_attention: softmax_scale must be positive and "
                     "finite");
   const bool fp16 = q.scalar_type() == torch::kHalf;
@@ -837,10 +841,8 @@ std::vector<torch::Tensor> packed_attn_fwd(
     c10::optional<torch::Tensor> cu_kv, c10::optional<double> softmax_scale,
     bool causal, bool training) {
   const torch::Tensor cu_k = cu_kv.has_value() ? *cu_kv : cu_q;
-  const double scale = softmax_scale.has_value()
-                           ? *softmax_scale
-                           : 1.0 / std::sqrt((double)q.size(-1));
-  const PackedShape s = packed_shape(q, k, v, cu_q, cu_k, scale);
+  double scale;
+  const PackedShape s = packed_shape(q, k, v, cu_q, cu_k, softmax_scale, scale);
   c10::DeviceGuard guard(q.device());
   auto o = torch::empty(q.sizes(), q.options());
   torch::Tensor lse, low;
@@ -869,10 +871,8 @@ std::vector<torch::Tensor> packed_attn_bwd(
     c10::optional<torch::Tensor> cu_kv, c10::optional<double> softmax_scale,
     bool causal) {
   const torch::Tensor cu_k = cu_kv.has_value() ? *cu_kv : cu_q;
-  const double scale = softmax_scale.has_value()
-                           ? *softmax_scale
-                           : 1.0 / std::sqrt((double)q.size(-1));
-  const PackedShape s = packed_shape(q, k, v, cu_q, cu_k, scale);
+  double scale;
+  const PackedShape s = packed_shape(q, k, v, cu_q, cu_k, softmax_scale, scale);
   c10::DeviceGuard guard(q.device());
   for (auto* t : {&o, &low})
     TORCH_CHECK_VALUE(t->sizes() == q.sizes() && t->is_contiguous() &&
@@ -891,7 +891,7 @@ std::vector<torch::Tensor> packed_attn_bwd(
   auto dq = torch::empty(q.sizes(), q.options());
   auto dk = torch::empty(k.sizes(), q.options());
   auto dv = torch::empty(k.sizes(), q.options());
-  if (s.b == 0 || s.nh == 0) return {dq, dk, dv};
+  if (s.b == 0 || s.nh == 0) return {dq, dk.zero_(), dv.zero_()};
   auto dot = torch::empty_like(lse);
   long os[3], qs[3], ks[3], vs[3];
   auto dr = packed_rows(dout, os), qr = packed_rows(q, qs),
@@ -1108,8 +1108,10 @@ torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
                     "paged_attention: on the GPU bf16 or fp16 with head size "
                     "64 or 128, got ", q.scalar_type(), ", ", d);
   for (auto* t : {&k, &v})
-    TORCH_CHECK_VALUE(t->stride(3) == 1 && t->stride(0) % 8 == 0 &&
-                          t->stride(1) % 8 == 0 && t->stride(2) % 8 == 0 &&
+    TORCH_CHECK_VALUE(t->stride(3) == 1 &&
+                          (t->size(0) == 1 || t->stride(0) % 8 == 0) &&
+                          (t->size(1) == 1 || t->stride(1) % 8 == 0) &&
+                          t->stride(2) % 8 == 0 &&
                           t->stride(2) < (1l << 27) &&
                           reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
                       "paged_attention: the rows of a page must start on 16 "
@@ -1127,7 +1129,7 @@ torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
                     "slot for each row");
   const double scale = softmax_scale.has_value() ? *softmax_scale
                                                  : 1.0 / std::sqrt((double)d);
-  TORCH_CHECK_VALUE(scale > 0 && std::isfinite((float)scale),
+  TORCH_CHECK_VALUE((float)scale > 0 && std::isfinite((float)scale),
                     "paged_attention: softmax_scale must be positive and "
                     "finite");
   int groups = 0, own, shared;

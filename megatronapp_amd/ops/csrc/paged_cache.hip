@@ -39,21 +39,22 @@ struct Pool {
 };
 
 // inclusive sum over the block; `total` is everybody's
-__device__ __forceinline__ int block_scan(int v, int* lds, int& total) {
+template <class N>
+__device__ __forceinline__ N block_scan(N v, N* lds, N& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int off = 1; off < WAVE; off <<= 1) {
-    const int x = __shfl_up(v, off, WAVE);
+    const N x = __shfl_up(v, off, WAVE);
     if (lane >= off) v += x;
   }
   __syncthreads();
   if (lane == 63) lds[wave] = v;
   __syncthreads();
-  int before = 0;
+  N before = 0;
   total = 0;
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) {
-    const int x = lds[w];
+    const N x = lds[w];
     before += w < wave ? x : 0;
     total += x;
   }
@@ -146,7 +147,7 @@ __global__ __launch_bounds__(PLAN) void fork_plan_kernel(
       }
     }
     int total;
-    const int k = copies + block_scan(copy, lds, total) - copy;
+    const int k = copies + block_scan((int)copy, lds, total) - copy;
     if (copy) pr.to = k;      // the k-th free page, below
     mine = pr;
     if (i < n && n > PLAN) plan[i] = pr;
@@ -334,6 +335,7 @@ __global__ __launch_bounds__(PLAN) void extend_kernel(Pool p, const int* slots,
                                                       int* offsets,
                                                       int* fresh) {
   __shared__ int lds[WAVES];
+  __shared__ long wide[WAVES];   // all that is asked for may pass 32 bits
   __shared__ int bad;
   extern __shared__ unsigned named[];
   int refs[4];
@@ -341,10 +343,10 @@ __global__ __launch_bounds__(PLAN) void extend_kernel(Pool p, const int* slots,
   if (threadIdx.x == 0) bad = 0;
   for (int i = threadIdx.x; i < (p.slots + 31) / 32; i += PLAN) named[i] = 0;
   __syncthreads();
-  int need = 0;
+  long need = 0;
   for (int base = 0; base < n; base += PLAN) {
     const int i = base + threadIdx.x;
-    int more = 0;
+    long more = 0;
     if (i < n) {
       const int s = slots[i], c = counts ? counts[i] : each;
       if (s < 0 || s >= p.slots || c < 0) {
@@ -359,16 +361,15 @@ __global__ __launch_bounds__(PLAN) void extend_kernel(Pool p, const int* slots,
           more = pages_for(len + c, p.page) - pages_for(len, p.page);
       }
     }
-    int total;
-    const int k = need + block_scan(more, lds, total) - more;
-    if (i < n) offsets[i] = k;
+    long total;
+    const long k = need + block_scan(more, wide, total) - more;
+    if (i < n) offsets[i] = (int)k;   // used where all of it fits
     need += total;
   }
   __syncthreads();
   bool ok = bad == 0;
-  const bool enough = !ok || need <= p.pages;
   // `fresh` holds as many as there are pages
-  ok = ok && enough && lowest_free(p, need, fresh, lds, refs);
+  ok = ok && need <= p.pages && lowest_free(p, (int)need, fresh, lds, refs);
   __threadfence_block();
   __syncthreads();
   if (!ok) {

@@ -415,6 +415,16 @@ def test_refusals_on_the_gpu():
         packed_attention(x, x, x, PackedSeqParams(cu_seqlens_q=_cu([4])))
     empty = x[:0]
     assert packed_attention(empty, empty, empty, params).shape == (0, 2, 64)
+    with pytest.raises(ValueError, match="must be"):
+        packed_attention(x[0, 0, 0], x, x, params)
+    # no queries, or no heads of them: nothing for the keys, and no keys:
+    # nothing for the queries
+    for q, k in ((empty, x), (x[:, :0], x), (x, empty)):
+        q, k, v = (t.clone().requires_grad_(True) for t in (q, k, k))
+        o = packed_attention(q, k, v, params)
+        assert o.shape == q.shape and (o == 0).all()
+        for t, g in zip((q, k, v), torch.autograd.grad(o.sum(), (q, k, v))):
+            assert g.shape == t.shape and (g == 0).all()
 
 
 @gpu

@@ -157,6 +157,20 @@ def test_requests_wait_for_pages():
     destroy()
 
 
+def test_a_step_admits_no_more_than_one_longest_prompt():
+    _cpu_only()
+    model = _model()
+    sp = SamplingParams(num_tokens_to_generate=3, top_k=1)
+    want = _engine(model).generate([PROMPTS[4]], sp)[0].generated_text
+    e = _engine(model, slots=4)
+    seen, inner = [], e.context.begin_prompts
+    e.context.begin_prompts = lambda s, n: seen.append(n) or inner(s, n)
+    out = e.generate([PROMPTS[4]] * 3 + [PROMPTS[0]], sp)   # 40 of 64 each
+    assert seen == [[40], [40], [40, 3]]
+    assert [r.generated_text for r in out[:3]] == [want] * 3
+    destroy()
+
+
 def test_beams_reorder_by_fork():
     _cpu_only()
     model = _model()
