@@ -140,11 +140,12 @@ void launch_cache_write(int*, int*, int*, int*, int, int, int, int, const int*,
                         const int*, int, int, void*, void*, const void*,
                         const void*, int, int, long, long, long, long,
                         hipStream_t);
-void paged_attn_pieces(int, int, int, int, int, int, int, long, int*, int*);
+void paged_attn_pieces(int, int, int, int, int, int, int, long, int*, int*,
+                       int*);
 void launch_paged_attn(const void*, long, long, const void*, const void*,
                        const long*, const long*, const int*, const int*,
                        const int*, const int*, const int*, int, int, int, int,
-                       int, int, int, int, int, int, int, int, void*, float*,
+                       int, int, int, int, int, int, int, int, int, void*, float*,
                        float*, float, bool, hipStream_t);
 
 namespace {
@@ -1132,7 +1133,7 @@ torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
   TORCH_CHECK_VALUE((float)scale > 0 && std::isfinite((float)scale),
                     "paged_attention: softmax_scale must be positive and "
                     "finite");
-  int groups = 0, own, shared;
+  int groups = 0, own, shared, evenly;
   if (prefix_rows.has_value()) {
     group_rows = paged_ints(*prefix_rows, q, 1, "shared_prefix.rows");
     group_lengths = paged_ints(*prefix_lengths, q, 1, "shared_prefix.lengths");
@@ -1155,7 +1156,7 @@ torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
                     (int)std::max(std::min(longest, room), 1l),
                     groups, (int)max_rows,
                     std::min(std::max(max_prefix, 0l), 1l << 30), &own,
-                    &shared);
+                    &shared, &evenly);
   const int pieces = own + shared;
   torch::Tensor part;
   if (pieces > 1)
@@ -1171,7 +1172,8 @@ torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
                     groups ? group_rows.data_ptr<int>() : nullptr,
                     groups ? group_lengths.data_ptr<int>() : nullptr, groups,
                     (int)max_rows, b, nh, ng, d, (int)k.size(0), page,
-                    (int)tables.size(1), count, own, shared, o.data_ptr(), po,
+                    (int)tables.size(1), count, own, shared, evenly,
+                    o.data_ptr(), po,
                     po ? po + (long)b * nh * pieces * d : nullptr,
                     (float)scale, fp16, cur_stream());
   return o;

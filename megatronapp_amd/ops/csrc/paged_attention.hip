@@ -50,11 +50,23 @@ struct Groups {
 };
 
 struct Out {
-  unsigned short* o;          // [b, nh, D], where there is one piece
+  unsigned short* o;          // [b, nh, D], of rows in one piece
   float* part;                // [b, nh, pieces, D]
   float* lse;                 // [b, nh, pieces]
-  int pieces;                 // of a row, the groups' ones last
+  int pieces;                 // of a row at most, the groups' ones first
+  int evenly;                 // into which a row is cut if it has the keys
+  int extra;                  // blocks for the pieces beyond that
 };
+
+// The pieces of a row's own keys: `evenly` for the sake of the card, but none
+// of fewer than LEAST keys, and more where they would have more than MOST.
+constexpr int LEAST = 256, MOST = 1024;
+
+__host__ __device__ constexpr int cuts(int keys, int evenly, int most) {
+  const int fill = std::min((keys + LEAST - 1) / LEAST, evenly);
+  const int n = std::max(fill, (keys + MOST - 1) / MOST);
+  return std::max(1, std::min(n, most));
+}
 
 // the page and the place in it of a token, at a multiple of 16
 __device__ __forceinline__ int page_of(const Cache& c, int token, int& in) {
@@ -122,6 +134,38 @@ __device__ __forceinline__ int pair_slot(int row, int slot) {
 }
 
 // --------------------------------------------------------- a row's own keys
+// the pieces of a row that no block of its own stands for
+__device__ __forceinline__ int extra_of(const Cache& c, const Groups& gr,
+                                        const Out& out, int row) {
+  const int len = length_at(c, slot_at(c, row));
+  return max(cuts(len - min(shared_at(c, gr, row), len), out.evenly,
+                  out.pieces - gr.pieces) - out.evenly, 0);
+}
+
+// The row and the piece of the index-th of these, or false behind the last.
+__device__ __forceinline__ bool find_extra(const Cache& c, const Groups& gr,
+                                           const Out& out, int index, int lane,
+                                           int& row, int& piece) {
+  for (int base = 0; base < gr.b; base += WAVE) {
+    const int own = base + lane < gr.b ? extra_of(c, gr, out, base + lane) : 0;
+    int sum = own;
+#pragma unroll
+    for (int off = 1; off < WAVE; off <<= 1) {
+      const int x = __shfl_up(sum, off, WAVE);
+      if (lane >= off) sum += x;
+    }
+    const int total = __builtin_amdgcn_readlane(sum, WAVE - 1);
+    if (index < total) {
+      const int at = __builtin_ctzll(__ballot(index < sum));
+      row = base + at;
+      piece = out.evenly + index - __builtin_amdgcn_readlane(sum - own, at);
+      return true;
+    }
+    index -= total;
+  }
+  return false;
+}
+
 // What a block's waves tell each other at the end.
 struct WaveSums {
   float m[4][HEADS], l[4][HEADS];
@@ -132,8 +176,8 @@ template <class T, int D>
 __device__ __forceinline__ void own_keys(const unsigned short* q, long qb,
                                          long qh, const Cache& c,
                                          const Groups& gr, const Out& out,
-                                         int nh, int ng, float scale,
-                                         unsigned block,
+                                         int nh, int ng, float scale, int hk,
+                                         int ht, int row, int piece,
                                          unsigned short* image,
                                          WaveSums& lds) {
   constexpr int NF = D / 32, ND = D / 16;
@@ -141,18 +185,17 @@ __device__ __forceinline__ void own_keys(const unsigned short* q, long qb,
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
-  const int rep = nh / ng, tiles = (rep + HEADS - 1) / HEADS;
-  const int pieces = out.pieces - gr.pieces;
-  const int hk = block % ng, ht = block / ng % tiles;
-  const int piece = block / ng / tiles % pieces;
-  const int row = block / ng / tiles / pieces;
+  const int rep = nh / ng;
   const int heads = min(HEADS, rep - ht * HEADS);
   const int head = hk * rep + ht * HEADS + min(n, heads - 1);
 
   const int slot = slot_at(c, row);
   const int len = length_at(c, slot);
   // this piece's keys
-  const int begin = min(shared_at(c, gr, row), len), own = len - begin;
+  const int shared = shared_at(c, gr, row);
+  const int begin = min(shared, len), own = len - begin;
+  const int pieces = cuts(own, out.evenly, out.pieces - gr.pieces);
+  if (piece >= pieces) return;
   const int per = ((own + pieces - 1) / pieces + KEYS - 1) / KEYS * KEYS;
   const int from = begin + min(piece * per, own);
   const int to = min(from + per, len);
@@ -322,16 +365,42 @@ __device__ __forceinline__ void own_keys(const unsigned short* q, long qb,
     const float by = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
     f32x4 y = *(f32x4*)(sums + hh * ROW + (d ^ ((hh & 7) << 2)));
     const long r = (long)row * nh + hk * rep + ht * HEADS + hh;
-    if (out.part) {
+    if (shared || pieces > 1) {
       f32x4 z = {y[0] * by, y[1] * by, y[2] * by, y[3] * by};
-      *(f32x4*)(out.part + (r * out.pieces + piece) * D + d) = z;
+      const long at = r * out.pieces + gr.pieces + piece;
+      *(f32x4*)(out.part + at * D + d) = z;
       if (d == 0)
-        out.lse[r * out.pieces + piece] =
+        out.lse[at] =
             ll == 0.f ? -INFINITY : mm + __builtin_amdgcn_logf(ll);
     } else {
       u32x2 z = {pack2<T>(y[0] * by, y[1] * by), pack2<T>(y[2] * by, y[3] * by)};
       *(u32x2*)(out.o + r * D + d) = z;
     }
+  }
+}
+
+// The first blocks take the extra pieces, which are of the longest rows.
+template <class T, int D>
+__device__ __forceinline__ void rows_block(const unsigned short* q, long qb,
+                                           long qh, const Cache& c,
+                                           const Groups& gr, const Out& out,
+                                           int nh, int ng, float scale,
+                                           unsigned block,
+                                           unsigned short* image,
+                                           WaveSums& sums) {
+  const int tiles = (nh / ng + HEADS - 1) / HEADS;
+  const bool extra = block < (unsigned)out.extra;
+  unsigned unit = extra ? block : block - out.extra;
+  for (;;) {
+    const int index = unit / ng / tiles;
+    int row = index / out.evenly, piece = index % out.evenly;
+    if (extra && !find_extra(c, gr, out, index, threadIdx.x & 63, row, piece))
+      return;
+    own_keys<T, D>(q, qb, qh, c, gr, out, nh, ng, scale, unit % ng,
+                   unit / ng % tiles, row, piece, image, sums);
+    if (!extra) return;
+    unit += out.extra;
+    __syncthreads();          // the sums are read, and their place is free
   }
 }
 
@@ -513,8 +582,7 @@ __device__ __forceinline__ void shared_keys(
     if (x0 + n < queries) {
       l = half_sum(l);
       const float by = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-      const long r = ((long)row * nh + head) * out.pieces + out.pieces -
-                     gr.pieces + piece;
+      const long r = ((long)row * nh + head) * out.pieces + piece;
       if (h == 0)
         out.lse[r] = l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l);
       float* dst = out.part + r * D + 4 * h;
@@ -536,8 +604,8 @@ __global__ __launch_bounds__(BLOCK, 2) void paged_rows_kernel(
     Out out, int nh, int ng, float scale) {
   __shared__ __attribute__((aligned(16))) unsigned short image[4 * KEYS * D];
   __shared__ WaveSums sums;
-  own_keys<T, D>(q, qb, qh, c, gr, out, nh, ng, scale, blockIdx.x, image,
-                 sums);
+  rows_block<T, D>(q, qb, qh, c, gr, out, nh, ng, scale, blockIdx.x, image,
+                   sums);
 }
 
 template <class T, int D>
@@ -553,8 +621,8 @@ __global__ __launch_bounds__(BLOCK, 2) void paged_groups_kernel(
     shared_keys<T, D>(q, qb, qh, c, gr, out, nh, ng, scale, blockIdx.x, img0,
                       img1);
   else
-    own_keys<T, D>(q, qb, qh, c, gr, out, nh, ng, scale,
-                   blockIdx.x - gr.blocks, img0, sums);
+    rows_block<T, D>(q, qb, qh, c, gr, out, nh, ng, scale,
+                     blockIdx.x - gr.blocks, img0, sums);
 }
 
 // -------------------------------------------------------------------- joining
@@ -570,11 +638,15 @@ __global__ __launch_bounds__(BLOCK) void paged_join_kernel(Cache c, Groups gr,
   const long r = (long)blockIdx.x * (BLOCK / WAVE) +
                  __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (r >= heads) return;
-  const float* lse = out.lse + r * out.pieces;
-  const float* part = out.part + r * out.pieces * D + d;
   // a row that shares nothing has no pieces of a group
-  const int pieces =
-      shared_at(c, gr, (int)(r / nh)) ? out.pieces : out.pieces - gr.pieces;
+  const int row = (int)(r / nh), len = length_at(c, slot_at(c, row));
+  const int shared = shared_at(c, gr, row), first = shared ? 0 : gr.pieces;
+  const int own = cuts(len - min(shared, len), out.evenly,
+                       out.pieces - gr.pieces);
+  if (!shared && own == 1) return;      // its block wrote o
+  const int pieces = gr.pieces - first + own;
+  const float* lse = out.lse + r * out.pieces + first;
+  const float* part = out.part + (r * out.pieces + first) * D + d;
   const float x0 = lane < pieces ? lse[lane] : -INFINITY;
   const float x1 = lane + WAVE < pieces ? lse[lane + WAVE] : -INFINITY;
   float mx = fmaxf(x0, x1);
@@ -613,22 +685,36 @@ __global__ __launch_bounds__(BLOCK) void paged_join_kernel(Cache c, Groups gr,
 
 }  // namespace
 
-// How the work is cut: pieces of a row's own keys, and of its group's (none:
-// every row reads its shared pages for itself).
+// How the work is cut: pieces of a row's own keys, at most and in general, and
+// of its group's (none: every row reads its shared pages for itself).
 //
 // A group's blocks run beside the rows' ones, one of each on a CU where there
 // are enough; both should end together.  A step of 64 keys of a group's block
 // takes the time in which the card reads some 9 MB of rows' own keys at D = 128
 // (half of that at 64), and rows are taken to have half of the longest one's
-// own keys; four steps are worth a piece.  256 rows on 16384 + 1..1024 tokens: 257, 185, 171, 186, 206
-// us in 2, 3, 4, 6, 8 pieces; 64 rows on 4096 + 33..700: 58, 48, 39, 40, 46 us
-// in 3, 4, 6, 8, 16.  Rows that read little more than SHARE bytes of shared
-// keys in all, mostly out of L2, are done sooner each for itself (24 rows in
-// four groups, 51 MB: 13 us against 16; 16 rows, 134 MB: 24 us against 17).
+// own keys; four steps are worth a piece.  256 rows on 16384 + 1..1024 tokens:
+// 257, 185, 171, 186, 206 us in 2, 3, 4, 6, 8 pieces; 64 rows on 4096 +
+// 33..700: 58, 48, 39, 40, 46 us in 3, 4, 6, 8, 16.  Rows that read little
+// more than SHARE bytes of shared keys in all, mostly out of L2, are done
+// sooner each for itself (24 rows in four groups, 51 MB: 13 us against 16; 16
+// rows, 134 MB: 24 us against 17).
+//
+// Rows in general are cut until there are two blocks for each of 256 CUs: at
+// 8 key heads 16 rows on 4096 tokens take 96, 59, 53, 57 us in 1, 2, 4, 8
+// pieces, 64 rows on 1024 at D = 64 27, 32, 39 us in 1, 2, 4.  Keys fewer than
+// LEAST are worth no piece: one row on 500 takes 8 us in one and 11 in two and
+// joined, 8 rows on 1024 14.5 us in pieces of 256, 15.8 in ones of 512.  Above
+// MOST keys a row is cut again, which only its own length decides: 64 rows on
+// 0, 100 .. 6300 tokens take 244, 158, 160, 164 us at MOST = 4096, 2048, 1024,
+// 512, 63 rows on 100 beside one on 8100 39, 27, 27 us at 2048, 1024, 512.
+// These pieces have no blocks of their own, which would mostly find nothing to
+// do: 512 blocks share them out.  With a block for every piece that a row may
+// have, 128 rows on 200 tokens beside one on 60000 take 114 us, and 86 so.
+// ROOM bounds the memory that the pieces take.
 void paged_attn_pieces(int b, int nh, int ng, int d, int max_length,
                        int groups, int max_rows, long max_prefix, int* own,
-                       int* shared) {
-  constexpr long SHARE = 96l << 20;
+                       int* shared, int* evenly) {
+  constexpr long SHARE = 96l << 20, FILL = 512, ROOM = 64l << 20;
   const long blocks = (long)b * ng * ((nh / ng + HEADS - 1) / HEADS);
   *shared = 0;
   long most = max_length;
@@ -646,9 +732,12 @@ void paged_attn_pieces(int b, int nh, int ng, int d, int max_length,
     *shared = (int)std::max(
         1l, std::min(std::min((steps + per - 1) / per, room / units), 64l));
   }
-  const long fill = ((*shared ? 512 : 1024) + blocks - 1) / blocks;
-  most = (most + 4 * KEYS - 1) / (4 * KEYS);
-  *own = (int)std::max(1l, std::min(std::min(fill, most), 64l));
+  *evenly = 1;
+  while (*evenly < 64 && blocks * *evenly < FILL) *evenly *= 2;
+  const long part = ROOM / ((long)b * nh * (d + 1) * 4);
+  *own = cuts((int)most, *evenly,
+              (int)std::max((long)*evenly, std::min(part, 64l)));
+  *evenly = std::min(*evenly, *own);
 }
 
 void launch_paged_attn(const void* q, long qb, long qh, const void* k,
@@ -657,18 +746,19 @@ void launch_paged_attn(const void* q, long qb, long qh, const void* k,
                        const int* group_rows, const int* group_lengths,
                        int groups, int max_rows, int b, int nh, int ng, int d,
                        int pages, int page, int width, int count, int own,
-                       int shared, void* o, float* part, float* lse,
+                       int shared, int evenly, void* o, float* part, float* lse,
                        float scale, bool fp16, hipStream_t stream) {
   const unsigned long p16 = page / 16;
   const Cache c = {(const unsigned short*)k, (const unsigned short*)v, tables,
                    lengths, slots, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
                    pages, page, width, count, ((1ul << 32) + p16 - 1) / p16};
-  const Out out = {(unsigned short*)o, part, lse, own + shared};
+  const long units = (long)b * ng * ((nh / ng + HEADS - 1) / HEADS);
+  const int extra = (int)std::min(units * (own - evenly), 512l);
+  const Out out = {(unsigned short*)o, part, lse, own + shared, evenly, extra};
   const int tiles =
       (int)std::max(1l, ((long)max_rows * (nh / ng) + BM - 1) / BM);
   const long first = shared ? (long)groups * tiles * ng * shared : 0;
-  const long blocks =
-      first + (long)b * own * ng * ((nh / ng + HEADS - 1) / HEADS);
+  const long blocks = first + extra + units * evenly;
   const long heads = (long)b * nh, each = BLOCK / WAVE;
   if (blocks * BLOCK >= 1l << 32 || heads * WAVE >= 1l << 32)
     throw std::runtime_error("paged attention: too many rows for one launch");

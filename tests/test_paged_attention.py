@@ -459,3 +459,26 @@ def test_refusals_on_the_gpu():
         paged_attention(q.float(), k.float(), v.float(), tables, lengths)
     assert paged_attention(q[:0], k, v, tables[:1], lengths[:1],
                            slots=lengths[:0]).shape == (0, 4, 64)
+
+
+# ------------------------------------------------------------------ pieces
+@gpu
+@pytest.mark.parametrize("n", [8200, 8600, 9000, 9200])
+def test_many_pieces_of_a_row(n):
+    """33 to 36 pieces of 256 keys."""
+    _check([n], nh=2, ng=1, d=128)
+    _check([n], nh=16, ng=16, d=64)
+
+
+@gpu
+@pytest.mark.parametrize("nh,ng,d", [(32, 32, 64), (40, 8, 128)])
+def test_long_rows_among_short_ones(nh, ng, d):
+    """A row's length alone gives it further pieces, which lie with other
+    rows' ones in blocks that they share."""
+    lens = [1 + 7 * i % 90 for i in range(140)]
+    for i, n in ((0, 5000), (63, 1025), (64, 2048), (65, 2049), (139, 12345)):
+        lens[i] = n
+    s = _state(lens, nh=nh, ng=ng, d=d)
+    want = oracle(*s)
+    for most in (None, 1, 3000):      # only the time depends on it
+        _near(paged_attention(*s, max_length=most), want, most)
