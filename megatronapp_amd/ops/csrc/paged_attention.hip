@@ -379,8 +379,11 @@ __device__ __forceinline__ void own_keys(const unsigned short* q, long qb,
   }
 }
 
-// The first blocks take the extra pieces, which are of the longest rows.
-template <class T, int D>
+// The first blocks take the extra pieces, which are of the longest rows.  A
+// launch without any has a kernel of its own, with fewer registers (at D = 64
+// 104 and four blocks on a CU, not 130 and three: 256 rows on 0..300 tokens
+// 17 us against 19).
+template <class T, int D, bool EXTRA>
 __device__ __forceinline__ void rows_block(const unsigned short* q, long qb,
                                            long qh, const Cache& c,
                                            const Groups& gr, const Out& out,
@@ -389,17 +392,20 @@ __device__ __forceinline__ void rows_block(const unsigned short* q, long qb,
                                            unsigned short* image,
                                            WaveSums& sums) {
   const int tiles = (nh / ng + HEADS - 1) / HEADS;
-  const bool extra = block < (unsigned)out.extra;
-  unsigned unit = extra ? block : block - out.extra;
-  for (;;) {
+  if (!EXTRA || block >= (unsigned)out.extra) {
+    const unsigned unit = EXTRA ? block - out.extra : block;
     const int index = unit / ng / tiles;
-    int row = index / out.evenly, piece = index % out.evenly;
-    if (extra && !find_extra(c, gr, out, index, threadIdx.x & 63, row, piece))
-      return;
+    own_keys<T, D>(q, qb, qh, c, gr, out, nh, ng, scale, unit % ng,
+                   unit / ng % tiles, index / out.evenly, index % out.evenly,
+                   image, sums);
+    return;
+  }
+  int row, piece;
+  for (unsigned unit = block;
+       find_extra(c, gr, out, unit / ng / tiles, threadIdx.x & 63, row, piece);
+       unit += out.extra) {
     own_keys<T, D>(q, qb, qh, c, gr, out, nh, ng, scale, unit % ng,
                    unit / ng % tiles, row, piece, image, sums);
-    if (!extra) return;
-    unit += out.extra;
     __syncthreads();          // the sums are read, and their place is free
   }
 }
@@ -598,14 +604,14 @@ __device__ __forceinline__ void shared_keys(
   }
 }
 
-template <class T, int D>
+template <class T, int D, bool EXTRA>
 __global__ __launch_bounds__(BLOCK, 2) void paged_rows_kernel(
     const unsigned short* __restrict__ q, long qb, long qh, Cache c, Groups gr,
     Out out, int nh, int ng, float scale) {
   __shared__ __attribute__((aligned(16))) unsigned short image[4 * KEYS * D];
   __shared__ WaveSums sums;
-  rows_block<T, D>(q, qb, qh, c, gr, out, nh, ng, scale, blockIdx.x, image,
-                   sums);
+  rows_block<T, D, EXTRA>(q, qb, qh, c, gr, out, nh, ng, scale, blockIdx.x,
+                          image, sums);
 }
 
 template <class T, int D>
@@ -621,8 +627,8 @@ __global__ __launch_bounds__(BLOCK, 2) void paged_groups_kernel(
     shared_keys<T, D>(q, qb, qh, c, gr, out, nh, ng, scale, blockIdx.x, img0,
                       img1);
   else
-    rows_block<T, D>(q, qb, qh, c, gr, out, nh, ng, scale,
-                     blockIdx.x - gr.blocks, img0, sums);
+    rows_block<T, D, true>(q, qb, qh, c, gr, out, nh, ng, scale,
+                           blockIdx.x - gr.blocks, img0, sums);
 }
 
 // -------------------------------------------------------------------- joining
@@ -771,10 +777,16 @@ void launch_paged_attn(const void* q, long qb, long qh, const void* k,
                          dim3((unsigned)blocks), dim3(BLOCK), 0, stream,    \
                          (const unsigned short*)q, qb, qh, c, gr, out, nh,  \
                          ng, scale * LOG2E);                                \
+    else if (extra)                                                         \
+      hipLaunchKernelGGL((paged_rows_kernel<T, DD, true>),                  \
+                         dim3((unsigned)blocks), dim3(BLOCK), 0, stream,    \
+                         (const unsigned short*)q, qb, qh, c, gr, out, nh,  \
+                         ng, scale * LOG2E);                                \
     else                                                                    \
-      hipLaunchKernelGGL((paged_rows_kernel<T, DD>), dim3((unsigned)blocks),\
-                         dim3(BLOCK), 0, stream, (const unsigned short*)q,  \
-                         qb, qh, c, gr, out, nh, ng, scale * LOG2E);        \
+      hipLaunchKernelGGL((paged_rows_kernel<T, DD, false>),                 \
+                         dim3((unsigned)blocks), dim3(BLOCK), 0, stream,    \
+                         (const unsigned short*)q, qb, qh, c, gr, out, nh,  \
+                         ng, scale * LOG2E);                                \
     HIP_CHECK_LAUNCH();                                                     \
     if (part) {                                                             \
       hipLaunchKernelGGL((paged_join_kernel<T, DD>),                        \
