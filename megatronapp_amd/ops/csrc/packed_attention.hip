@@ -156,6 +156,26 @@ __device__ __forceinline__ int head_of(int x, int ng, int rep) {
 }
 
 // ------------------------------------------------------------------ forward
+// A wave holds 32 rows of Q as the right operand of S^T = K Q^T, and P^T, which
+// that leaves in its registers, is the right operand of O^T = V^T P^T; the four
+// waves share the tiles of K and V, of which the next one comes into the other
+// of two images while one is used.  Two blocks of 252 registers at D = 128 and
+// three of 144 at 64 run on a CU, each at another place of its loop, so that
+// one's exponentials go beside the other's products.
+//
+// At D = 64 the vector unit bounds it (busy 64% of the time, the matrix unit
+// 28%): an element takes some six of its instructions and two products; 15
+// documents of 1 to 2048 tokens, 32 heads, take 149 us in training, 680
+// TFLOP/s.  At 128 both are near: 8192 + 5003 + 3001 + 188 tokens, 32 heads,
+// fp16 take 830 us, 1000 TFLOP/s, at the 1.8 GHz that the power allows.  Where
+// sequences are few and uneven, the longest tiles are more than a CU's share
+// of the work: ten prompts of 0 to 2048 tokens, 32 heads, 82 us (740), eight
+// documents of 45 to 2048, 16 heads, in training 74 us (710).
+//
+// Taken back: 64 rows a wave at D = 64 (half the reads of K and V: equal, for
+// short prompts 9.0 us against 7.5), four blocks of 128 registers there (149
+// us -> 159), the next tile's scores before this one's sums (spills), a higher
+// priority for the products (equal), images of K and V apart (equal).
 template <class T, int D, bool CAUSAL>
 __global__ __launch_bounds__(BLOCK, 2) void packed_fwd_kernel(
     const unsigned short* __restrict__ q, const unsigned short* __restrict__ k,
@@ -298,8 +318,17 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_fwd_kernel(
 }
 
 // ----------------------------------------------------------------- backward
-// dQ: rows of queries, over their keys.  Each row's D is found on the way, and
-// left for the other kernel.
+// dQ: rows of queries, over their keys, as in the forward.  S and dP are found
+// again; the other kernel's blocks could add dQ up, but only by atomics, whose
+// order changes results.  Each row's D is found on the way, and left for the
+// other kernel (a kernel of its own: backward 247 us, so 235).
+//
+// Eight documents of 45 to 2048 tokens, 16 heads of 128: 103 us, 760 TFLOP/s;
+// fifteen of 1 to 2048, 32 heads of 64: 198 us, 770.  The matrix unit is busy
+// a third of the time, the vector unit 27% at 128 and 47% at 64; two waves on
+// a SIMD do not cover more of each other's waits.  Eight waves on a tile, four
+// on every other 32 keys, keep all of a CU's waves in step: the backward takes
+// 280 us for 244, and 587 for 466.
 template <class T, int D, bool CAUSAL>
 __global__ __launch_bounds__(BLOCK, 2) void packed_bwd_dq_kernel(
     const unsigned short* __restrict__ q, const unsigned short* __restrict__ k,
@@ -427,7 +456,14 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_bwd_dq_kernel(
 // At D = 128 a wave's two sums alone take 128 registers.  So that two waves
 // still fit a SIMD, K's and V's fragments stay in LDS, and eight waves work on
 // the 128 keys: four on the first 32 queries of a tile, four on the others,
-// whose sums are added at the end.
+// whose sums are added at the end (one wave a SIMD: 228 us for 165 then, and
+// 546 for 361 at D = 64).
+//
+// The same documents as for dQ: 141 us, 740 TFLOP/s, and 268 us, 760.  Both
+// units are busy a third of the time, four tenths of it pass in waits, most
+// for LDS, where each 32 x 32 tile reads Q and dO along both axes.  Four waves
+// a block at D = 64, two blocks a CU, are 5% faster on the fifteen documents
+// and 3% slower on 8192 tokens; three or four waves a SIMD spill.
 template <int D>
 struct Dkv {
   static constexpr int HALVES = 2;

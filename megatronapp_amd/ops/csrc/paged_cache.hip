@@ -98,6 +98,11 @@ __device__ bool lowest_free(const Pool& p, int need, int* out, int* lds,
 // ---------------------------------------------------------------------- fork
 // plan[0]: whether to go on; then for each pair the parent's length, its
 // part-filled page and the page that takes its tokens (-1: none)
+//
+// Four beams of 201 tokens, 24 layers: 9.5 us, the latency of two launches that
+// wait for each other (one cannot do: a page may only be written once the whole
+// call is known to be sound).  63 samples of 8237 tokens, 32 layers: 121 us;
+// 743 MB would take 148 at a copy's 5.0 TB/s, but all read the same page.
 struct Pair {
   int length, from, to, pad;
 };
@@ -229,6 +234,9 @@ __global__ __launch_bounds__(BLOCK) void free_kernel(Pool p,
 // ------------------------------------------------------------------- compact
 // Live pages behind the first `live` places go to the holes among these, in
 // order.  moves[0]: how many; then (from, to) each; map: every page's place.
+//
+// 43 sequences of up to 2386 tokens in 1500 pages, 22 more retired, 16 layers:
+// 320 us, of which the plan 6; 1.52 GB at 4.8 TB/s, near a copy's 5.0.
 __global__ __launch_bounds__(PLAN) void compact_plan_kernel(Pool p, int* map,
                                                             int* moves,
                                                             int* movers) {
