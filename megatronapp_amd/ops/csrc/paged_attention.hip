@@ -172,7 +172,7 @@ __device__ __forceinline__ bool find_extra(const Cache& c, const Groups& gr,
 // LDS, out of which it is read transposed; the next step's loads are under way
 // while one is used, and page numbers come 64 at a time.  Memory bounds it: 32
 // rows of 2048 tokens, 8 key heads of 128, take 52 us, 5.1 TB/s; one row of
-// 8192 takes 18 us, mostly latencies of its pieces' 8 steps and of the join.
+// 8192 takes 17 us, mostly latencies of its pieces' 8 steps and of the join.
 // Steps of 64 keys at D = 64 lose 15%.
 
 // What a block's waves tell each other at the end.
@@ -198,7 +198,15 @@ __device__ __forceinline__ void own_keys(const unsigned short* q, long qb,
   const int heads = min(HEADS, rep - ht * HEADS);
   const int head = hk * rep + ht * HEADS + min(n, heads - 1);
 
+  // under way before the lengths are known: Q, and the first page numbers
+  typename T::x8 qf[NF];
+  const unsigned short* src = q + row * qb + head * qh + 8 * g;
+#pragma unroll
+  for (int f = 0; f < NF; ++f) qf[f] = *(const typename T::x8*)(src + 32 * f);
   const int slot = slot_at(c, row);
+  const int* table = c.tables + (long)max(0, min(slot, c.count - 1)) * c.width;
+  Pages ids = {0, -WAVE};
+  if (c.count > 0 && c.width > 0) ids = {table[min(lane, c.width - 1)], 0};
   const int len = length_at(c, slot);
   // this piece's keys
   const int shared = shared_at(c, gr, row);
@@ -208,19 +216,12 @@ __device__ __forceinline__ void own_keys(const unsigned short* q, long qb,
   const int per = ((own + pieces - 1) / pieces + KEYS - 1) / KEYS * KEYS;
   const int from = begin + min(piece * per, own);
   const int to = min(from + per, len);
-  const int* table = c.tables + (long)max(0, min(slot, c.count - 1)) * c.width;
-
-  typename T::x8 qf[NF];
-  const unsigned short* src = q + row * qb + head * qh + 8 * g;
-#pragma unroll
-  for (int f = 0; f < NF; ++f) qf[f] = *(const typename T::x8*)(src + 32 * f);
 
   f32x4 acc[ND];
 #pragma unroll
   for (int i = 0; i < ND; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, ms = 0.f, l = 0.f;
   unsigned short* img = image + wave * KEYS * D;
-  Pages ids = {0, -WAVE};
 
   typename T::x8 kn[2][NF];
   s16x8 vn[NV];
@@ -426,7 +427,7 @@ __device__ __forceinline__ void rows_block(const unsigned short* q, long qb,
 // rows' own keys, read beside them, cost little: 64 rows on 4096 + 33..700
 // tokens, 32/8 heads of 128, take 34 us (113 MB, 4.7 GFLOP) and the join 6;
 // 256 rows on 16384 + 1..1024 170 (611 MB, 71 GFLOP) and 8.  Each row for
-// itself: 91 and 1190.
+// itself, joined: 97 and 1190.
 template <class T, int D>
 __device__ __forceinline__ void shared_keys(
     const unsigned short* q, long qb, long qh, const Cache& c,
@@ -660,17 +661,27 @@ __global__ __launch_bounds__(BLOCK) void paged_join_kernel(Cache c, Groups gr,
   const long r = (long)blockIdx.x * (BLOCK / WAVE) +
                  __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (r >= heads) return;
+  // under way before it is known which of them there are: all the log-sums,
+  // and the first of the outputs
+  const float* lse = out.lse + r * out.pieces;
+  const float* part = out.part + r * out.pieces * D + d;
+  float x0 = lane < out.pieces ? lse[lane] : 0.f;
+  float x1 = lane + WAVE < out.pieces ? lse[lane + WAVE] : 0.f;
+  constexpr int AHEAD = 4;
+  f32x4 y[AHEAD];
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k)
+    y[k] = *(const f32x4*)(
+        part + (long)min(k * PARTS + lane / LANES, out.pieces - 1) * D);
   // a row that shares nothing has no pieces of a group
   const int row = (int)(r / nh), len = length_at(c, slot_at(c, row));
   const int shared = shared_at(c, gr, row), first = shared ? 0 : gr.pieces;
   const int own = cuts(len - min(shared, len), out.evenly,
                        out.pieces - gr.pieces);
   if (!shared && own == 1) return;      // its block wrote o
-  const int pieces = gr.pieces - first + own;
-  const float* lse = out.lse + r * out.pieces + first;
-  const float* part = out.part + (r * out.pieces + first) * D + d;
-  const float x0 = lane < pieces ? lse[lane] : -INFINITY;
-  const float x1 = lane + WAVE < pieces ? lse[lane + WAVE] : -INFINITY;
+  const int last = gr.pieces + own;
+  if (lane < first || lane >= last) x0 = -INFINITY;
+  if (lane + WAVE < first || lane + WAVE >= last) x1 = -INFINITY;
   float mx = fmaxf(x0, x1);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1)
@@ -682,17 +693,21 @@ __global__ __launch_bounds__(BLOCK) void paged_join_kernel(Cache c, Groups gr,
   for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off, WAVE);
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   // all lanes stay in: a lane that left would not hand over its weights
-#pragma unroll 4
-  for (int base = 0; base < pieces; base += PARTS) {
-    const int i = base + lane / LANES, last = pieces - 1;
+  auto add = [&](int i, const f32x4& z) __attribute__((always_inline)) {
     const float a = __shfl(w0, i & 63, WAVE), b = __shfl(w1, i & 63, WAVE);
     const float w = i < WAVE ? a : b;
-    const f32x4 y = *(const f32x4*)(part + (long)min(i, last) * D);
     // a piece of no keys adds nothing, nor does one that is not there
-    if (i < pieces && w != 0.f) {
+    if (i < last && w != 0.f) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] += w * y[j];
+      for (int j = 0; j < 4; ++j) o[j] += w * z[j];
     }
+  };
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) add(k * PARTS + lane / LANES, y[k]);
+#pragma unroll 4
+  for (int base = AHEAD * PARTS; base < last; base += PARTS) {
+    const int i = base + lane / LANES;
+    add(i, *(const f32x4*)(part + (long)min(i, last - 1) * D));
   }
 #pragma unroll
   for (int off = LANES; off < WAVE; off <<= 1)
