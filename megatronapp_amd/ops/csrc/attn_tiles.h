@@ -142,12 +142,32 @@ __device__ __forceinline__ void load_tile(unsigned short* dst,
   }
 }
 
-// A operand of 32x32x16: row tile_row(n) + row0, elements 16f + 8h ..
+// Where a lane reads in an image, in bytes: `rows` for its row n (or
+// tile_row(n)) as an operand of 32x32x16, `cols` for what the transposing reads
+// address.  All other places of a tile are these with some of the slot's bits
+// flipped and multiples of 16 rows added, which cost an instruction and
+// nothing.
+template <int D>
+struct Places {
+  unsigned rows, cols;
+  __device__ __forceinline__ Places(int lane, bool permuted = true) {
+    const int h = lane >> 5, n = lane & 31, r = permuted ? tile_row(n) : n;
+    rows = r * 2 * D + 16 * slot_of<D>(r, h);
+    const int c = 8 * h + ((lane >> 2) & 3);
+    cols = c * 2 * D +
+           16 * slot_of<D>(c, 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) +
+           8 * (lane & 1);
+  }
+};
+
+// operand of 32x32x16: the lane's row of those from row0 on, elements
+// 16f + 8h ..
 template <class T, int D>
 __device__ __forceinline__ typename T::x8 read_rows(const unsigned short* img,
-                                                    int row, int f, int h) {
-  return *(const typename T::x8*)(img + row * D +
-                                  8 * slot_of<D>(row, 2 * f + h));
+                                                    int row0, int f,
+                                                    const Places<D>& p) {
+  return *(const typename T::x8*)((const char*)img + row0 * 2 * D +
+                                  (p.rows ^ 32 * f));
 }
 
 // operand of 32x32x16 whose k are the image's rows row0 .. row0 + 15 and
@@ -155,15 +175,13 @@ __device__ __forceinline__ typename T::x8 read_rows(const unsigned short* img,
 template <class T, int D>
 __device__ __forceinline__ typename T::x8 read_cols(const unsigned short* img,
                                                     int row0, int c,
-                                                    int lane) {
+                                                    const Places<D>& p) {
   s16x8 v;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int row = row0 + 8 * (lane >> 5) + 4 * i + ((lane >> 2) & 3);
-    const int slot = 4 * c + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
     s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lds_s16x4*)(img + row * D + 8 * slot_of<D>(row, slot) +
-                     4 * (lane & 1)));
+        (lds_s16x4*)((const char*)img + (row0 + 4 * i) * 2 * D +
+                     (p.cols ^ (64 * c + 16 * i))));
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[4 * i + j] = x[j];
   }

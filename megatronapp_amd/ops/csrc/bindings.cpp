@@ -117,11 +117,12 @@ void launch_packed_attn_fwd(const void*, const void*, const void*, void*,
                             void*, float*, const int*, const int*, int, int, int, int,
                             int, int, int, float, bool, bool, const long*,
                             const long*, const long*, hipStream_t);
+int packed_attn_shares(int, int, int, int, int, int, int, long*);
 void launch_packed_attn_bwd(const void*, const void*, const void*,
                             const void*, const void*, const void*,
-                            const float*, float*, void*, void*, void*,
-                            const int*, const int*, int,
-                            int, int, int, int, int, int, float, bool, bool,
+                            const float*, float*, void*, void*, void*, float*,
+                            int, const int*, const int*, int, int, int, int,
+                            int, int, int, float, bool, bool,
                             const long*, const long*, const long*, const long*,
                             hipStream_t);
 
@@ -899,11 +900,17 @@ std::vector<torch::Tensor> packed_attn_bwd(
        kr = packed_rows(k, ks), vr = packed_rows(v, vs);
   const torch::Tensor iq = int32_row(cu_q),
                       ik = cu_k.is_same(cu_q) ? iq : int32_row(cu_k);
+  long floats = 0;
+  const int shares = packed_attn_shares(s.n, s.tq, s.tk, s.b, s.nh, s.ng, s.d,
+                                        &floats);
+  torch::Tensor sums;
+  if (floats) sums = torch::empty({floats}, q.options().dtype(torch::kFloat32));
   launch_packed_attn_bwd(
       dr.data_ptr(), qr.data_ptr(), kr.data_ptr(), vr.data_ptr(), o.data_ptr(),
       low.data_ptr(), lse.data_ptr<float>(), dot.data_ptr<float>(), dq.data_ptr(),
-      dk.data_ptr(), dv.data_ptr(), iq.data_ptr<int>(), ik.data_ptr<int>(),
-      s.n, s.tq, s.tk, s.b, s.nh, s.ng, s.d, (float)scale, causal, s.fp16, os,
+      dk.data_ptr(), dv.data_ptr(),
+      floats ? sums.data_ptr<float>() : nullptr, shares,
+      iq.data_ptr<int>(), ik.data_ptr<int>(), s.n, s.tq, s.tk, s.b, s.nh, s.ng, s.d, (float)scale, causal, s.fp16, os,
       qs, ks, vs, cur_stream());
   return {dq, dk, dv};
 }

@@ -19,6 +19,8 @@
 
 #include "attn_tiles.h"
 
+#include <algorithm>
+
 namespace {
 
 constexpr int BM = 128;     // rows of a block: four waves of 32
@@ -159,13 +161,13 @@ __device__ __forceinline__ int head_of(int x, int ng, int rep) {
 // A wave holds 32 rows of Q as the right operand of S^T = K Q^T, and P^T, which
 // that leaves in its registers, is the right operand of O^T = V^T P^T; the four
 // waves share the tiles of K and V, of which the next one comes into the other
-// of two images while one is used.  Two blocks of 252 registers at D = 128 and
-// three of 144 at 64 run on a CU, each at another place of its loop, so that
-// one's exponentials go beside the other's products.
+// of two images while one is used.  Two blocks of 227 registers at D = 128 and
+// four of 120 at 64 run on a CU, each at another place of its loop, so that one
+// does its exponentials beside the other's products.
 //
 // At D = 64 the vector unit bounds it (busy 64% of the time, the matrix unit
 // 28%): an element takes some six of its instructions and two products; 15
-// documents of 1 to 2048 tokens, 32 heads, take 149 us in training, 680
+// documents of 1 to 2048 tokens, 32 heads, take 146 us in training, 700
 // TFLOP/s.  At 128 both are near: 8192 + 5003 + 3001 + 188 tokens, 32 heads,
 // fp16 take 830 us, 1000 TFLOP/s, at the 1.8 GHz that the power allows.  Where
 // sequences are few and uneven, the longest tiles are more than a CU's share
@@ -173,9 +175,9 @@ __device__ __forceinline__ int head_of(int x, int ng, int rep) {
 // documents of 45 to 2048, 16 heads, in training 74 us (710).
 //
 // Taken back: 64 rows a wave at D = 64 (half the reads of K and V: equal, for
-// short prompts 9.0 us against 7.5), four blocks of 128 registers there (149
-// us -> 159), the next tile's scores before this one's sums (spills), a higher
-// priority for the products (equal), images of K and V apart (equal).
+// short prompts 9.0 us against 7.5), the next tile's scores before this one's
+// sums (spills), a higher priority for the products (equal), images of K and V
+// apart (equal).
 template <class T, int D, bool CAUSAL>
 __global__ __launch_bounds__(BLOCK, 2) void packed_fwd_kernel(
     const unsigned short* __restrict__ q, const unsigned short* __restrict__ k,
@@ -187,6 +189,7 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_fwd_kernel(
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, n = lane & 31;
+  const Places<D> at_lane(lane);
   Span s;
   const unsigned x = blockIdx.x % (b * nh), slot = blockIdx.x / (b * nh);
   if (!find_span<false>(pk, slot, lane, s)) return;
@@ -237,10 +240,10 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_fwd_kernel(
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       st[u] = zeros16();
-      const int kr = 32 * u + tile_row(n);
 #pragma unroll
       for (int f = 0; f < NF; ++f)
-        st[u] = T::mfma32(read_rows<T, D>(img, kr, f, h), qf[f], st[u]);
+        st[u] = T::mfma32(read_rows<T, D>(img, 32 * u, f, at_lane), qf[f],
+                            st[u]);
     }
     reads_ahead<2 * NF, 1>();
     if (at + BN > wave_least) {
@@ -283,8 +286,8 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_fwd_kernel(
         const typename T::x8 pf = pack8<T>(st[u], 8 * x);
 #pragma unroll
         for (int i = 0; i < ND; ++i)
-          acc[i] = T::mfma32(read_cols<T, D>(vi, 32 * u + 16 * x, i, lane), pf,
-                             acc[i]);
+          acc[i] = T::mfma32(read_cols<T, D>(vi, 32 * u + 16 * x, i, at_lane),
+                             pf, acc[i]);
       }
   };
   // one tile is used while the next one comes in
@@ -344,6 +347,7 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_bwd_dq_kernel(
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, n = lane & 31;
+  const Places<D> at_lane(lane);
   Span s;
   const unsigned x = blockIdx.x % (b * nh), slot = blockIdx.x / (b * nh);
   if (!find_span<false>(pk, slot, lane, s)) return;
@@ -407,11 +411,10 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_bwd_dq_kernel(
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       f32x16 st = zeros16(), dp = zeros16();
-      const int kr = 32 * u + tile_row(n);
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
-        st = T::mfma32(read_rows<T, D>(img, kr, f, h), qf[f], st);
-        dp = T::mfma32(read_rows<T, D>(vi, kr, f, h), df[f], dp);
+        st = T::mfma32(read_rows<T, D>(img, 32 * u, f, at_lane), qf[f], st);
+        dp = T::mfma32(read_rows<T, D>(vi, 32 * u, f, at_lane), df[f], dp);
       }
       reads_ahead<2 * NF, 1>();
 #pragma unroll
@@ -428,8 +431,8 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_bwd_dq_kernel(
         const typename T::x8 sf = pack8<T>(dp, 8 * x);
 #pragma unroll
         for (int i = 0; i < ND; ++i)
-          acc[i] = T::mfma32(read_cols<T, D>(img, 32 * u + 16 * x, i, lane),
-                             sf, acc[i]);
+          acc[i] = T::mfma32(
+              read_cols<T, D>(img, 32 * u + 16 * x, i, at_lane), sf, acc[i]);
       }
     }
   };
@@ -471,14 +474,17 @@ struct Dkv {
   static constexpr int WAVES = 4 * HALVES;
 };
 
+template <int D>
+constexpr long SHARE = BM * D / 4;    // of four numbers: one tile's dK (or dV)
+
 template <class T, int D, bool CAUSAL>
 __global__ __launch_bounds__(Dkv<D>::WAVES * 64, 2) void packed_bwd_dkv_kernel(
     const unsigned short* __restrict__ q, const unsigned short* __restrict__ k,
     const unsigned short* __restrict__ v,
     const unsigned short* __restrict__ dout, const float* __restrict__ lse,
     const float* __restrict__ dot, unsigned short* __restrict__ dk,
-    unsigned short* __restrict__ dv, Packing pk, int b, int nh, int ng,
-    float scale, Strides qs, Strides ks, Strides vs, Strides os) {
+    unsigned short* __restrict__ dv, float* __restrict__ sums, int shares,
+    Packing pk, int b, int nh, int ng, float scale, Strides qs, Strides ks, Strides vs, Strides os) {
   constexpr int HALVES = Dkv<D>::HALVES, WAVES = Dkv<D>::WAVES;
   constexpr int BQ = Dkv<D>::BQ;
   constexpr bool KV_LDS = D == 128;
@@ -492,10 +498,11 @@ __global__ __launch_bounds__(Dkv<D>::WAVES * 64, 2) void packed_bwd_dkv_kernel(
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int part = wave & 3, half = wave >> 2;
   const int h = lane >> 5, n = lane & 31;
+  const Places<D> at_lane(lane);
   Span s;
-  const unsigned x = blockIdx.x % (b * ng);
-  if (!find_span<true>(pk, blockIdx.x / (b * ng), lane, s)) return;
-  const int bi = x / ng, hk = x % ng, rep = nh / ng;
+  const unsigned x = blockIdx.x % (b * ng * shares);
+  if (!find_span<true>(pk, blockIdx.x / (b * ng * shares), lane, s)) return;
+  const int hk = x % ng, bi = x / ng % b, share = x / ng / b, rep = nh / ng;
   const float c = scale * LOG2E;
 
   const int j0 = s.tile * BM + part * 32;       // the wave's first key
@@ -520,19 +527,23 @@ __global__ __launch_bounds__(Dkv<D>::WAVES * 64, 2) void packed_bwd_dkv_kernel(
       vf[f] = *(const typename T::x8*)(vsrc + 16 * f + 8 * h);
     }
   }
+  const Places<D> kv_lane(lane, false);
   auto k_frag = [&](int f) __attribute__((always_inline)) {
-    if constexpr (KV_LDS) return read_rows<T, D>(kv_lds, 32 * part + n, f, h);
+    if constexpr (KV_LDS) return read_rows<T, D>(kv_lds, 32 * part, f, kv_lane);
     else return kf[f];
   };
   auto v_frag = [&](int f) __attribute__((always_inline)) {
     if constexpr (KV_LDS)
-      return read_rows<T, D>(kv_lds + BM * D, 32 * part + n, f, h);
+      return read_rows<T, D>(kv_lds + BM * D, 32 * part, f, kv_lane);
     else return vf[f];
   };
   // the first query that sees the block's first key
   const int ahead = CAUSAL ? s.sk - s.sq : 0;
   const int first = CAUSAL ? max(0, s.tile * BM - ahead) / BQ : 0;
   const int per = max(0, (s.sq + BQ - 1) / BQ - first);
+  // the block's share of the heads' tiles
+  const int begin = rep * per * share / shares;
+  int left = rep * per * (share + 1) / shares - begin;
 
   f32x16 ak[ND], av[ND];
 #pragma unroll
@@ -567,11 +578,10 @@ __global__ __launch_bounds__(Dkv<D>::WAVES * 64, 2) void packed_bwd_dkv_kernel(
     const float* sl = (const float*)(img + 2 * BQ * D) + 32 * u + 8 * h;
     const float* sd = sl + BQ;
     f32x16 st = zeros16(), dp = zeros16();
-    const int qr = 32 * u + tile_row(n);
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
-      st = T::mfma32(read_rows<T, D>(img, qr, f, h), k_frag(f), st);
-      dp = T::mfma32(read_rows<T, D>(di, qr, f, h), v_frag(f), dp);
+      st = T::mfma32(read_rows<T, D>(img, 32 * u, f, at_lane), k_frag(f), st);
+      dp = T::mfma32(read_rows<T, D>(di, 32 * u, f, at_lane), v_frag(f), dp);
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -592,15 +602,16 @@ __global__ __launch_bounds__(Dkv<D>::WAVES * 64, 2) void packed_bwd_dkv_kernel(
       const typename T::x8 sf = pack8<T>(dp, 8 * y);
 #pragma unroll
       for (int i = 0; i < ND; ++i) {
-        av[i] = T::mfma32(read_cols<T, D>(di, 32 * u + 16 * y, i, lane), pf,
-                          av[i]);
-        ak[i] = T::mfma32(read_cols<T, D>(img, 32 * u + 16 * y, i, lane), sf,
-                          ak[i]);
+        av[i] = T::mfma32(read_cols<T, D>(di, 32 * u + 16 * y, i, at_lane),
+                          pf, av[i]);
+        ak[i] = T::mfma32(read_cols<T, D>(img, 32 * u + 16 * y, i, at_lane),
+                          sf, ak[i]);
       }
     }
   };
   // one tile is used while the next one comes in
-  int r1 = 0, t1 = 0;             // the next tile's head and number
+  int r1 = left ? begin / per : 0;    // the next tile's head and number
+  int t1 = left ? begin % per : 0;
   auto turn = [&](int at, unsigned short* img, unsigned short* next)
                   __attribute__((always_inline)) {
     __builtin_amdgcn_s_waitcnt(0x0f70);         // vmcnt(0)
@@ -609,16 +620,16 @@ __global__ __launch_bounds__(Dkv<D>::WAVES * 64, 2) void packed_bwd_dkv_kernel(
       t1 = 0;
       ++r1;
     }
-    if (r1 < rep) fetch(r1, (first + t1) * BQ, next);
+    if (--left) fetch(r1, (first + t1) * BQ, next);
     if (j0 >= s.sk) return;
 #pragma unroll
     for (int u = 0; u < BQ / 32 / HALVES; ++u)
       part_step(at, HALVES * u + half, img);
   };
-  if (per > 0) fetch(0, first * BQ, qd0_lds);
-  while (per > 0 && r1 < rep) {
+  if (left) fetch(r1, (first + t1) * BQ, qd0_lds);
+  while (left) {
     turn((first + t1) * BQ, qd0_lds, qd1_lds);
-    if (r1 < rep) turn((first + t1) * BQ, qd1_lds, qd0_lds);
+    if (left) turn((first + t1) * BQ, qd1_lds, qd0_lds);
   }
   if constexpr (HALVES == 2) {
     // the second half's sums, handed over through the images
@@ -645,6 +656,24 @@ __global__ __launch_bounds__(Dkv<D>::WAVES * 64, 2) void packed_bwd_dkv_kernel(
     hand_over(av);
     if (half) return;
   }
+  if (shares > 1) {           // left as the registers hold them
+    const long unit = (long)(blockIdx.x / (b * ng * shares)) * (b * ng) + bi *
+                      ng + hk;
+    f32x4* to = (f32x4*)sums + (unit * shares + share) * 2 * SHARE<D> +
+                part * 4 * ND * WAVE + lane;
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const f32x4 a = {ak[i][4 * y], ak[i][4 * y + 1], ak[i][4 * y + 2],
+                         ak[i][4 * y + 3]};
+        const f32x4 v = {av[i][4 * y], av[i][4 * y + 1], av[i][4 * y + 2],
+                         av[i][4 * y + 3]};
+        to[(4 * i + y) * WAVE] = a;
+        to[SHARE<D> + (4 * i + y) * WAVE] = v;
+      }
+    return;
+  }
   if (j >= s.sk) return;
   const long at = ((row * b + bi) * ng + hk) * D;
 #pragma unroll
@@ -652,6 +681,39 @@ __global__ __launch_bounds__(Dkv<D>::WAVES * 64, 2) void packed_bwd_dkv_kernel(
     store_cols<T>(dk + at + 32 * i, ak[i], scale, h);
     store_cols<T>(dv + at + 32 * i, av[i], 1.f, h);
   }
+}
+
+// The shares' sums of a tile's dK and dV, added up in order: a wave for 32 keys
+// and 32 columns of one of them.
+template <class T, int D>
+__global__ __launch_bounds__(BLOCK) void packed_bwd_add_kernel(
+    const float* __restrict__ sums, unsigned short* __restrict__ dk,
+    unsigned short* __restrict__ dv, int shares, Packing pk, int b, int ng,
+    float scale) {
+  constexpr int ND = D / 32;
+  const int lane = threadIdx.x & 63;
+  const int part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = blockIdx.y % ND, second = blockIdx.y / ND;
+  const f32x4* from = (const f32x4*)sums +
+                      ((long)blockIdx.x * shares * 2 + second) * SHARE<D> +
+                      (part * ND + i) * 4 * WAVE + lane;
+  Span s;
+  const unsigned x = blockIdx.x % (b * ng);
+  if (!find_span<true>(pk, blockIdx.x / (b * ng), lane, s)) return;
+  f32x16 acc = zeros16();
+#pragma unroll 4
+  for (int k = 0; k < shares; ++k)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const f32x4 z = from[k * 2 * SHARE<D> + y * WAVE];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[4 * y + e] += z[e];
+    }
+  const int j = s.tile * BM + part * 32 + (lane & 31);
+  if (j >= s.sk) return;
+  store_cols<T>((second ? dv : dk) +
+                    ((long)(s.k0 + j) * b * ng + x) * D + 32 * i,
+                acc, second ? 1.f : scale, lane >> 5);
 }
 
 // each sequence may end in a part of a tile
@@ -697,10 +759,37 @@ void launch_packed_attn_fwd(const void* q, const void* k, const void* v,
   HIP_CHECK_LAUNCH();
 }
 
+// Into how many shares a tile's work for dK and dV is cut, so that there are
+// two blocks for each of 256 CUs (of a causal mask's tiles the first has twice
+// the average to do), but none of fewer than two tiles of queries; where every
+// CU has a block already, only long sequences are.  Sequences are taken to be
+// of one length.  The shares' sums are written and read once more, in 32 bits,
+// at most some 130 MB.
+//
+// Backward in one share and so, us: 4096 tokens, 32/8 heads of 128 655 and 502
+// (four shares: 522), of 64 370 and 283; 16384 tokens, 8/2 heads of 128 2540
+// and 1850; 1024 tokens, 32/8 heads of 128 151 and 84; 8192 tokens, 8/1 heads
+// of 128 1950 and 590; 4096 tokens, 8 heads of 128 233 and 212.  In two shares
+// all the same: 2048 tokens, 16 heads of 128 126 and 130, five sequences of
+// 6921 tokens, 32/8 heads of 64 228 and 256.
+int packed_attn_shares(int n, int tq, int tk, int b, int nh, int ng, int d,
+                       long* floats) {
+  constexpr long FILL = 512, LEAST = 2;
+  const long blocks = (long)b * ng * (tk / BM + (n + 1) / 2);
+  const int bq = d == 128 ? Dkv<128>::BQ : Dkv<64>::BQ;
+  const long tiles = (long)(nh / ng) * (tq / std::max(n, 1)) / (2 * bq);
+  long fill = (FILL + blocks / 2) / std::max(blocks, 1l);
+  if (blocks >= FILL / 2 && tiles < d * 3 / 16) fill = 1;
+  const long shares = std::max(1l, std::min(std::min(fill, tiles / LEAST), 8l));
+  *floats = shares > 1 ? (long)b * ng * ((long)tk / BM + n + 2) * shares * 2 *
+                             BM * d : 0;
+  return (int)shares;
+}
+
 void launch_packed_attn_bwd(const void* dout, const void* q, const void* k,
                             const void* v, const void* o, const void* low,
-                            const float* lse, float* dot, void* dq, void* dk, void* dv,
-                            const int* cu_q, const int* cu_k, int n, int tq,
+                            const float* lse, float* dot, void* dq, void* dk,
+                            void* dv, float* sums, int shares, const int* cu_q, const int* cu_k, int n, int tq,
                             int tk, int b, int nh, int ng, int d, float scale,
                             bool causal, bool fp16, const long* os,
                             const long* qs, const long* ks, const long* vs,
@@ -724,16 +813,27 @@ void launch_packed_attn_bwd(const void* dout, const void* q, const void* k,
     HIP_CHECK_LAUNCH();
   }
   if (tk > 0) {
-    const dim3 grid = grid_for((long)b * ng, tk, n);
+    const dim3 grid = grid_for((long)b * ng * shares, tk, n);
 #define RUN(T, DD, CC)                                                       \
   hipLaunchKernelGGL((packed_bwd_dkv_kernel<T, DD, CC>),                     \
                      grid, dim3(Dkv<DD>::WAVES * 64), 0, stream,             \
                      (const unsigned short*)q, (const unsigned short*)k,     \
                      (const unsigned short*)v, (const unsigned short*)dout,  \
-                     lse, dot, (unsigned short*)dk, (unsigned short*)dv, pk, \
-                     b, nh, ng, scale, sq, sk, sv, so)
+                     lse, dot, (unsigned short*)dk, (unsigned short*)dv,     \
+                     sums, shares, pk, b, nh, ng, scale, sq, sk, sv, so)
     PACKED_DISPATCH(RUN);
 #undef RUN
     HIP_CHECK_LAUNCH();
+    if (shares > 1) {
+      const dim3 tiles(grid_for((long)b * ng, tk, n).x, d / 16);
+#define ADD(T, DD)                                                           \
+  hipLaunchKernelGGL((packed_bwd_add_kernel<T, DD>), tiles, dim3(BLOCK), 0,  \
+                     stream, sums, (unsigned short*)dk, (unsigned short*)dv, \
+                     shares, pk, b, ng, scale)
+      if (fp16) { if (d == 128) ADD(Fp16, 128); else ADD(Fp16, 64); }
+      else { if (d == 128) ADD(Bf16, 128); else ADD(Bf16, 64); }
+#undef ADD
+      HIP_CHECK_LAUNCH();
+    }
   }
 }

@@ -438,6 +438,7 @@ __device__ __forceinline__ void shared_keys(
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, n = lane & 31, rep = nh / ng;
+  const Places<D> at_lane(lane);
   const int hk = block % ng, piece = block / ng % gr.pieces;
   const int g = block / ng / gr.pieces % gr.groups;
   const int first_row = group_row(gr, g);
@@ -530,10 +531,10 @@ __device__ __forceinline__ void shared_keys(
       for (int u = 0; u < 2; ++u) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) st[u][r] = 0.f;
-        const int kr = 32 * u + tile_row(n);
 #pragma unroll
         for (int f = 0; f < NF; ++f)
-          st[u] = T::mfma32(read_rows<T, D>(img, kr, f, h), qf[f], st[u]);
+          st[u] = T::mfma32(read_rows<T, D>(img, 32 * u, f, at_lane), qf[f],
+                             st[u]);
       }
       reads_ahead<2 * NF, 1>();
       if (!all || at + BN > to || fine != 15) {
@@ -577,7 +578,7 @@ __device__ __forceinline__ void shared_keys(
 #pragma unroll
           for (int i = 0; i < ND; ++i)
             acc[i] = T::mfma32(
-                read_cols<T, D>(img + BN * D, 32 * u + 16 * y, i, lane), pf,
+                read_cols<T, D>(img + BN * D, 32 * u + 16 * y, i, at_lane), pf,
                 acc[i]);
         }
     };

@@ -225,6 +225,27 @@ def test_batch_and_scale():
 
 
 @gpu
+@pytest.mark.parametrize("lens,nh,ng,d,b", [
+    ([300], 8, 1, 64, 1),               # four shares of a tile's work
+    ([700, 20, 100], 16, 1, 128, 1),    # eight, some without any
+    ([600], 3, 1, 128, 2),
+    ([40] * 20, 32, 1, 128, 1),         # more tiles than the host expects
+    ([2100], 2, 2, 128, 1),             # of one head
+])
+def test_shares_of_the_keys_gradients(lens, nh, ng, d, b):
+    """Few tiles: several blocks share the queries of one."""
+    _check(lens, nh=nh, ng=ng, d=d, b=b, tail=5)
+    _check(lens, nh=nh, ng=ng, d=d, b=b, causal=False,
+           dtype=torch.float16)
+
+
+@gpu
+def test_shares_without_queries():
+    _check([0, 300], [50, 300], nh=8, ng=1, d=64)
+    _check([300, 7], [40, 0], nh=16, ng=1, d=128)
+
+
+@gpu
 def test_many_sequences():
     _check([(i * 7) % 13 for i in range(300)], nh=2, ng=1, d=64, tail=2)
 
