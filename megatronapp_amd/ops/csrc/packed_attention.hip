@@ -462,31 +462,34 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_bwd_dq_kernel(
 // whose sums are added at the end (one wave a SIMD: 228 us for 165 then, and
 // 546 for 361 at D = 64).
 //
-// The same documents as for dQ: 141 us, 740 TFLOP/s, and 268 us, 760.  Both
+// The same documents as for dQ: 141 us, 740 TFLOP/s, and 245 us, 830.  Both
 // units are busy a third of the time, four tenths of it pass in waits, most
-// for LDS, where each 32 x 32 tile reads Q and dO along both axes.  Four waves
-// a block at D = 64, two blocks a CU, are 5% faster on the fifteen documents
-// and 3% slower on 8192 tokens; three or four waves a SIMD spill.
-template <int D>
+// for LDS, where each 32 x 32 tile reads Q and dO along both axes.
+//
+// Eight waves keep in step, which costs time; at D = 64, where K and V are in
+// registers, two blocks of four waves fit a CU instead, and are taken (MANY)
+// where tiles are many.
+template <int D, bool MANY>
 struct Dkv {
-  static constexpr int HALVES = 2;
-  static constexpr int BQ = D == 128 ? 64 : 128;   // queries of a tile
+  static constexpr int HALVES = MANY ? 1 : 2;
+  static constexpr int BQ = D == 128 ? 64 : 64 * HALVES;   // queries of a tile
   static constexpr int WAVES = 4 * HALVES;
 };
 
 template <int D>
 constexpr long SHARE = BM * D / 4;    // of four numbers: one tile's dK (or dV)
 
-template <class T, int D, bool CAUSAL>
-__global__ __launch_bounds__(Dkv<D>::WAVES * 64, 2) void packed_bwd_dkv_kernel(
+template <class T, int D, bool CAUSAL, bool MANY>
+__global__ __launch_bounds__((Dkv<D, MANY>::WAVES * 64), 2)
+void packed_bwd_dkv_kernel(
     const unsigned short* __restrict__ q, const unsigned short* __restrict__ k,
     const unsigned short* __restrict__ v,
     const unsigned short* __restrict__ dout, const float* __restrict__ lse,
     const float* __restrict__ dot, unsigned short* __restrict__ dk,
     unsigned short* __restrict__ dv, float* __restrict__ sums, int shares,
     Packing pk, int b, int nh, int ng, float scale, Strides qs, Strides ks, Strides vs, Strides os) {
-  constexpr int HALVES = Dkv<D>::HALVES, WAVES = Dkv<D>::WAVES;
-  constexpr int BQ = Dkv<D>::BQ;
+  constexpr int HALVES = Dkv<D, MANY>::HALVES;
+  constexpr int WAVES = Dkv<D, MANY>::WAVES, BQ = Dkv<D, MANY>::BQ;
   constexpr bool KV_LDS = D == 128;
   // Q, dO, then the rows' lse and D
   constexpr int IMG = 2 * BQ * D + 4 * BQ;
@@ -759,6 +762,19 @@ void launch_packed_attn_fwd(const void* q, const void* k, const void* v,
   HIP_CHECK_LAUNCH();
 }
 
+// Tiles of keys, where every other sequence ends in a part of one.
+static long dkv_blocks(int n, int tk, int b, int ng) {
+  return (long)b * ng * (tk / BM + (n + 1) / 2);
+}
+
+// From so many blocks on, three for each of 256 CUs, four waves do at D = 64.
+// Backward with eight and four waves, us, 16 heads: 4096 tokens in two
+// sequences, 528 blocks, 99 and 108, 6144 in three, 800 blocks, 132 and 121;
+// 1024 in each of eight, 1088, 110 and 100; 32 heads, 300 in each of twelve,
+// 1088, 75 and 60; 32/8 heads, 8192 + 5003, 832, 1435 and 1508; the fifteen
+// documents, 1120, 467 and 444.
+static constexpr long FOUR_WAVES = 768;
+
 // Into how many shares a tile's work for dK and dV is cut, so that there are
 // two blocks for each of 256 CUs (of a causal mask's tiles the first has twice
 // the average to do), but none of fewer than two tiles of queries; where every
@@ -775,8 +791,8 @@ void launch_packed_attn_fwd(const void* q, const void* k, const void* v,
 int packed_attn_shares(int n, int tq, int tk, int b, int nh, int ng, int d,
                        long* floats) {
   constexpr long FILL = 512, LEAST = 2;
-  const long blocks = (long)b * ng * (tk / BM + (n + 1) / 2);
-  const int bq = d == 128 ? Dkv<128>::BQ : Dkv<64>::BQ;
+  const long blocks = dkv_blocks(n, tk, b, ng);
+  const int bq = d == 128 ? Dkv<128, false>::BQ : Dkv<64, false>::BQ;
   const long tiles = (long)(nh / ng) * (tq / std::max(n, 1)) / (2 * bq);
   long fill = (FILL + blocks / 2) / std::max(blocks, 1l);
   if (blocks >= FILL / 2 && tiles < d * 3 / 16) fill = 1;
@@ -814,15 +830,22 @@ void launch_packed_attn_bwd(const void* dout, const void* q, const void* k,
   }
   if (tk > 0) {
     const dim3 grid = grid_for((long)b * ng * shares, tk, n);
-#define RUN(T, DD, CC)                                                       \
-  hipLaunchKernelGGL((packed_bwd_dkv_kernel<T, DD, CC>),                     \
-                     grid, dim3(Dkv<DD>::WAVES * 64), 0, stream,             \
+#define LAUNCH(T, DD, CC, FOUR)                                              \
+  hipLaunchKernelGGL((packed_bwd_dkv_kernel<T, DD, CC, FOUR>),               \
+                     grid, dim3(Dkv<DD, FOUR>::WAVES * 64), 0, stream,       \
                      (const unsigned short*)q, (const unsigned short*)k,     \
                      (const unsigned short*)v, (const unsigned short*)dout,  \
                      lse, dot, (unsigned short*)dk, (unsigned short*)dv,     \
                      sums, shares, pk, b, nh, ng, scale, sq, sk, sv, so)
+#define RUN(T, DD, CC)                                                       \
+  do {                                                                       \
+    if (DD == 64 && many) LAUNCH(T, 64, CC, true);                           \
+    else LAUNCH(T, DD, CC, false);                                           \
+  } while (0)
+    const bool many = dkv_blocks(n, tk, b, ng) >= FOUR_WAVES;
     PACKED_DISPATCH(RUN);
 #undef RUN
+#undef LAUNCH
     HIP_CHECK_LAUNCH();
     if (shares > 1) {
       const dim3 tiles(grid_for((long)b * ng, tk, n).x, d / 16);

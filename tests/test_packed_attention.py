@@ -246,6 +246,17 @@ def test_shares_without_queries():
 
 
 @gpu
+@pytest.mark.parametrize("lens,heads", [
+    ([7 * i % 23 for i in range(60)], 32),
+    ([300, 513, 1, 129] + [40] * 50, 16),
+])
+def test_many_tiles(lens, heads):
+    """Blocks of four waves for the gradients of the keys."""
+    _check(lens, nh=heads, ng=heads, d=64, tail=9)
+    _check(lens, nh=heads, ng=heads, d=64, causal=False)
+
+
+@gpu
 def test_many_sequences():
     _check([(i * 7) % 13 for i in range(300)], nh=2, ng=1, d=64, tail=2)
 
