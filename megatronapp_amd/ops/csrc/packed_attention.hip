@@ -161,8 +161,8 @@ __device__ __forceinline__ int head_of(int x, int ng, int rep) {
 // A wave holds 32 rows of Q as the right operand of S^T = K Q^T, and P^T, which
 // that leaves in its registers, is the right operand of O^T = V^T P^T; the four
 // waves share the tiles of K and V, of which the next one comes into the other
-// of two images while one is used.  Two blocks of 227 registers at D = 128 and
-// four of 120 at 64 run on a CU, each at another place of its loop, so that one
+// of two images while one is used.  Two blocks of 188 registers at D = 128 and
+// four of 123 at 64 run on a CU, each at another place of its loop, so that one
 // does its exponentials beside the other's products.
 //
 // At D = 64 the vector unit bounds it (busy 64% of the time, the matrix unit
@@ -175,9 +175,9 @@ __device__ __forceinline__ int head_of(int x, int ng, int rep) {
 // documents of 45 to 2048, 16 heads, in training 74 us (710).
 //
 // Taken back: 64 rows a wave at D = 64 (half the reads of K and V: equal, for
-// short prompts 9.0 us against 7.5), the next tile's scores before this one's
-// sums (spills), a higher priority for the products (equal), images of K and V
-// apart (equal).
+// short prompts 9.0 us against 7.5), the next tile's scores beside this one's
+// exponentials (equal at 128, where nothing spills, and 155 us -> 165 at 64), a
+// higher priority for the products (equal), images of K and V apart (equal).
 template <class T, int D, bool CAUSAL>
 __global__ __launch_bounds__(BLOCK, 2) void packed_fwd_kernel(
     const unsigned short* __restrict__ q, const unsigned short* __restrict__ k,
@@ -289,6 +289,7 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_fwd_kernel(
           acc[i] = T::mfma32(read_cols<T, D>(vi, 32 * u + 16 * x, i, at_lane),
                              pf, acc[i]);
       }
+    reads_ahead<4 * ND, 2>();
   };
   // one tile is used while the next one comes in
   auto turn = [&](int t, unsigned short* img, unsigned short* next) {
@@ -434,6 +435,7 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_bwd_dq_kernel(
           acc[i] = T::mfma32(
               read_cols<T, D>(img, 32 * u + 16 * x, i, at_lane), sf, acc[i]);
       }
+      reads_ahead<2 * ND, 2>();
     }
   };
   auto turn = [&](int t, unsigned short* img, unsigned short* next) {
@@ -586,6 +588,7 @@ void packed_bwd_dkv_kernel(
       st = T::mfma32(read_rows<T, D>(img, 32 * u, f, at_lane), k_frag(f), st);
       dp = T::mfma32(read_rows<T, D>(di, 32 * u, f, at_lane), v_frag(f), dp);
     }
+    reads_ahead<2 * NF, KV_LDS ? 2 : 1>();
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int y = 16 * (r >> 3) + (r & 7);
@@ -611,6 +614,7 @@ void packed_bwd_dkv_kernel(
                           sf, ak[i]);
       }
     }
+    reads_ahead<4 * ND, 2>();
   };
   // one tile is used while the next one comes in
   int r1 = left ? begin / per : 0;    // the next tile's head and number
