@@ -7,7 +7,8 @@ before the first or behind the last sequence, give zeros, and get and give no
 gradient.
 
 On the GPU this is ``ops/csrc/packed_attention.hip`` (bf16 and fp16, head
-sizes 64 and 128); on the CPU a plain computation in 32 bits or more.  A
+sizes 64 and 128), whose gradient cannot be differentiated again; on the CPU a
+plain computation in 32 bits or more.  A
 sequence's values reach no other sequence, whatever they are.  Within one, a
 value of v that is not finite may reach earlier rows of the same 64-key tile
 (nothing times NaN is NaN).
@@ -31,25 +32,6 @@ def packed_attention_supported(query: torch.Tensor) -> bool:
     return (query.is_cuda and _ops.have_ops()
             and query.dtype in (torch.bfloat16, torch.float16)
             and query.shape[-1] in HEAD_SIZES)
-
-
-class _PackedAttnFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, cu_q, cu_k, scale, causal):
-        o, lse, low = _ops.get_ops().packed_attn_fwd(q, k, v, cu_q, cu_k,
-                                                     scale, causal, True)
-        ctx.save_for_backward(q, k, v, o, low, lse, cu_q, cu_k)
-        ctx.scale = scale
-        ctx.causal = causal
-        return o
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, do):
-        q, k, v, o, low, lse, cu_q, cu_k = ctx.saved_tensors
-        dq, dk, dv = _ops.get_ops().packed_attn_bwd(
-            do, q, k, v, o, low, lse, cu_q, cu_k, ctx.scale, ctx.causal)
-        return dq, dk, dv, None, None, None, None
 
 
 def _check(query, key, value, cu_q, cu_k, scale):
@@ -138,13 +120,8 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor,
     if cu_q is None:
         raise ValueError("packed_attention: cu_seqlens_q is missing")
     if query.is_cuda:
-        if torch.is_grad_enabled() and (query.requires_grad
-                                        or key.requires_grad
-                                        or value.requires_grad):
-            return _PackedAttnFn.apply(query, key, value, cu_q, cu_k,
-                                       softmax_scale, causal)
-        return _ops.get_ops().packed_attn_fwd(query, key, value, cu_q, cu_k,
-                                              softmax_scale, causal, False)[0]
+        return _ops.get_ops().packed_attention(query, key, value, cu_q, cu_k,
+                                               softmax_scale, causal)
     cu_k = cu_q if cu_k is None else cu_k
     scale = (1.0 / math.sqrt(query.shape[-1]) if softmax_scale is None
              else float(softmax_scale))

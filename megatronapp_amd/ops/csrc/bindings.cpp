@@ -915,6 +915,51 @@ std::vector<torch::Tensor> packed_attn_bwd(
   return {dq, dk, dv};
 }
 
+// A node of its own kind rather than Python's: a backward of small sequences
+// takes the host 90 us there.
+struct PackedAttn : public torch::autograd::Function<PackedAttn> {
+  static torch::Tensor forward(torch::autograd::AutogradContext* ctx,
+                               torch::Tensor q, torch::Tensor k,
+                               torch::Tensor v, torch::Tensor cu_q,
+                               c10::optional<torch::Tensor> cu_kv,
+                               c10::optional<double> scale, bool causal) {
+    const auto r = packed_attn_fwd(q, k, v, cu_q, cu_kv, scale, causal, true);
+    ctx->save_for_backward({q, k, v, r[0], r[2], r[1], cu_q,
+                            cu_kv.has_value() ? *cu_kv : torch::Tensor()});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["causal"] = causal;
+    return r[0];
+  }
+
+  static torch::autograd::variable_list backward(
+      torch::autograd::AutogradContext* ctx,
+      torch::autograd::variable_list grads) {
+    TORCH_CHECK(!torch::GradMode::is_enabled(),
+                "packed_attention: its gradient has none of its own");
+    const auto s = ctx->get_saved_variables();
+    torch::autograd::variable_list out(7);
+    if (!grads[0].defined()) return out;
+    c10::optional<torch::Tensor> cu_kv;
+    if (s[7].defined()) cu_kv = s[7];
+    auto g = packed_attn_bwd(grads[0], s[0], s[1], s[2], s[3], s[4], s[5],
+                             s[6], cu_kv,
+                             ctx->saved_data["scale"].toOptional<double>(),
+                             ctx->saved_data["causal"].toBool());
+    for (int i = 0; i < 3; ++i) out[i] = g[i];
+    return out;
+  }
+};
+
+torch::Tensor packed_attention(torch::Tensor q, torch::Tensor k,
+                               torch::Tensor v, torch::Tensor cu_q,
+                               c10::optional<torch::Tensor> cu_kv,
+                               c10::optional<double> scale, bool causal) {
+  if (torch::GradMode::is_enabled() &&
+      (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+    return PackedAttn::apply(q, k, v, cu_q, cu_kv, scale, causal);
+  return packed_attn_fwd(q, k, v, cu_q, cu_kv, scale, causal, false)[0];
+}
+
 // ------------------------------------------------------------- paged cache
 // pages [layers, 2, P, groups, page, d]; refs [P], tables [slots, W], lengths
 // [slots] and status [1] int32, all on one GPU and contiguous
@@ -1365,7 +1410,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   mod.def("wgrad_accum_bgrad", &wgrad_accum_bgrad);
   mod.def("attn_fwd", &attn_fwd);
   mod.def("attn_fwd_ablate", &attn_fwd_ablate);
-  mod.def("packed_attn_fwd", &packed_attn_fwd);
+  mod.def("packed_attention", &packed_attention);
   mod.def("cache_fork", &cache_fork);
   mod.def("cache_free", &cache_free);
   mod.def("cache_compact", &cache_compact);
@@ -1373,7 +1418,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   mod.def("cache_extend", &cache_extend);
   mod.def("cache_write", &cache_write);
   mod.def("paged_attn", &paged_attn);
-  mod.def("packed_attn_bwd", &packed_attn_bwd);
   mod.def("attn_bwd", &attn_bwd);
   mod.def("colsum_accum", &colsum_accum);
   mod.def("embedding_bwd_accum", &embedding_bwd_accum);

@@ -460,6 +460,21 @@ def test_refusals_on_the_gpu():
 
 
 @gpu
+def test_no_second_gradient():
+    q, k, v, dout = _inputs([5], [5])
+    params = PackedSeqParams(cu_seqlens_q=_cu([5], q.device))
+    q.requires_grad_()
+    o = packed_attention(q, k, v, params)
+    with pytest.raises(RuntimeError, match="gradient"):
+        torch.autograd.grad(o, q, dout, create_graph=True)
+    o = packed_attention(q, k, v, params)
+    with torch.no_grad():
+        q.add_(1)                       # the backward needs it as it was
+    with pytest.raises(RuntimeError, match="modified"):
+        o.backward(dout)
+
+
+@gpu
 def test_flash_attention_keeps_sequences_apart():
     """The layers' attention hands a packed stream to the kernel, and gives
     what the eager path gives."""
