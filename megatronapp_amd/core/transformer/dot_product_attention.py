@@ -30,6 +30,10 @@ def attention_mask_func(attention_scores, attention_mask):
     return attention_scores.masked_fill(attention_mask, -10000.0)
 
 
+# A packed stream has its sequences' ends where others have padding.
+_CAUSAL = (AttnMaskType.causal, AttnMaskType.padding_causal)
+
+
 class DotProductAttention(nn.Module):
     def __init__(self, config: TransformerConfig, layer_number: int,
                  attn_mask_type: AttnMaskType, attention_type: str = "self",
@@ -98,7 +102,7 @@ class DotProductAttention(nn.Module):
             from ..enums import AttnMaskType as _AMT
             attention_mask = packed_attention_mask(
                 packed_seq_params.cu_seqlens_q, sk,
-                causal=(mask_type == _AMT.causal))
+                causal=mask_type in _CAUSAL)
             mask_type = _AMT.padding
         probs = self.scale_mask_softmax(scores, attention_mask, mask_type)
 
@@ -215,7 +219,7 @@ class FlashAttention(nn.Module):
                      else self.attn_mask_type)
         o = packed_attention(query, key, value, packed_seq_params,
                              softmax_scale=self.softmax_scale,
-                             causal=mask_type == AttnMaskType.causal)
+                             causal=mask_type in _CAUSAL)
         return o.reshape(o.shape[0], o.shape[1], -1)
 
     def forward(self, query, key, value, attention_mask=None,

@@ -406,6 +406,42 @@ def test_captured_and_replayed():
 
 
 @gpu
+def test_shares_captured_and_replayed():
+    """The shares are chosen when the graph is made; later lengths are cut as
+    these were, and two graphs keep their sums apart."""
+    lens = [700, 20, 100]
+    q, k, v, dout = _inputs(lens, lens, nh=16, ng=1, d=128)
+    cu = _cu(lens, "cuda")
+    params = PackedSeqParams(cu_seqlens_q=cu)
+    x = [t.clone().requires_grad_(True) for t in (q, k, v)]
+
+    def run():
+        o = packed_attention(*x, params)
+        return (o.detach(),) + torch.autograd.grad(o, x, dout)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    outs = []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            outs.append(run())
+    for new in (lens, [1, 818, 1], [0, 0, 820], [300, 300, 220]):
+        cu.copy_(_cu(new))
+        graphs[0].replay()
+        graphs[1].replay()
+        want = run()
+        graphs[0].replay()
+        torch.cuda.synchronize()
+        for out in outs:
+            for a, b in zip(out, want):
+                assert torch.equal(a, b), new
+
+
+@gpu
 def test_gradient_matches_differences():
     """The kernel's gradient against central differences of the formula in
     64 bits, along one direction for each input.  The differences' own error
@@ -503,4 +539,28 @@ def test_flash_attention_keeps_sequences_apart():
     eager = DotProductAttention(cfg, 1, AttnMaskType.causal)(
         q.float(), k.float(), v.float(), packed_seq_params=params)
     _near("eager", eager.view(q.shape), want)
+    destroy()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_padding_causal_is_causal_in_a_packed_stream(device):
+    from tests.utils import destroy, initialize_model_parallel
+    from megatronapp_amd.core.enums import AttnMaskType
+    from megatronapp_amd.core.transformer.dot_product_attention import (
+        FlashAttention)
+    from megatronapp_amd.core.transformer_config import TransformerConfig
+    initialize_model_parallel()
+    cfg = TransformerConfig(num_layers=1, hidden_size=256,
+                            num_attention_heads=4, num_query_groups=2,
+                            bf16=device == "cuda", hidden_dropout=0.0,
+                            attention_dropout=0.0)
+    dtype = torch.bfloat16 if device == "cuda" else torch.float32
+    q, k, v, _ = _inputs([10, 6], [10, 6], dtype=dtype, device=device)
+    params = PackedSeqParams(cu_seqlens_q=_cu([10, 6], device),
+                             cu_seqlens_kv=_cu([10, 6], device))
+    got = [FlashAttention(cfg, 1, t)(q, k, v, packed_seq_params=params)
+           for t in (AttnMaskType.causal, AttnMaskType.padding_causal,
+                     AttnMaskType.padding)]
+    assert torch.equal(got[0], got[1])
+    assert not torch.equal(got[0], got[2])
     destroy()
