@@ -89,6 +89,9 @@ class PagedKVCache:
                 lengths.shape[0] != page_tables.shape[0]:
             raise ValueError("PagedKVCache: the tensors' sizes do not fit "
                              "each other")
+        if page_tables.shape[1] * pages.shape[4] >= 1 << 31:
+            raise ValueError("PagedKVCache: a sequence of 2^31 tokens and "
+                             "more does not fit its length")
         self.pages = pages
         self.ref_counts = ref_counts
         self.page_tables = page_tables
@@ -259,7 +262,7 @@ class PagedKVCache:
               slots: Slots, cu_seqlens: Optional[torch.Tensor] = None):
         """Puts key and value [tokens, groups, d] in the last places of the
         slots' sequences: one token each, or tokens cu_seqlens[i] to
-        cu_seqlens[i + 1] as the last of slots[i]."""
+        cu_seqlens[i + 1] as the last of slots[i].  No slot is named twice."""
         slots = self._list("slots", slots, self.max_slots, True)
         if not 0 <= layer < self.pages.shape[0]:
             raise ValueError(f"PagedKVCache: no layer {layer}")

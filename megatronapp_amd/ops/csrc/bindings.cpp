@@ -907,11 +907,11 @@ std::vector<torch::Tensor> packed_attn_bwd(
   if (floats) sums = torch::empty({floats}, q.options().dtype(torch::kFloat32));
   launch_packed_attn_bwd(
       dr.data_ptr(), qr.data_ptr(), kr.data_ptr(), vr.data_ptr(), o.data_ptr(),
-      low.data_ptr(), lse.data_ptr<float>(), dot.data_ptr<float>(), dq.data_ptr(),
-      dk.data_ptr(), dv.data_ptr(),
-      floats ? sums.data_ptr<float>() : nullptr, shares,
-      iq.data_ptr<int>(), ik.data_ptr<int>(), s.n, s.tq, s.tk, s.b, s.nh, s.ng, s.d, (float)scale, causal, s.fp16, os,
-      qs, ks, vs, cur_stream());
+      low.data_ptr(), lse.data_ptr<float>(), dot.data_ptr<float>(),
+      dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+      floats ? sums.data_ptr<float>() : nullptr, shares, iq.data_ptr<int>(),
+      ik.data_ptr<int>(), s.n, s.tq, s.tk, s.b, s.nh, s.ng, s.d, (float)scale,
+      causal, s.fp16, os, qs, ks, vs, cur_stream());
   return {dq, dk, dv};
 }
 
@@ -992,7 +992,8 @@ CacheRefs cache_refs(const torch::Tensor& pages, const torch::Tensor& refs,
   TORCH_CHECK(refs.numel() == pages.size(2) &&
                   lengths.numel() == tables.size(0) && status.numel() > 0 &&
                   token % 16 == 0 && pages.size(2) < (1l << 30) &&
-                  tables.size(0) <= (1l << 18) && tables.size(1) < (1l << 30),
+                  tables.size(0) <= (1l << 18) &&
+                  tables.size(1) * (long)pages.size(4) < (1l << 31),
               "the cache's tensors do not fit each other");
   return {refs.data_ptr<int>(),    tables.data_ptr<int>(),
           lengths.data_ptr<int>(), status.data_ptr<int>(),

@@ -366,3 +366,14 @@ def test_captured_and_replayed_with_forks():
     a, b = walk(False), walk(True)
     for x, y in zip(a.state, b.state):
         assert torch.equal(x, y)
+
+
+def test_lengths_that_pass_32_bits_are_refused():
+    ints = dict(dtype=torch.int32)
+    with pytest.raises(ValueError, match="2.31"):
+        PagedKVCache.from_state(torch.zeros(1, 2, 1, 1, 512, 8),
+                                torch.zeros(1, **ints),
+                                torch.zeros(1, 1 << 22, **ints),
+                                torch.zeros(1, **ints))
+    with pytest.raises(ValueError, match="2.31"):
+        PagedKVCache(1, 1, 1 << 20, 1, 8, 1, 1 << 31, device="cpu")
