@@ -61,7 +61,8 @@ struct Fp16 {
 template <class T>
 __device__ __forceinline__ unsigned pack2(float a, float b) {
   f32x2 f = {a, b};
-  return __builtin_bit_cast(unsigned, __builtin_convertvector(f, typename T::x2));
+  return __builtin_bit_cast(unsigned,
+                            __builtin_convertvector(f, typename T::x2));
 }
 
 // eight floats of a C tile as half of a product's operand

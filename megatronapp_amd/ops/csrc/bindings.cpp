@@ -114,9 +114,10 @@ void launch_attn_bwd(const void*, const void*, const void*, const void*,
                      int, int, int, int, int, int, float, bool, hipStream_t);
 
 void launch_packed_attn_fwd(const void*, const void*, const void*, void*,
-                            void*, float*, const int*, const int*, int, int, int, int,
-                            int, int, int, float, bool, bool, const long*,
-                            const long*, const long*, hipStream_t);
+                            void*, float*, const int*, const int*, int, int,
+                            int, int, int, int, int, float, bool, bool,
+                            const long*, const long*, const long*,
+                            hipStream_t);
 int packed_attn_shares(int, int, int, int, int, int, int, long*);
 void launch_packed_attn_bwd(const void*, const void*, const void*,
                             const void*, const void*, const void*,
@@ -146,7 +147,8 @@ void paged_attn_pieces(int, int, int, int, int, int, int, long, int*, int*,
 void launch_paged_attn(const void*, long, long, const void*, const void*,
                        const long*, const long*, const int*, const int*,
                        const int*, const int*, const int*, int, int, int, int,
-                       int, int, int, int, int, int, int, int, int, void*, float*,
+                       int, int, int, int, int, int, int, int, int, void*,
+                       float*,
                        float*, float, bool, hipStream_t);
 
 namespace {
@@ -1095,7 +1097,8 @@ void cache_write(CACHE_ARGS, long layer, torch::Tensor k, torch::Tensor v,
   } else {
     TORCH_CHECK(k.size(0) == n, "write: one token for each slot");
   }
-  TORCH_CHECK(k.size(0) * (long)c.groups < (1l << 31), "write: too many tokens");
+  TORCH_CHECK(k.size(0) * (long)c.groups < (1l << 31),
+              "write: too many tokens");
   if (k.size(0) == 0 || c.groups == 0) return;
   const long es = pages.element_size();
   auto rows = [&](const torch::Tensor& t) {

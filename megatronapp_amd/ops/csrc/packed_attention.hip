@@ -492,7 +492,8 @@ void packed_bwd_dkv_kernel(
     const unsigned short* __restrict__ dout, const float* __restrict__ lse,
     const float* __restrict__ dot, unsigned short* __restrict__ dk,
     unsigned short* __restrict__ dv, float* __restrict__ sums, int shares,
-    Packing pk, int b, int nh, int ng, float scale, Strides qs, Strides ks, Strides vs, Strides os) {
+    Packing pk, int b, int nh, int ng, float scale, Strides qs, Strides ks,
+    Strides vs, Strides os) {
   constexpr int HALVES = Dkv<D, MANY>::HALVES;
   constexpr int WAVES = Dkv<D, MANY>::WAVES, BQ = Dkv<D, MANY>::BQ;
   constexpr bool KV_LDS = D == 128;
@@ -736,15 +737,19 @@ dim3 grid_for(long heads, int total, int n) {
 
 }  // namespace
 
-#define PACKED_DISPATCH(RUN)                                              \
-  do {                                                                    \
-    if (fp16) {                                                           \
-      if (d == 128) { if (causal) RUN(Fp16, 128, true); else RUN(Fp16, 128, false); } \
-      else { if (causal) RUN(Fp16, 64, true); else RUN(Fp16, 64, false); }  \
-    } else {                                                              \
-      if (d == 128) { if (causal) RUN(Bf16, 128, true); else RUN(Bf16, 128, false); } \
-      else { if (causal) RUN(Bf16, 64, true); else RUN(Bf16, 64, false); }  \
-    }                                                                     \
+#define PACKED_MASK(RUN, T, D)                       \
+  do {                                               \
+    if (causal) RUN(T, D, true); else RUN(T, D, false); \
+  } while (0)
+#define PACKED_DISPATCH(RUN)                         \
+  do {                                               \
+    if (fp16) {                                      \
+      if (d == 128) PACKED_MASK(RUN, Fp16, 128);     \
+      else PACKED_MASK(RUN, Fp16, 64);               \
+    } else {                                         \
+      if (d == 128) PACKED_MASK(RUN, Bf16, 128);     \
+      else PACKED_MASK(RUN, Bf16, 64);               \
+    }                                                \
   } while (0)
 
 void launch_packed_attn_fwd(const void* q, const void* k, const void* v,
@@ -812,8 +817,8 @@ int packed_attn_shares(int n, int tq, int tk, int b, int nh, int ng, int d,
 void launch_packed_attn_bwd(const void* dout, const void* q, const void* k,
                             const void* v, const void* o, const void* low,
                             const float* lse, float* dot, void* dq, void* dk,
-                            void* dv, float* sums, int shares, const int* cu_q, const int* cu_k, int n, int tq,
-                            int tk, int b, int nh, int ng, int d, float scale,
+                            void* dv, float* sums, int shares, const int* cu_q,
+                            const int* cu_k, int n, int tq, int tk, int b, int nh, int ng, int d, float scale,
                             bool causal, bool fp16, const long* os,
                             const long* qs, const long* ks, const long* vs,
                             hipStream_t stream) {

@@ -348,7 +348,8 @@ __device__ __forceinline__ void own_keys(const unsigned short* q, long qb,
     if (wave == turn) {
 #pragma unroll
       for (int i = 0; i < ND; ++i) {
-        f32x4* p = (f32x4*)(sums + n * ROW + ((i * 16 + 4 * g) ^ ((n & 7) << 2)));
+        f32x4* p =
+            (f32x4*)(sums + n * ROW + ((i * 16 + 4 * g) ^ ((n & 7) << 2)));
         f32x4 x = acc[i];
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[r] *= a;
@@ -383,7 +384,8 @@ __device__ __forceinline__ void own_keys(const unsigned short* q, long qb,
         out.lse[at] =
             ll == 0.f ? -INFINITY : mm + __builtin_amdgcn_logf(ll);
     } else {
-      u32x2 z = {pack2<T>(y[0] * by, y[1] * by), pack2<T>(y[2] * by, y[3] * by)};
+      u32x2 z = {pack2<T>(y[0] * by, y[1] * by),
+                 pack2<T>(y[2] * by, y[3] * by)};
       *(u32x2*)(out.o + r * D + d) = z;
     }
   }

@@ -456,7 +456,8 @@ void launch_cache_fork(int* refs, int* tables, int* lengths, int* status,
                        int planes, int groups, int token, const int* src,
                        const int* dst, int n, int* scratch,
                        hipStream_t stream) {
-  const Pool p = pool_of(refs, tables, lengths, status, pages, slots, width, page);
+  const Pool p =
+      pool_of(refs, tables, lengths, status, pages, slots, width, page);
   int* go = scratch;                        // [4]
   Pair* plan = (Pair*)(scratch + 4);        // [n] of 4
   int* fresh = scratch + 4 + 4l * n;        // [n]
@@ -474,7 +475,8 @@ void launch_cache_fork(int* refs, int* tables, int* lengths, int* status,
 void launch_cache_free(int* refs, int* tables, int* lengths, int* status,
                        int pages, int slots, int width, int page,
                        const int* list, int n, hipStream_t stream) {
-  const Pool p = pool_of(refs, tables, lengths, status, pages, slots, width, page);
+  const Pool p =
+      pool_of(refs, tables, lengths, status, pages, slots, width, page);
   hipLaunchKernelGGL(free_kernel, dim3(n), dim3(BLOCK), 0, stream, p, list);
   HIP_CHECK_LAUNCH();
 }
@@ -483,7 +485,8 @@ void launch_cache_compact(int* refs, int* tables, int* lengths, int* status,
                           int pages, int slots, int width, int page,
                           void* data, int planes, long bytes, int* scratch,
                           hipStream_t stream) {
-  const Pool p = pool_of(refs, tables, lengths, status, pages, slots, width, page);
+  const Pool p =
+      pool_of(refs, tables, lengths, status, pages, slots, width, page);
   int* moves = scratch;                     // [2 + 2 P]
   int* map = scratch + 2 + 2l * pages;      // [P]
   int* movers = map + pages;                // [P]
@@ -515,7 +518,8 @@ void launch_cache_extend(int* refs, int* tables, int* lengths, int* status,
                          int pages, int slots, int width, int page,
                          const int* list, const int* counts, int each, int n,
                          int* scratch, hipStream_t stream) {
-  const Pool p = pool_of(refs, tables, lengths, status, pages, slots, width, page);
+  const Pool p =
+      pool_of(refs, tables, lengths, status, pages, slots, width, page);
   hipLaunchKernelGGL(extend_kernel, dim3(1), dim3(PLAN), (slots + 31) / 32 * 4,
                      stream, p, list, counts, each, n, scratch, scratch + n);
   HIP_CHECK_LAUNCH();
@@ -527,7 +531,8 @@ void launch_cache_write(int* refs, int* tables, int* lengths, int* status,
                         void* keys, void* values, const void* k, const void* v,
                         int groups, int token, long kt, long kh, long vt,
                         long vh, hipStream_t stream) {
-  const Pool p = pool_of(refs, tables, lengths, status, pages, slots, width, page);
+  const Pool p =
+      pool_of(refs, tables, lengths, status, pages, slots, width, page);
   const long items = (long)tokens * groups;
   hipLaunchKernelGGL(write_kernel,
                      dim3((unsigned)((items + BLOCK / 16 - 1) / (BLOCK / 16))),
