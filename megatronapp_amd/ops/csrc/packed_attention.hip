@@ -178,16 +178,19 @@ __device__ __forceinline__ int head_of(int x, int ng, int rep) {
 // short prompts 9.0 us against 7.5), the next tile's scores beside this one's
 // exponentials (equal at 128, where nothing spills, and 155 us -> 165 at 64), a
 // higher priority for the products (equal), images of K and V apart (equal).
-template <class T, int D, bool CAUSAL>
-__global__ __launch_bounds__(BLOCK, 2) void packed_fwd_kernel(
+template <class T, int D, bool CAUSAL, int HALVES>
+__global__ __launch_bounds__(BLOCK * HALVES, 2) void packed_fwd_kernel(
     const unsigned short* __restrict__ q, const unsigned short* __restrict__ k,
     const unsigned short* __restrict__ v, unsigned short* __restrict__ o,
     unsigned short* __restrict__ low, float* __restrict__ lse, Packing pk,
     int b, int nh, int ng, float c, Strides qs, Strides ks, Strides vs) {
-  __shared__ __attribute__((aligned(16))) unsigned short kv0_lds[2 * BN * D];
-  __shared__ __attribute__((aligned(16))) unsigned short kv1_lds[2 * BN * D];
+  constexpr int IMG = 2 * BN * D;
+  __shared__ __attribute__((aligned(16))) unsigned short kv0_lds[HALVES * IMG];
+  __shared__ __attribute__((aligned(16))) unsigned short kv1_lds[HALVES * IMG];
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
+  const int half = HALVES == 1 ? 0
+                               : __builtin_amdgcn_readfirstlane(tid >> 8);
   const int h = lane >> 5, n = lane & 31;
   const Places<D> at_lane(lane);
   Span s;
@@ -228,6 +231,7 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_fwd_kernel(
   const float lag = low ? 0.f : 8.f;
 
   auto fetch = [&](int t, unsigned short* img) {
+    if (HALVES > 1 && t >= tiles) return;
     const int last = s.sk - 1 - t * BN;
     load_tile<D, BN, 4>(img, kp + (long)t * BN * ks.t, ks.t, last, wave, lane);
     load_tile<D, BN, 4>(img + BN * D, vp + (long)t * BN * vs.t, vs.t, last,
@@ -291,17 +295,50 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_fwd_kernel(
       }
     reads_ahead<4 * ND, 2>();
   };
-  // one tile is used while the next one comes in
+  // one tile is used while the next one comes in; each half of the waves has
+  // every other tile
+  unsigned short* const img0 = kv0_lds + half * IMG;
+  unsigned short* const img1 = kv1_lds + half * IMG;
   auto turn = [&](int t, unsigned short* img, unsigned short* next) {
     __builtin_amdgcn_s_waitcnt(0x0f70);         // vmcnt(0)
     __syncthreads();
-    if (t + 1 < tiles) fetch(t + 1, next);
-    step(t, img);
+    if (t + HALVES < tiles) fetch(t + HALVES + half, next);
+    step(t + half, img);
   };
-  if (tiles > 0) fetch(0, kv0_lds);
-  for (int t = 0; t < tiles; t += 2) {
-    turn(t, kv0_lds, kv1_lds);
-    if (t + 1 < tiles) turn(t + 1, kv1_lds, kv0_lds);
+  if (tiles > 0) fetch(half, img0);
+  for (int t = 0; t < tiles; t += 2 * HALVES) {
+    turn(t, img0, img1);
+    if (t + HALVES < tiles) turn(t + HALVES, img1, img0);
+  }
+  if constexpr (HALVES == 2) {
+    // the second half's sums, handed over through the images
+    static_assert(sizeof(kv0_lds) >= 2 * (16 * ND + 2) * WAVE * 4,
+                  "room for them");
+    constexpr int EACH = (16 * ND + 2) * WAVE;
+    float* to = (float*)(wave < 2 ? kv0_lds : kv1_lds) + (wave & 1) * EACH +
+                lane;
+    __syncthreads();
+    if (half) {
+      to[0] = m;
+      to[WAVE] = l;
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) to[(2 + i * 16 + r) * WAVE] = acc[i][r];
+    }
+    __syncthreads();
+    if (half) return;
+    const float other = to[0], top = fmaxf(m, other);
+    const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    const float e = other == -INFINITY ? 0.f
+                                       : __builtin_amdgcn_exp2f(other - top);
+    m = top;
+    l = l * a + to[WAVE] * e;
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        acc[i][r] = acc[i][r] * a + to[(2 + i * 16 + r) * WAVE] * e;
   }
   if (!mine) return;
   l = half_sum(l);
@@ -330,11 +367,11 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_fwd_kernel(
 // Eight documents of 45 to 2048 tokens, 16 heads of 128: 103 us, 760 TFLOP/s;
 // fifteen of 1 to 2048, 32 heads of 64: 198 us, 770.  The matrix unit is busy
 // a third of the time, the vector unit 27% at 128 and 47% at 64; two waves on
-// a SIMD do not cover more of each other's waits.  Eight waves on a tile, four
-// on every other 32 keys, keep all of a CU's waves in step: the backward takes
-// 280 us for 244, and 587 for 466.
-template <class T, int D, bool CAUSAL>
-__global__ __launch_bounds__(BLOCK, 2) void packed_bwd_dq_kernel(
+// a SIMD do not cover more of each other's waits.  Eight waves on a tile there
+// keep all of a CU's waves in step: the backward takes 280 us for 244, and 587
+// for 466.
+template <class T, int D, bool CAUSAL, int HALVES>
+__global__ __launch_bounds__(BLOCK * HALVES, 2) void packed_bwd_dq_kernel(
     const unsigned short* __restrict__ q, const unsigned short* __restrict__ k,
     const unsigned short* __restrict__ v,
     const unsigned short* __restrict__ dout,
@@ -343,10 +380,13 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_bwd_dq_kernel(
     float* __restrict__ dot, unsigned short* __restrict__ dq, Packing pk,
     int b, int nh, int ng, float scale, Strides qs, Strides ks, Strides vs,
     Strides os) {
-  __shared__ __attribute__((aligned(16))) unsigned short kv0_lds[2 * BN * D];
-  __shared__ __attribute__((aligned(16))) unsigned short kv1_lds[2 * BN * D];
+  constexpr int IMG = 2 * BN * D;
+  __shared__ __attribute__((aligned(16))) unsigned short kv0_lds[HALVES * IMG];
+  __shared__ __attribute__((aligned(16))) unsigned short kv1_lds[HALVES * IMG];
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
+  const int half = HALVES == 1 ? 0
+                               : __builtin_amdgcn_readfirstlane(tid >> 8);
   const int h = lane >> 5, n = lane & 31;
   const Places<D> at_lane(lane);
   Span s;
@@ -384,7 +424,7 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_bwd_dq_kernel(
         rd += ((float)e[i] + (float)r[i]) * (float)df[f][i];
     }
     rd = half_sum(rd);
-    if (h == 0 && p < s.sq) dot[stat] = rd;
+    if (h == 0 && half == 0 && p < s.sq) dot[stat] = rd;
   }
   const int most = keys_of<CAUSAL>(s, min(s.tile * BM + BM, s.sq) - 1);
   const int wave_most = keys_of<CAUSAL>(s, min(p0 + 31, s.sq - 1));
@@ -399,6 +439,7 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_bwd_dq_kernel(
   for (int i = 0; i < ND; ++i) acc[i] = zeros16();
 
   auto fetch = [&](int t, unsigned short* img) {
+    if (HALVES > 1 && t >= tiles) return;
     const int last = s.sk - 1 - t * BN;
     load_tile<D, BN, 4>(img, kp + (long)t * BN * ks.t, ks.t, last, wave, lane);
     load_tile<D, BN, 4>(img + BN * D, vp + (long)t * BN * vs.t, vs.t, last,
@@ -438,16 +479,38 @@ __global__ __launch_bounds__(BLOCK, 2) void packed_bwd_dq_kernel(
       reads_ahead<2 * ND, 2>();
     }
   };
+  // one tile is used while the next one comes in; each half of the waves has
+  // every other tile
+  unsigned short* const img0 = kv0_lds + half * IMG;
+  unsigned short* const img1 = kv1_lds + half * IMG;
   auto turn = [&](int t, unsigned short* img, unsigned short* next) {
     __builtin_amdgcn_s_waitcnt(0x0f70);         // vmcnt(0)
     __syncthreads();
-    if (t + 1 < tiles) fetch(t + 1, next);
-    step(t, img);
+    if (t + HALVES < tiles) fetch(t + HALVES + half, next);
+    step(t + half, img);
   };
-  if (tiles > 0) fetch(0, kv0_lds);
-  for (int t = 0; t < tiles; t += 2) {
-    turn(t, kv0_lds, kv1_lds);
-    if (t + 1 < tiles) turn(t + 1, kv1_lds, kv0_lds);
+  if (tiles > 0) fetch(half, img0);
+  for (int t = 0; t < tiles; t += 2 * HALVES) {
+    turn(t, img0, img1);
+    if (t + HALVES < tiles) turn(t + HALVES, img1, img0);
+  }
+  if constexpr (HALVES == 2) {
+    static_assert(sizeof(kv0_lds) >= 2 * 16 * ND * WAVE * 4, "room for them");
+    float* to = (float*)(wave < 2 ? kv0_lds : kv1_lds) +
+                (wave & 1) * 16 * ND * WAVE + lane;
+    __syncthreads();
+    if (half) {
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) to[(i * 16 + r) * WAVE] = acc[i][r];
+    }
+    __syncthreads();
+    if (half) return;
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][r] += to[(i * 16 + r) * WAVE];
   }
   if (p >= s.sq) return;
   unsigned short* dst = dq + ((row * b + bi) * nh + head) * D;
@@ -752,6 +815,23 @@ dim3 grid_for(long heads, int total, int n) {
     }                                                \
   } while (0)
 
+// Tiles of a stream, where every other sequence ends in a part of one.
+static long tiles_of(int n, int total, long heads) {
+  return heads * (total / BM + (n + 1) / 2);
+}
+
+// Whether a tile of queries has eight waves, four for every other tile of keys,
+// so that its block is done in half the time: where there are hardly more than
+// two blocks for each of 256 CUs, and sequences are not short.  Forward and
+// dQ, us, with four waves and with eight: 2048 tokens, 16 heads of 128, 272
+// blocks, 46 + 46 and 39 + 40; 4096 tokens, 8 heads, 264, 82 + 81 and 67 + 66,
+// 16 heads, 528, 98 + 95 and 85 + 78; two of 2048, 16 heads, 528, 53 + 52 and
+// 51 + 49; 1500 + 900 tokens, 32 heads of 64, 608, 29 + 36 and 32 + 39; five
+// of 310 tokens in all 7.0 and 7.7.
+static bool in_halves(int n, int tq, int tk, int b, int nh) {
+  return tiles_of(n, tq, (long)b * nh) <= 576 && tk / std::max(n, 1) >= 512;
+}
+
 void launch_packed_attn_fwd(const void* q, const void* k, const void* v,
                             void* o, void* low, float* lse, const int* cu_q,
                             const int* cu_k, int n, int tq, int tk, int b,
@@ -760,24 +840,26 @@ void launch_packed_attn_fwd(const void* q, const void* k, const void* v,
                             const long* vs, hipStream_t stream) {
   const Packing pk = {cu_q, cu_k, n, tq, tk};
   const dim3 grid = grid_for((long)b * nh, tq, n);
-#define RUN(T, DD, CC)                                                      \
-  hipLaunchKernelGGL((packed_fwd_kernel<T, DD, CC>), grid, dim3(BLOCK), 0,  \
-                     stream, (const unsigned short*)q,                      \
-                     (const unsigned short*)k, (const unsigned short*)v,    \
-                     (unsigned short*)o, (unsigned short*)low, lse, pk, b,  \
-                     nh, ng, scale * LOG2E,                                 \
-                     Strides{qs[0], qs[1], qs[2]},                          \
+#define LAUNCH(T, DD, CC, HALVES)                                           \
+  hipLaunchKernelGGL((packed_fwd_kernel<T, DD, CC, HALVES>), grid,          \
+                     dim3(BLOCK * HALVES), 0, stream,                       \
+                     (const unsigned short*)q, (const unsigned short*)k,    \
+                     (const unsigned short*)v, (unsigned short*)o,          \
+                     (unsigned short*)low, lse, pk, b, nh, ng,              \
+                     scale * LOG2E, Strides{qs[0], qs[1], qs[2]},           \
                      Strides{ks[0], ks[1], ks[2]},                          \
                      Strides{vs[0], vs[1], vs[2]})
+#define RUN(T, DD, CC)                                                      \
+  do {                                                                      \
+    if (halves) LAUNCH(T, DD, CC, 2); else LAUNCH(T, DD, CC, 1);            \
+  } while (0)
+  const bool halves = in_halves(n, tq, tk, b, nh);
   PACKED_DISPATCH(RUN);
 #undef RUN
+#undef LAUNCH
   HIP_CHECK_LAUNCH();
 }
 
-// Tiles of keys, where every other sequence ends in a part of one.
-static long dkv_blocks(int n, int tk, int b, int ng) {
-  return (long)b * ng * (tk / BM + (n + 1) / 2);
-}
 
 // From so many blocks on, three for each of 256 CUs, four waves do at D = 64.
 // Backward with eight and four waves, us, 16 heads: 4096 tokens in two
@@ -803,7 +885,7 @@ static constexpr long FOUR_WAVES = 768;
 int packed_attn_shares(int n, int tq, int tk, int b, int nh, int ng, int d,
                        long* floats) {
   constexpr long FILL = 512, LEAST = 2;
-  const long blocks = dkv_blocks(n, tk, b, ng);
+  const long blocks = tiles_of(n, tk, (long)b * ng);
   const int bq = d == 128 ? Dkv<128, false>::BQ : Dkv<64, false>::BQ;
   const long tiles = (long)(nh / ng) * (tq / std::max(n, 1)) / (2 * bq);
   long fill = (FILL + blocks / 2) / std::max(blocks, 1l);
@@ -818,26 +900,32 @@ void launch_packed_attn_bwd(const void* dout, const void* q, const void* k,
                             const void* v, const void* o, const void* low,
                             const float* lse, float* dot, void* dq, void* dk,
                             void* dv, float* sums, int shares, const int* cu_q,
-                            const int* cu_k, int n, int tq, int tk, int b, int nh, int ng, int d, float scale,
-                            bool causal, bool fp16, const long* os,
-                            const long* qs, const long* ks, const long* vs,
+                            const int* cu_k, int n, int tq, int tk, int b,
+                            int nh, int ng, int d, float scale, bool causal,
+                            bool fp16, const long* os, const long* qs,
+                            const long* ks, const long* vs,
                             hipStream_t stream) {
   const Packing pk = {cu_q, cu_k, n, tq, tk};
   const Strides so = {os[0], os[1], os[2]}, sq = {qs[0], qs[1], qs[2]},
                 sk = {ks[0], ks[1], ks[2]}, sv = {vs[0], vs[1], vs[2]};
   if (tq > 0) {
     const dim3 grid = grid_for((long)b * nh, tq, n);
-#define RUN(T, DD, CC)                                                       \
-  hipLaunchKernelGGL((packed_bwd_dq_kernel<T, DD, CC>),                      \
-                     grid, dim3(BLOCK), 0, stream,                   \
+#define LAUNCH(T, DD, CC, HALVES)                                            \
+  hipLaunchKernelGGL((packed_bwd_dq_kernel<T, DD, CC, HALVES>), grid,        \
+                     dim3(BLOCK * HALVES), 0, stream,                        \
                      (const unsigned short*)q, (const unsigned short*)k,     \
                      (const unsigned short*)v, (const unsigned short*)dout,  \
                      (const unsigned short*)o, (const unsigned short*)low,   \
-                     lse, dot,                                               \
-                     (unsigned short*)dq, pk, b, nh, ng, scale,              \
+                     lse, dot, (unsigned short*)dq, pk, b, nh, ng, scale,    \
                      sq, sk, sv, so)
+#define RUN(T, DD, CC)                                                       \
+  do {                                                                       \
+    if (halves) LAUNCH(T, DD, CC, 2); else LAUNCH(T, DD, CC, 1);             \
+  } while (0)
+    const bool halves = in_halves(n, tq, tk, b, nh);
     PACKED_DISPATCH(RUN);
 #undef RUN
+#undef LAUNCH
     HIP_CHECK_LAUNCH();
   }
   if (tk > 0) {
@@ -854,7 +942,7 @@ void launch_packed_attn_bwd(const void* dout, const void* q, const void* k,
     if (DD == 64 && many) LAUNCH(T, 64, CC, true);                           \
     else LAUNCH(T, DD, CC, false);                                           \
   } while (0)
-    const bool many = dkv_blocks(n, tk, b, ng) >= FOUR_WAVES;
+    const bool many = tiles_of(n, tk, (long)b * ng) >= FOUR_WAVES;
     PACKED_DISPATCH(RUN);
 #undef RUN
 #undef LAUNCH

@@ -246,6 +246,25 @@ def test_shares_without_queries():
 
 
 @gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens_q,lens_k,causal", [
+    ([513], None, True),
+    ([1100], None, False),
+    ([700, 0, 900], None, True),
+    ([5], [1500], True),                # of two halves the queries see both
+    ([40, 3], [63, 1200], True),        # and here the first one alone
+    ([1300], [600], True),              # rows without keys
+])
+def test_two_halves_of_the_keys(lens_q, lens_k, causal, d):
+    """Few tiles of long sequences: eight waves a tile."""
+    _check(lens_q, lens_k, causal=causal, d=d, nh=2, ng=1, tail=3,
+           dtype=torch.float16)
+    _check(lens_q, lens_k, causal=causal, d=d, nh=3, ng=3, grads=False)
+    # scores of some 20: all weight on few keys, in one half or the other
+    _check(lens_q, lens_k, causal=causal, d=d, nh=1, ng=1, scale=1.0)
+
+
+@gpu
 @pytest.mark.parametrize("lens,heads", [
     ([7 * i % 23 for i in range(60)], 32),
     ([300, 513, 1, 129] + [40] * 50, 16),
