@@ -65,7 +65,9 @@ def oracle(q, k, v, lens_q, lens_k, causal, scale=None, dout=None, h=0.0,
                 do = dout[qs, b, head].double()
                 dp = do @ z.t()
                 ds = p * (dp - (do * o).sum(-1, keepdim=True))
-                eds = h * ds.abs() + tiny * see + \
+                # a weight below 2^-126 is zero, and its product too
+                lost = 2.0 ** -126 * (dp - (do * o).sum(-1, keepdim=True))
+                eds = h * ds.abs() + tiny * see + see * lost.abs() + \
                     p * (do.abs() * err).sum(-1, keepdim=True)
                 for n, at, val, e in (
                         ("dq", (qs, b, head), ds @ y, eds @ y.abs()),
@@ -80,8 +82,12 @@ def oracle(q, k, v, lens_q, lens_k, causal, scale=None, dout=None, h=0.0,
 
 
 def _rounding(dtype):
+    """Half a step, and what is lost at the small end: fp16 has steps of 2^-24
+    there, so up to 2^-25; bf16 has the range of 32 bits, in which the kernel's
+    exponentials and products are, and those below the smallest normal number,
+    2^-126, come out as zero."""
     return (torch.finfo(dtype).eps / 2,
-            2.0 ** -25 if dtype == torch.float16 else 0.0)
+            2.0 ** -25 if dtype == torch.float16 else 2.0 ** -126)
 
 
 def _inputs(lens_q, lens_k, tail=0, b=1, nh=4, ng=2, d=64,
