@@ -27,52 +27,52 @@ def _text(values):
 def listed():
     return [
         # three short prompts admitted in one engine step: latency
-        {"name": "prompt few tokens", "op": "prompt", "type": "bf16",
+        {"name": "prompt, few tokens", "op": "prompt", "type": "bf16",
          "lens": "17,64,9", "tail": 0, "heads": 16, "groups": 16, "dim": 64},
         # a step's waiting prompts packed into one stream, grouped heads;
         # an empty one, a single token, padding behind the last
-        {"name": "prompt ragged", "op": "prompt", "type": "bf16",
+        {"name": "prompt, ragged", "op": "prompt", "type": "bf16",
          "lens": "801,1,1290,0,333,64,2048,517,129,700", "tail": 37,
          "heads": 32, "groups": 8, "dim": 128},
         # long documents
-        {"name": "prompt long", "op": "prompt", "type": "fp16",
+        {"name": "prompt, long", "op": "prompt", "type": "fp16",
          "lens": "8192,5003,3001,188", "tail": 0, "heads": 32, "groups": 8,
          "dim": 128},
         # a packed training micro-batch, one head for each key head
-        {"name": "train packed", "op": "train", "type": "bf16",
+        {"name": "train, packed", "op": "train", "type": "bf16",
          "lens": "2048,1025,511,1536,77,951,1999,45", "tail": 0,
          "heads": 16, "groups": 16, "dim": 128},
         # many documents of unlike length, grouped heads
-        {"name": "train grouped", "op": "train", "type": "bf16",
+        {"name": "train, grouped", "op": "train", "type": "bf16",
          "lens": "2048,1300,257,2047,640,1,1777,900,128,1500,2048,333,1055,"
                  "1280,1006", "tail": 64, "heads": 32, "groups": 8,
          "dim": 64},
         # a few short conversations, nothing shared: latency
-        {"name": "decode few rows", "op": "decode", "type": "bf16",
+        {"name": "decode, few rows", "op": "decode", "type": "bf16",
          "rows": "1,1,1", "prefix": "0,0,0", "own": "41,7,66", "heads": 16,
          "groups": 16, "dim": 64, "page": 16},
         # several system prompts in one batch, one of them unshared
-        {"name": "decode prefix groups", "op": "decode", "type": "fp16",
+        {"name": "decode, prefix groups", "op": "decode", "type": "fp16",
          "rows": "9,1,6,8", "prefix": "512,0,1040,96",
          "own": "5,190,33,1,250,77,16,140,61,2030,300,12,88,129,1,47,64,201,"
                 "9,33,150,74,280,18", "heads": 32, "groups": 8, "dim": 64,
          "page": 16},
         # a batch on one long system prompt
-        {"name": "decode one prefix", "op": "decode", "type": "bf16",
+        {"name": "decode, one prefix", "op": "decode", "type": "bf16",
          "rows": "64", "prefix": "4096",
          "own": _text(33 + (i * 211) % 667 for i in range(64)),
          "heads": 32, "groups": 8, "dim": 128, "page": 32},
         # the largest batch on a document that all rows ask about
-        {"name": "decode long prefix", "op": "decode", "type": "bf16",
+        {"name": "decode, long prefix", "op": "decode", "type": "bf16",
          "rows": "256", "prefix": "16384",
          "own": _text(1 + (i * 389) % 1024 for i in range(256)),
          "heads": 32, "groups": 8, "dim": 128, "page": 64},
         # one beam search step: every beam continues one of the beams
-        {"name": "fork beams", "op": "fork", "layers": 24, "groups": 16,
+        {"name": "fork, beams", "op": "fork", "layers": 24, "groups": 16,
          "dim": 64, "page": 16, "pages": 96, "lens": "201,201,201,201",
          "src": "1,1,0,1", "dst": "0,1,2,3"},
         # many samples of one prompt
-        {"name": "fork samples", "op": "fork", "layers": 32, "groups": 8,
+        {"name": "fork, samples", "op": "fork", "layers": 32, "groups": 8,
          "dim": 128, "page": 64, "pages": 512,
          "lens": _text([8237] + [0] * 63), "src": _text([0] * 63),
          "dst": _text(range(1, 64))},
