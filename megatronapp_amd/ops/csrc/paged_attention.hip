@@ -368,11 +368,13 @@ __device__ __forceinline__ void own_keys(const unsigned short* q, long qb,
     float mm = -INFINITY, ll = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) mm = fmaxf(mm, lds.m[w][hh]);
+    // a wave without a maximum has a sum of zero, or saw nothing but NaN
 #pragma unroll
     for (int w = 0; w < 4; ++w)
-      ll += lds.m[w][hh] == -INFINITY
-                ? 0.f
-                : lds.l[w][hh] * __builtin_amdgcn_exp2f(lds.m[w][hh] - mm);
+      ll += lds.l[w][hh] *
+            (lds.m[w][hh] == -INFINITY
+                 ? 1.f
+                 : __builtin_amdgcn_exp2f(lds.m[w][hh] - mm));
     const float by = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
     f32x4 y = *(f32x4*)(sums + hh * ROW + (d ^ ((hh & 7) << 2)));
     const long r = (long)row * nh + hk * rep + ht * HEADS + hh;

@@ -482,3 +482,34 @@ def test_long_rows_among_short_ones(nh, ng, d):
     want = oracle(*s)
     for most in (None, 1, 3000):      # only the time depends on it
         _near(paged_attention(*s, max_length=most), want, most)
+
+
+# ------------------------------------------------------------------- NaN
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_query_of_nan_gives_nan(d):
+    """Rows of one piece, of several, and of a group: NaN for the head that
+    has it, and what the other heads and rows give stays."""
+    own = [1, 40, 300, 3000, 5, 90, 700]
+    s = _grouped_state([3, 4], [640, 160], own, d=d, nh=8, ng=2)
+    rows = [0, 1, 2, 3, 6]
+    q = s[0].clone()
+    q[rows, 3] = math.nan
+    for kw in ({}, dict(max_length=1),
+               dict(shared_prefix=_groups([0, 3, 7], [640, 160]))):
+        want = paged_attention(*s, **kw)
+        got = paged_attention(q, *s[1:], **kw)
+        assert torch.isnan(got[rows, 3]).all(), kw
+        got[rows, 3] = want[rows, 3]
+        assert torch.equal(got, want), kw
+
+
+@gpu
+def test_keys_of_nan_give_nan():
+    """A page whose keys are NaN is a piece, or some waves' part of one,
+    without any score."""
+    q, k, v, tables, lengths = _state([2000, 100], d=64, page=256)
+    k[int(tables[0, 3])] = math.nan
+    for most in (None, 1):
+        got = paged_attention(q, k, v, tables, lengths, max_length=most)
+        assert torch.isnan(got[0]).all() and torch.isfinite(got[1]).all()
