@@ -758,17 +758,26 @@ std::vector<torch::Tensor> attn_fwd_ablate(torch::Tensor q, torch::Tensor k,
 }
 
 // --------------------------------------------------------- packed attention
+bool on_16_bytes(const torch::Tensor& t) {
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+
+// A copy that begins on 16 bytes: contiguous() hands a contiguous tensor back,
+// wherever it begins.
+torch::Tensor laid_out(const torch::Tensor& t) {
+  return t.clone(at::MemoryFormat::Contiguous);
+}
+
 // [t, b, h, d] (or [t, h, d], b = 1) in 16 bits; views are read as they are
 // where each row of a head is adjacent and starts on 16 bytes, others are laid
 // out first.  Arguments that cannot be are ValueErrors in Python.
 torch::Tensor packed_rows(const torch::Tensor& t, long* strides) {
   const int h = (int)t.dim() - 2;
-  bool fits = t.stride(h + 1) == 1 &&
-              reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  bool fits = t.stride(h + 1) == 1 && on_16_bytes(t);
   for (int i = 0; i <= h; ++i)
     fits = fits && (t.size(i) <= 1 ||
                     (t.stride(i) % 8 == 0 && t.stride(i) < (1l << 27)));
-  auto r = fits ? t : t.contiguous();
+  auto r = fits ? t : laid_out(t);
   // a single row's stride is never used
   strides[0] = r.size(0) <= 1 ? 0 : (long)r.stride(0);
   strides[1] = h == 1 || r.size(1) <= 1 ? 0 : (long)r.stride(1);
@@ -982,8 +991,7 @@ CacheRefs cache_refs(const torch::Tensor& pages, const torch::Tensor& refs,
                      const torch::Tensor& tables, const torch::Tensor& lengths,
                      const torch::Tensor& status) {
   TORCH_CHECK(pages.is_cuda() && pages.dim() == 6 && pages.size(1) == 2 &&
-                  pages.is_contiguous() &&
-                  reinterpret_cast<uintptr_t>(pages.data_ptr()) % 16 == 0,
+                  pages.is_contiguous() && on_16_bytes(pages),
               "pages must be [layers, 2, P, groups, page, d], contiguous, on "
               "the GPU");
   check_ints(refs, pages, 1, "ref_counts");
@@ -1103,9 +1111,8 @@ void cache_write(CACHE_ARGS, long layer, torch::Tensor k, torch::Tensor v,
   const long es = pages.element_size();
   auto rows = [&](const torch::Tensor& t) {
     const bool fits = t.stride(2) == 1 && t.stride(0) * es % 16 == 0 &&
-                      t.stride(1) * es % 16 == 0 &&
-                      reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-    return fits ? t : t.contiguous();
+                      t.stride(1) * es % 16 == 0 && on_16_bytes(t);
+    return fits ? t : laid_out(t);
   };
   auto kr = rows(k), vr = rows(v);
   const long plane = (long)c.pages * c.groups * c.page * c.token;
@@ -1169,8 +1176,7 @@ torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
                           (t->size(0) == 1 || t->stride(0) % 8 == 0) &&
                           (t->size(1) == 1 || t->stride(1) % 8 == 0) &&
                           t->stride(2) % 8 == 0 &&
-                          t->stride(2) < (1l << 27) &&
-                          reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
+                          t->stride(2) < (1l << 27) && on_16_bytes(*t),
                       "paged_attention: the rows of a page must start on 16 "
                       "bytes");
   const auto tables = paged_ints(page_tables, q, 2, "page_tables");
@@ -1202,9 +1208,8 @@ torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
   auto o = torch::empty({b, nh, d}, q.options());
   if (o.numel() == 0) return o;
   const bool fits = q.stride(2) == 1 && q.stride(0) % 8 == 0 &&
-                    q.stride(1) % 8 == 0 &&
-                    reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0;
-  auto qr = fits ? q : q.contiguous();
+                    q.stride(1) % 8 == 0 && on_16_bytes(q);
+  auto qr = fits ? q : laid_out(q);
   const long room = tables.size(1) * (long)page;
   const long longest = max_length.has_value() ? *max_length : room;
   max_rows = std::max(1l, std::min(max_rows, (long)b));

@@ -589,3 +589,28 @@ def test_padding_causal_is_causal_in_a_packed_stream(device):
     assert torch.equal(got[0], got[1])
     assert not torch.equal(got[0], got[2])
     destroy()
+
+
+def _off_16_bytes(x):
+    """The same values, contiguous, from two bytes behind a border on."""
+    y = torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)[1:].view(
+        x.shape)
+    assert y.is_contiguous() and y.data_ptr() % 16 == 2
+    return y.copy_(x.detach())
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_contiguous_tensors_off_16_bytes(d):
+    """All four inputs, which the kernels load 16 bytes at a time."""
+    lens = [50, 0, 177]
+    params = PackedSeqParams(cu_seqlens_q=_cu(lens, "cuda"))
+
+    def run(x):
+        x = [t.detach().requires_grad_(i < 3) for i, t in enumerate(x)]
+        o = packed_attention(*x[:3], params)
+        return (o.detach(),) + torch.autograd.grad(o, x[:3], x[3])
+
+    inputs = _inputs(lens, lens, tail=3, d=d)
+    for a, b in zip(run(inputs), run([_off_16_bytes(t) for t in inputs])):
+        assert torch.equal(a, b)

@@ -377,3 +377,18 @@ def test_lengths_that_pass_32_bits_are_refused():
                                 torch.zeros(1, **ints))
     with pytest.raises(ValueError, match="2.31"):
         PagedKVCache(1, 1, 1 << 20, 1, 8, 1, 1 << 31, device="cpu")
+
+
+@gpu
+def test_contiguous_tokens_off_16_bytes_are_written():
+    c = make("cuda", d=64, groups=4)
+    odd = torch.randn(3 * 4 * 64 + 1, device="cuda").bfloat16()[1:].view(
+        3, 4, 64)
+    assert odd.is_contiguous() and odd.data_ptr() % 16 == 2
+    c.extend([4, 0, 2], 1)
+    c.write(0, odd, odd, [4, 0, 2])
+    c.check()
+    for i, s in enumerate([4, 0, 2]):
+        p = int(c.page_tables[s, 0])
+        assert torch.equal(c.keys(0)[p, :, 0], odd[i])
+        assert torch.equal(c.values(0)[p, :, 0], odd[i])
