@@ -129,7 +129,10 @@ class PagedInferenceContext:
         self._set_slots(slots)
         self.prefill = False
         self.cache.extend(self._slots, 1)
-        self._positions = self.cache.lengths[self._slots.long()].long() - 1
+        # where no page was left an empty slot stays so, which check() reports;
+        # its row still indexes tables of positions
+        self._positions = (self.cache.lengths[self._slots.long()].long()
+                           - 1).clamp_(min=0)
         key = (tuple(slots), tuple(shared or ()))
         if self._groups != key:
             self._groups = key

@@ -320,3 +320,25 @@ def test_all_of_them_as_a_server_would():
     for t in (0, 15, 16, 69, 70, 102, 103, 107):
         a = max(x for x in (0, 70, 103) if x <= t)
         near(prompt[t], q[t], kv[0, 0, a:t + 1], kv[0, 1, a:t + 1])
+
+
+def _context(slots=3, pages=None, page=16, longest=64, device="cpu"):
+    from megatronapp_amd.core.inference.paged_context import (
+        PagedInferenceContext)
+    return PagedInferenceContext(
+        1, 2, 64, slots, longest, page, pages, device=device,
+        dtype=torch.float32 if device == "cpu" else torch.bfloat16)
+
+
+def _new_keys(t, b=1):
+    return torch.randn(3, t, b, 2, 64).unbind(0)
+
+
+def test_a_step_without_pages_left_has_positions_in_range():
+    """They index tables of positions, on the GPU without a check."""
+    ctx = _context(pages=1)
+    ctx.begin_prompts([0], [16])
+    ctx.set_active([0, 1])
+    assert ctx.row_positions().tolist() == [15, 0]
+    with pytest.raises(RuntimeError, match="no free page"):
+        ctx.cache.check()
