@@ -102,7 +102,12 @@ class PagedInferenceContext:
         self.active = list(slots)
 
     def begin_prompts(self, slots: List[int], lengths: List[int]):
-        """The next call of the model is one stream of these prompts."""
+        """The next call of the model is one stream of these prompts, in
+        slots that hold nothing."""
+        used = [s for s in slots if self.host_lengths[s]]
+        if used:
+            raise ValueError(f"PagedInferenceContext: slots in use: {used}; "
+                             "release() empties them")
         self._set_slots(slots)
         self.prefill = True
         self.cache.extend(self._slots, lengths)

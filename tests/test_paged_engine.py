@@ -342,3 +342,16 @@ def test_a_step_without_pages_left_has_positions_in_range():
     assert ctx.row_positions().tolist() == [15, 0]
     with pytest.raises(RuntimeError, match="no free page"):
         ctx.cache.check()
+
+
+def test_prompts_are_refused_in_slots_in_use():
+    """Their tokens would lie behind what the slot holds, and not see it."""
+    ctx = _context()
+    ctx.begin_prompts([0, 2], [5, 1])
+    for slots in ([0], [1, 2]):
+        with pytest.raises(ValueError, match="in use"):
+            ctx.begin_prompts(slots, [3] * len(slots))
+    assert ctx.cache.lengths.tolist() == ctx.host_lengths == [5, 0, 1]
+    ctx.release(0)
+    ctx.begin_prompts([0], [3])
+    assert ctx.cache.lengths.tolist() == ctx.host_lengths == [3, 0, 1]
