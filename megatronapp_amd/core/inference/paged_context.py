@@ -95,6 +95,14 @@ class PagedInferenceContext:
             self.host_lengths[s] = n
         self._groups = None
 
+    def _check_room(self, slots: List[int], more: List[int]):
+        full = [s for s, n in zip(slots, more)
+                if self.host_lengths[s] + n > self.max_sequence_length]
+        if full:
+            raise ValueError(f"PagedInferenceContext: slots {full} would "
+                             "hold more than max_sequence_length "
+                             f"{self.max_sequence_length}")
+
     def _set_slots(self, slots: List[int]):
         if self._slots is None or slots != self.active:
             self._slots = torch.tensor(slots, dtype=torch.int32,
@@ -108,6 +116,7 @@ class PagedInferenceContext:
         if used:
             raise ValueError(f"PagedInferenceContext: slots in use: {used}; "
                              "release() empties them")
+        self._check_room(slots, lengths)
         self._set_slots(slots)
         self.prefill = True
         self.cache.extend(self._slots, lengths)
@@ -131,6 +140,7 @@ class PagedInferenceContext:
         ``shared`` says how the batch begins, as (rows, tokens) of groups of
         rows that share as many first tokens."""
         assert not prefill, "begin_prompts() admits prompts"
+        self._check_room(slots, [1] * len(slots))
         self._set_slots(slots)
         self.prefill = False
         self.cache.extend(self._slots, 1)

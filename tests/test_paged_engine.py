@@ -355,3 +355,17 @@ def test_prompts_are_refused_in_slots_in_use():
     ctx.release(0)
     ctx.begin_prompts([0], [3])
     assert ctx.cache.lengths.tolist() == ctx.host_lengths == [3, 0, 1]
+
+
+def test_sequences_end_at_the_longest():
+    """The pages may hold more than that, and tables of positions do not."""
+    ctx = _context(longest=20)
+    with pytest.raises(ValueError, match="max_sequence_length"):
+        ctx.begin_prompts([0, 1], [20, 21])
+    ctx.begin_prompts([0, 1], [20, 19])
+    ctx.set_active([1])
+    ctx.advance(1)
+    for slots in ([1], [0], [2, 0]):
+        with pytest.raises(ValueError, match="max_sequence_length"):
+            ctx.set_active(slots)
+    assert ctx.cache.lengths.tolist() == ctx.host_lengths == [20, 20, 0]
