@@ -415,16 +415,25 @@ torch::Tensor scaled_masked_softmax_fwd(torch::Tensor x,
                                         c10::optional<torch::Tensor> mask,
                                         double scale) {
   check_bf16(x, "x");
-  // x: [b, np, sq, sk]
+  // x: [b, np, sq, sk]; mask: [b or 1, np or 1, sq or 1, sk], or without np
   const int sk = (int)x.size(-1);
   const int sq = (int)x.size(-2);
-  const int np = (int)x.size(1);
+  int np = (int)x.size(1);
   const long rows = x.numel() / sk;
   auto y = torch::empty_like(x);
   const void* mptr = nullptr;
   torch::Tensor m8;
   if (mask.has_value()) {
-    m8 = mask->to(torch::kUInt8).contiguous();
+    const auto m = mask->dim() == 3 ? mask->unsqueeze(1) : *mask;
+    TORCH_CHECK(x.dim() == 4 && m.dim() == 4,
+                "scaled_masked_softmax: x must be [b, np, sq, sk], mask "
+                "[b, np, sq, sk] or [b, sq, sk]");
+    // the kernel reads a mask for each of the batch, or for each row of it
+    const bool heads = m.size(1) != 1;
+    m8 = m.expand({x.size(0), heads ? np : 1, sq, sk})
+             .to(torch::kUInt8)
+             .contiguous();
+    if (heads) np = 1;
     mptr = m8.data_ptr();
   }
   launch_softmax_masked_fwd(x.data_ptr(), mptr, y.data_ptr(), rows, np, sq, sk,

@@ -1059,3 +1059,27 @@ def test_split_qkv_flash_zero_copy_grads():
         hn ** -0.5, True)
     ref = torch.cat([dq, dk, dv], dim=-1).reshape(sq, b, -1)
     assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("shape", [(1, 1, 24, 40), (3, 1, 24, 40),
+                                   (3, 2, 24, 40), (1, 2, 24, 40),
+                                   (3, 1, 1, 40), (3, 24, 40)])
+def test_masked_softmax_broadcasts_its_mask(shape):
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(3, 2, 24, 40, generator=g).bfloat16().cuda()
+    mask = (torch.rand(shape, generator=g) < 0.4).cuda()
+    got = _ops().scaled_masked_softmax_fwd(x, mask, 0.5)
+    wide = mask.unsqueeze(1) if mask.dim() == 3 else mask
+    want = torch.softmax((x.double() * 0.5).masked_fill(wide, float("-inf")), -1)
+    # one rounding to bf16 (2^-8 at most), beside sums and exponentials in 32
+    # bits, which 1% of it covers; a row that is masked whole gives zeros
+    want = want.nan_to_num(0.0)
+    assert ((got.double() - want).abs() <= 1.01 * 2.0 ** -8 * want).all()
+
+
+def test_masked_softmax_refuses_masks_that_do_not_fit():
+    x = torch.zeros(2, 2, 8, 8, device="cuda").bfloat16()
+    for shape in ((3, 1, 8, 8), (2, 1, 8, 16), (8, 8), (2, 3, 8, 8)):
+        with pytest.raises(RuntimeError):
+            _ops().scaled_masked_softmax_fwd(
+                x, torch.zeros(shape, dtype=torch.bool, device="cuda"), 1.0)
