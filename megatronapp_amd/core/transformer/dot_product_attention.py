@@ -95,15 +95,18 @@ class DotProductAttention(nn.Module):
         scores = scores.view(b, np_, sq, sk)
 
         mask_type = attn_mask_type if attn_mask_type is not None else self.attn_mask_type
+        unseeing = None
         if packed_seq_params is not None and \
                 packed_seq_params.cu_seqlens_q is not None:
-            # packed (THD) stream: block-diagonal causal mask
+            # packed (THD) stream: block-diagonal mask; rows that see no key
+            # give zeros
             from ..packed_seq_params import packed_attention_mask
             from ..enums import AttnMaskType as _AMT
             attention_mask = packed_attention_mask(
-                packed_seq_params.cu_seqlens_q, sk,
-                causal=mask_type in _CAUSAL)
+                packed_seq_params.cu_seqlens_q, sq, mask_type in _CAUSAL,
+                packed_seq_params.cu_seqlens_kv, sk)
             mask_type = _AMT.padding
+            unseeing = attention_mask.all(-1).view(sq, 1, 1)
         probs = self.scale_mask_softmax(scores, attention_mask, mask_type)
 
         # MegaScope raw-attention-score tap (reference
@@ -127,6 +130,8 @@ class DotProductAttention(nn.Module):
         v = value.permute(1, 2, 0, 3).reshape(b * np_, sk, hn_v)    # [b*np, sk, hn_v]
         context = torch.bmm(probs.view(b * np_, sq, sk), v)         # [b*np, sq, hn_v]
         context = context.transpose(0, 1).reshape(sq, b, np_ * hn_v)
+        if unseeing is not None:        # their weights are not all zero
+            context = context.masked_fill(unseeing, 0.0)
         return context
 
 

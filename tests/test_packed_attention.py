@@ -614,3 +614,54 @@ def test_contiguous_tensors_off_16_bytes(d):
     inputs = _inputs(lens, lens, tail=3, d=d)
     for a, b in zip(run(inputs), run([_off_16_bytes(t) for t in inputs])):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("mask", ["causal", "padding"])
+@pytest.mark.parametrize("cu_q,cu_k,tq,tk", [
+    ([3, 10, 20], None, 20, 20),            # places in front
+    ([0, 10, 16], None, 20, 20),            # and behind
+    ([0, 10, 20, 20], None, 20, 20),        # an empty last one
+    ([2, 2, 9, 9, 15], None, 18, 18),       # all of these
+    ([0, 4, 4, 9], [0, 7, 10, 12], 9, 12),  # continued prompts, one empty
+    ([1, 6, 8], [3, 5, 5], 10, 7),          # rows and sequences without keys
+    ([0, 5, 500], None, 12, 12),            # an end out of the stream
+    ([4], None, 6, 6),                      # no sequence at all
+])
+def test_fallback_gives_what_the_kernel_gives(cu_q, cu_k, tq, tk, mask,
+                                              device):
+    """32 bits are not the kernel's, so the layers' attention takes the eager
+    path; both are off by some 1e-6 of terms of order one."""
+    from tests.utils import destroy, initialize_model_parallel
+    from megatronapp_amd.core.enums import AttnMaskType
+    from megatronapp_amd.core.transformer.dot_product_attention import (
+        FlashAttention)
+    from megatronapp_amd.core.transformer_config import TransformerConfig
+    initialize_model_parallel()
+    cfg = TransformerConfig(num_layers=1, hidden_size=32,
+                            num_attention_heads=4, num_query_groups=2,
+                            hidden_dropout=0.0, attention_dropout=0.0)
+    g = torch.Generator().manual_seed(8)
+    q, dout = (torch.randn(tq, 2, 4, 8, generator=g).to(device)
+               for _ in range(2))
+    k, v = (torch.randn(tk, 2, 2, 8, generator=g).to(device)
+            for _ in range(2))
+    x = [t.requires_grad_(True) for t in (q, k, v)]
+    params = PackedSeqParams(*(
+        ["thd"] + [c if c is None else
+                   torch.tensor(c, dtype=torch.int32, device=device)
+                   for c in (cu_q, cu_k)]))
+    got = FlashAttention(cfg, 1, AttnMaskType[mask])(
+        *x, packed_seq_params=params).view(tq, 2, 4, 8)
+    on_host = PackedSeqParams(*(
+        ["thd"] + [c if c is None else torch.tensor(c) for c in (cu_q, cu_k)]))
+    y = [t.detach().cpu().requires_grad_(True) for t in x]
+    want = packed_attention(*y, on_host, causal=mask == "causal")
+    pairs = [(got, want)] + list(zip(
+        torch.autograd.grad(got, x, dout),
+        torch.autograd.grad(want, y, dout.cpu(), materialize_grads=True,
+                            allow_unused=True)
+        if want.requires_grad else [torch.zeros_like(t) for t in y]))
+    for a, b in pairs:
+        assert (a.detach().cpu() - b.detach()).abs().max() < 1e-5
+    destroy()
