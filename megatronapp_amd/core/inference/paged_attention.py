@@ -17,6 +17,7 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from ... import ops as _ops
 
@@ -160,5 +161,9 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor,
              else float(softmax_scale))
     _check(query, key_pages, value_pages, page_tables, lengths, slots,
            shared_prefix, scale)
+    if any(forward_ad.unpack_dual(x).tangent is not None
+           for x in (query, key_pages, value_pages)):
+        raise ValueError("paged_attention: has no gradient, in forward mode "
+                         "neither")
     return _paged_attention_plain(query, key_pages, value_pages, page_tables,
                                   lengths, slots, scale)

@@ -7,11 +7,11 @@ before the first or behind the last sequence, give zeros, and get and give no
 gradient.
 
 On the GPU this is ``ops/csrc/packed_attention.hip`` (bf16 and fp16, head
-sizes 64 and 128), whose gradient cannot be differentiated again; on the CPU a
-plain computation in 32 bits or more.  A
-sequence's values reach no other sequence, whatever they are.  Within one, a
-value of v that is not finite may reach earlier rows of the same 64-key tile
-(nothing times NaN is NaN).
+sizes 64 and 128), whose gradient cannot be differentiated again, and which
+refuses forward-mode derivatives; on the CPU a plain computation in 32 bits or
+more.  A sequence's values reach no other sequence, whatever they are.  Within
+one, a value of v that is not finite may reach earlier rows of the same 64-key
+tile (nothing times NaN is NaN).
 """
 
 from __future__ import annotations

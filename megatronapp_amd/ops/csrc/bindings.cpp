@@ -4,6 +4,7 @@
 #include <torch/extension.h>
 
 #include <ATen/hip/HIPContext.h>
+#include <c10/core/AutogradState.h>
 
 #include <cmath>
 
@@ -851,6 +852,15 @@ PackedShape packed_shape(const torch::Tensor& q, const torch::Tensor& k,
           (int)cu_q.numel() - 1, fp16};
 }
 
+// Whether forward mode wants a derivative along with the value.  A call that
+// has none would else come back as a constant.
+bool has_tangent(std::initializer_list<const torch::Tensor*> inputs) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return false;
+  for (auto* t : inputs)
+    if (t->_fw_grad(0).defined()) return true;
+  return false;
+}
+
 torch::Tensor int32_row(const torch::Tensor& t) {
   return (t.scalar_type() == torch::kInt32 ? t : t.to(torch::kInt32))
       .contiguous();
@@ -974,6 +984,9 @@ torch::Tensor packed_attention(torch::Tensor q, torch::Tensor k,
                                torch::Tensor v, torch::Tensor cu_q,
                                c10::optional<torch::Tensor> cu_kv,
                                c10::optional<double> scale, bool causal) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent({&q, &k, &v}),
+                              "packed_attention: on the GPU no forward-mode "
+                              "derivative");
   if (torch::GradMode::is_enabled() &&
       (q.requires_grad() || k.requires_grad() || v.requires_grad()))
     return PackedAttn::apply(q, k, v, cu_q, cu_kv, scale, causal);
@@ -1157,6 +1170,9 @@ torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
   TORCH_CHECK_VALUE(q.dim() == 3 && k.dim() == 4 && v.sizes() == k.sizes(),
                     "paged_attention: query must be [b, heads, d], key and "
                     "value pages [P, groups, page, d]");
+  TORCH_CHECK_VALUE(!has_tangent({&q, &k, &v}),
+                    "paged_attention: has no gradient, in forward mode "
+                    "neither");
   const int b = (int)q.size(0), nh = (int)q.size(1), d = (int)q.size(2);
   const int ng = (int)k.size(1), page = (int)k.size(2);
   TORCH_CHECK_VALUE(k.size(3) == d && ng > 0 && nh % ng == 0 &&

@@ -665,3 +665,36 @@ def test_fallback_gives_what_the_kernel_gives(cu_q, cu_k, tq, tk, mask,
     for a, b in pairs:
         assert (a.detach().cpu() - b.detach()).abs().max() < 1e-5
     destroy()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("which", range(3))
+def test_forward_mode_has_its_derivative_or_is_refused(which, device):
+    """On the CPU the tangent is that of differences; the kernel has none, and
+    says so rather than give a constant."""
+    from torch.autograd import forward_ad
+    dtype = torch.bfloat16 if device == "cuda" else torch.float64
+    q, k, v, dout = _inputs([5, 3], [5, 3], device=device, dtype=dtype)
+    x, way = [q, k, v], [dout, k.flip(0), v.flip(0)][which]
+    params = PackedSeqParams(cu_seqlens_q=_cu([5, 3], device))
+    for wants in (False, True):     # a reverse gradient beside it
+        y = [t.clone().requires_grad_(wants) for t in x]
+        with forward_ad.dual_level():
+            y[which] = forward_ad.make_dual(y[which], way)
+            if device == "cuda":
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    packed_attention(*y, params)
+                continue
+            got = forward_ad.unpack_dual(packed_attention(*y, params)).tangent
+        ends = []
+        for step in (1e-5, -1e-5):
+            z = list(x)
+            z[which] = z[which] + step * way
+            ends.append(packed_attention(*z, params))
+        # the third derivative, of some hundreds at most, times the step's
+        # square, and 64 bits' 1e-16 of values of order one over the step
+        assert (got - (ends[0] - ends[1]) / 2e-5).abs().max() < 1e-7
+    if device == "cuda":            # without a wish for it, a value
+        with forward_ad.dual_level(), forward_ad._set_fwd_grad_enabled(False):
+            y[which] = forward_ad.make_dual(x[which], way)
+            packed_attention(*y, params)

@@ -513,3 +513,14 @@ def test_keys_of_nan_give_nan():
     for most in (None, 1):
         got = paged_attention(q, k, v, tables, lengths, max_length=most)
         assert torch.isnan(got[0]).all() and torch.isfinite(got[1]).all()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("which", range(3))
+def test_forward_mode_is_refused(which, device):
+    from torch.autograd import forward_ad
+    s = list(_state([20, 20], device=device))
+    with forward_ad.dual_level():
+        s[which] = forward_ad.make_dual(s[which], torch.ones_like(s[which]))
+        with torch.no_grad(), pytest.raises(ValueError, match="forward mode"):
+            paged_attention(*s)
