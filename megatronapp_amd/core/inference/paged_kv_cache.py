@@ -20,6 +20,7 @@ from __future__ import annotations
 from typing import Optional, Sequence, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from ... import ops as _ops
 
@@ -262,7 +263,8 @@ class PagedKVCache:
               slots: Slots, cu_seqlens: Optional[torch.Tensor] = None):
         """Puts key and value [tokens, groups, d] in the last places of the
         slots' sequences: one token each, or tokens cu_seqlens[i] to
-        cu_seqlens[i + 1] as the last of slots[i].  No slot is named twice."""
+        cu_seqlens[i + 1] as the last of slots[i].  No slot is named twice.
+        The cache holds values: no derivative goes through it."""
         slots = self._list("slots", slots, self.max_slots, True)
         if not 0 <= layer < self.pages.shape[0]:
             raise ValueError(f"PagedKVCache: no layer {layer}")
@@ -385,6 +387,8 @@ class PagedKVCache:
 
     def _write_plain(self, layer, key, value, slots, cu):
         cu = list(range(len(slots) + 1)) if cu is None else cu.tolist()
+        key, value = (forward_ad.unpack_dual(x.detach()).primal
+                      for x in (key, value))
         for s, a, b in zip(slots, cu[:-1], cu[1:]):
             for t in range(max(a, 0), min(b, key.shape[0])):
                 if not 0 <= s < self.max_slots:

@@ -392,3 +392,19 @@ def test_contiguous_tokens_off_16_bytes_are_written():
         p = int(c.page_tables[s, 0])
         assert torch.equal(c.keys(0)[p, :, 0], odd[i])
         assert torch.equal(c.values(0)[p, :, 0], odd[i])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_the_cache_holds_values_without_their_derivatives(device):
+    from torch.autograd import forward_ad
+    c = make(device)
+    x = torch.randn(1, 2, 8).to(c.pages).requires_grad_(True)
+    c.extend([0], 1)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        c.write(0, dual * 2, dual, [0])
+        assert not c.pages.requires_grad
+        assert forward_ad.unpack_dual(c.pages).tangent is None
+    page = int(c.page_tables[0, 0])
+    assert torch.equal(c.keys(0)[page, :, 0], x[0].detach() * 2)
+    assert torch.equal(c.values(0)[page, :, 0], x[0].detach())
