@@ -698,3 +698,18 @@ def test_forward_mode_has_its_derivative_or_is_refused(which, device):
         with forward_ad.dual_level(), forward_ad._set_fwd_grad_enabled(False):
             y[which] = forward_ad.make_dual(x[which], way)
             packed_attention(*y, params)
+
+
+@gpu
+@pytest.mark.parametrize("lens", [[300, 41, 200], [2100], [64, 1000, 3]])
+@pytest.mark.parametrize("d", [64, 128])
+def test_the_same_bits_with_and_without_gradients(lens, d):
+    """Recomputation runs the first forward without them and the second one
+    with them.  Large scores: the running maximum moves often."""
+    q, k, v, _ = _inputs(lens, lens, d=d)
+    q = q * 6.0
+    params = PackedSeqParams(cu_seqlens_q=_cu(lens, "cuda"))
+    with torch.no_grad():
+        first = packed_attention(q, k, v, params)
+    again = packed_attention(q.requires_grad_(True), k, v, params)
+    assert torch.equal(first, again.detach())
