@@ -91,9 +91,9 @@ def _check(query, key_pages, value_pages, page_tables, lengths, slots,
             f"paged_attention: query {tuple(query.shape)} and pages "
             f"{tuple(key_pages.shape)} do not fit each other")
     page = key_pages.shape[2]
-    if page < 16 or page % 16 or (page > 512 and page & (page - 1)):
+    if page < 16 or page % 16:
         raise ValueError("paged_attention: pages must hold a multiple of 16 "
-                         "tokens, above 512 a power of two")
+                         "tokens")
     if key_pages.dtype != query.dtype or value_pages.dtype != query.dtype or \
             not query.is_floating_point():
         raise ValueError("paged_attention: query and pages must share one "

@@ -1179,10 +1179,9 @@ torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
                         k.size(0) > 0 && k.size(0) < (1l << 30),
                     "paged_attention: query ", q.sizes(), " and pages ",
                     k.sizes(), " do not fit each other");
-  TORCH_CHECK_VALUE(page >= 16 && page % 16 == 0 &&
-                        (page <= 512 || (page & (page - 1)) == 0),
+  TORCH_CHECK_VALUE(page >= 16 && page % 16 == 0,
                     "paged_attention: pages must hold a multiple of 16 "
-                    "tokens, above 512 a power of two");
+                    "tokens");
   TORCH_CHECK_VALUE(k.scalar_type() == q.scalar_type() &&
                         v.scalar_type() == q.scalar_type(),
                     "paged_attention: query and pages must share one floating "

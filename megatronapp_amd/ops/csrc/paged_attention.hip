@@ -38,7 +38,8 @@ struct Cache {
   const int* slots;           // [b], or the rows themselves
   long kp, kh, kt, vp, vh, vt;  // strides of pages, heads, tokens
   int pages, page, width, count;  // pages, tokens of one, table, its rows
-  unsigned long magic;        // 2^32 / (page / 16), rounded up
+  unsigned long magic;        // 2^shift / (page / 16), rounded up
+  int shift;
 };
 
 // Groups of rows that share their first pages; none: groups == 0.
@@ -69,8 +70,13 @@ __host__ __device__ constexpr int cuts(int keys, int evenly, int most) {
 }
 
 // the page and the place in it of a token, at a multiple of 16
+//
+// With p = page / 16 and shift = 37 + floor(log2 p), magic is at most 2^37 and
+// off by less than one.  x = token / 16 is below 2^27, so the product fits 64
+// bits and is off by less than 2^27, where 2^shift / p, one part in p of a
+// page, is above 2^36: the quotient is exact for any multiple of 16.
 __device__ __forceinline__ int page_of(const Cache& c, int token, int& in) {
-  const int i = (int)(((unsigned long)(token >> 4) * c.magic) >> 32);
+  const int i = (int)(((unsigned long)(token >> 4) * c.magic) >> c.shift);
   in = token - i * c.page;
   return i;
 }
@@ -791,9 +797,11 @@ void launch_paged_attn(const void* q, long qb, long qh, const void* k,
                        int shared, int evenly, void* o, float* part, float* lse,
                        float scale, bool fp16, hipStream_t stream) {
   const unsigned long p16 = page / 16;
+  const int shift = 37 + 63 - __builtin_clzl(p16);
   const Cache c = {(const unsigned short*)k, (const unsigned short*)v, tables,
                    lengths, slots, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-                   pages, page, width, count, ((1ul << 32) + p16 - 1) / p16};
+                   pages, page, width, count, ((1ul << shift) + p16 - 1) / p16,
+                   shift};
   const long units = (long)b * ng * ((nh / ng + HEADS - 1) / HEADS);
   const int extra = (int)std::min(units * (own - evenly), 512l);
   const Out out = {(unsigned short*)o, part, lse, own + shared, evenly, extra};

@@ -524,3 +524,34 @@ def test_forward_mode_is_refused(which, device):
         s[which] = forward_ad.make_dual(s[which], torch.ones_like(s[which]))
         with torch.no_grad(), pytest.raises(ValueError, match="forward mode"):
             paged_attention(*s)
+
+
+# ------------------------------------------------------------ sizes of pages
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("page", [528, 1040, 16400])
+def test_any_multiple_of_sixteen_is_a_page(page, device):
+    """As for the cache itself."""
+    s = _state([1, page - 1, page, page + 1, 2 * page + 3], page=page, d=64,
+               spare=1, device=device)
+    want = oracle(*s)
+    _near(paged_attention(*s), want)
+    if device == "cuda":
+        s2 = _grouped_state([9], [2 * page], [5 * i for i in range(9)],
+                            page=page, d=64, nh=8)
+        _near(paged_attention(*s2, shared_prefix=_groups([0, 9], [2 * page])),
+              oracle(*s2))
+
+
+def test_pages_are_found_by_a_product():
+    """The kernel's division of tokens / 16 below 2^27 by p sixteenths, at
+    both sides of every kind of border."""
+    for p in list(range(1, 600)) + [1000, 1023, 1025, 65535, 99991,
+                                    (1 << 27) // 16 - 1, (1 << 27) - 1]:
+        shift = 36 + p.bit_length()
+        magic = ((1 << shift) + p - 1) // p
+        top = (1 << 27) - 1
+        assert top * magic < 1 << 64
+        for k in {1, 2, 3, 1000, top // p - 1, top // p}:
+            for x in (k * p - 1, k * p, k * p + 1, top):
+                if 0 <= x <= top:
+                    assert x * magic >> shift == x // p, (x, p)
