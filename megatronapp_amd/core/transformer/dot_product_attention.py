@@ -214,9 +214,13 @@ class FlashAttention(nn.Module):
     def _packed(self, query, key, value, attention_mask, attn_mask_type,
                 attention_bias, packed_seq_params):
         """A stream of sequences: each attends within itself."""
+        from ..tensor_tracer import FlagType, get_tensor_tracers
+        tt = get_tensor_tracers()
         if not packed_attention_supported(query) or \
                 value.shape != key.shape or \
-                (self.dropout_p > 0 and self.training):
+                (self.dropout_p > 0 and self.training) or \
+                (tt is not None and tt.enabled(       # the kernel has no scores
+                    FlagType.RawAttentionScore, self._fallback.layer_number)):
             return self._fallback(query, key, value, attention_mask,
                                   attn_mask_type, attention_bias,
                                   packed_seq_params)

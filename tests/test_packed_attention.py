@@ -713,3 +713,39 @@ def test_the_same_bits_with_and_without_gradients(lens, d):
         first = packed_attention(q, k, v, params)
     again = packed_attention(q.requires_grad_(True), k, v, params)
     assert torch.equal(first, again.detach())
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_scores_of_a_packed_stream_are_reported(device):
+    """A tracer that asks for them gets them: the kernel has none."""
+    from tests.utils import destroy, initialize_model_parallel
+    from megatronapp_amd.core.enums import AttnMaskType
+    from megatronapp_amd.core.tensor_tracer import (FlagType,
+                                                    enable_tensor_tracers)
+    from megatronapp_amd.core.transformer.dot_product_attention import (
+        FlashAttention)
+    from megatronapp_amd.core.transformer_config import TransformerConfig
+    initialize_model_parallel()
+    dtype = torch.float16 if device == "cuda" else torch.float32
+    cfg = TransformerConfig(num_layers=1, hidden_size=256,
+                            num_attention_heads=4, num_query_groups=2,
+                            fp16=device == "cuda", hidden_dropout=0.0,
+                            attention_dropout=0.0)
+    q, k, v, _ = _inputs([10, 6], [10, 6], dtype=dtype, device=device)
+    cu = _cu([10, 6], device)
+    attend = FlashAttention(cfg, 1, AttnMaskType.causal)
+    tt, seen = enable_tensor_tracers(), []
+    tt.set_num_layers(1)
+    tt.set_report(seen.append)
+    for asked in ("False", "True"):
+        tt.tt_flags.set_by_configs({"Raw_attention_score": asked})
+        o = attend(q, k, v, packed_seq_params=PackedSeqParams(
+            cu_seqlens_q=cu, cu_seqlens_kv=cu))
+        assert o.shape == (16, 1, 256)
+        assert len(seen) == (asked == "True")
+    tt.set_report(None)
+    assert seen[0]["update_type"] == FlagType.RawAttentionScore.value
+    assert seen[0]["args"] == [1, 4, 16, 16]
+    p = torch.tensor(seen[0]["result"]).view(4, 16, 16)
+    assert (p[:, 10:, :10] == 0).all() and (p.triu(1) == 0).all()
+    destroy()
