@@ -14,7 +14,7 @@ from typing import List, Optional, Tuple
 import torch
 
 from .. import parallel_state
-from ..packed_seq_params import PackedSeqParams
+from ..packed_seq_params import PackedSeqParams, packed_attention_mask
 from ..transformer.packed_attention import packed_attention
 from .paged_attention import HEAD_SIZES, SharedPrefix, paged_attention
 from .paged_kv_cache import PagedKVCache
@@ -203,3 +203,32 @@ class PagedInferenceContext:
                 max_length=max(self.host_lengths[s]
                                for s in self.active) + 1).unsqueeze(0)
         return out.reshape(out.shape[0], out.shape[1], -1)
+
+    def attention_weights(self, layer_number: int, query: torch.Tensor,
+                          key: torch.Tensor,
+                          softmax_scale: float) -> torch.Tensor:
+        """For tracers, after attend() of the same tensors: what it weighed
+        the values with, in 32 bits.  [1, heads, tokens, tokens] of packed
+        prompts, [rows, heads, 1, longest] of a decode step."""
+        heads, d = query.shape[2:]
+        groups = key.shape[2]
+        if self.prefill:
+            t = query.shape[0]
+            q = query.permute(1, 2, 0, 3).float().reshape(groups, -1, d)
+            k = key.permute(1, 2, 3, 0).float()[0]          # [groups, d, t]
+            hide = packed_attention_mask(self._packing.cu_seqlens_q, t)
+            shape = (1, heads, t, t)
+        else:
+            longest = max(self.host_lengths[s] for s in self.active) + 1
+            cache, rows = self.cache, self._slots.long()
+            pages = cache.page_tables[rows, :-(-longest // cache.page_size)]
+            k = cache.keys(self._layers[layer_number])[
+                pages.clamp(min=0).long()]      # [rows, pages, groups, page, d]
+            k = k.permute(0, 2, 4, 1, 3).flatten(3)[..., :longest].float()
+            q = query[0].float().view(len(rows), groups, -1, d)
+            hide = torch.arange(longest, device=k.device) >= \
+                cache.lengths[rows, None]
+            hide = hide[:, None, None]
+            shape = (len(rows), heads, 1, longest)
+        scores = torch.matmul(q, k).view(shape) * softmax_scale
+        return torch.softmax(scores.masked_fill(hide, float("-inf")), -1)

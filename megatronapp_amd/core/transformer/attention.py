@@ -209,9 +209,8 @@ class SelfAttention(MegatronModule):
 
         if getattr(inference_context, "is_paged", False):
             with trace_scope("attention"):
-                core_attn_out = inference_context.attend(
-                    self.layer_number, query, key, value,
-                    softmax_scale=self.core_attention.effective_scale())
+                core_attn_out = self.core_attention(
+                    query, key, value, paged_context=inference_context)
             if tt is not None and tt.enabled(FlagType.ContextLayer,
                                              self.layer_number):
                 tt.report(FlagType.ContextLayer, self.layer_number,

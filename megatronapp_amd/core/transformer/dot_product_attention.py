@@ -34,6 +34,17 @@ def attention_mask_func(attention_scores, attention_mask):
 _CAUSAL = (AttnMaskType.causal, AttnMaskType.padding_causal)
 
 
+def _attend_paged(context, layer_number, query, key, value, scale):
+    """Prompts or a decode step of a paged cache, which the context knows."""
+    out = context.attend(layer_number, query, key, value, scale)
+    from ..tensor_tracer import FlagType, get_tensor_tracers
+    tt = get_tensor_tracers()
+    if tt is not None and tt.enabled(FlagType.RawAttentionScore, layer_number):
+        tt.report(FlagType.RawAttentionScore, layer_number,
+                  context.attention_weights(layer_number, query, key, scale))
+    return out
+
+
 class DotProductAttention(nn.Module):
     def __init__(self, config: TransformerConfig, layer_number: int,
                  attn_mask_type: AttnMaskType, attention_type: str = "self",
@@ -74,7 +85,11 @@ class DotProductAttention(nn.Module):
         return (self.scale_mask_softmax.scale or 1.0) / self.norm_factor
 
     def forward(self, query, key, value, attention_mask=None,
-                attn_mask_type=None, attention_bias=None, packed_seq_params=None):
+                attn_mask_type=None, attention_bias=None, packed_seq_params=None,
+                paged_context=None):
+        if paged_context is not None:
+            return _attend_paged(paged_context, self.layer_number, query, key,
+                                 value, self.effective_scale())
         # q: [sq, b, np, hn]; k/v: [sk, b, ng, hn]
         sq, b, np_, hn = query.shape
         sk, _, ng, _ = key.shape
@@ -232,7 +247,11 @@ class FlashAttention(nn.Module):
         return o.reshape(o.shape[0], o.shape[1], -1)
 
     def forward(self, query, key, value, attention_mask=None,
-                attn_mask_type=None, attention_bias=None, packed_seq_params=None):
+                attn_mask_type=None, attention_bias=None, packed_seq_params=None,
+                paged_context=None):
+        if paged_context is not None:
+            return _attend_paged(paged_context, self._fallback.layer_number,
+                                 query, key, value, self.effective_scale())
         if packed_seq_params is not None and \
                 packed_seq_params.cu_seqlens_q is not None:
             return self._packed(query, key, value, attention_mask,

@@ -369,3 +369,72 @@ def test_sequences_end_at_the_longest():
         with pytest.raises(ValueError, match="max_sequence_length"):
             ctx.set_active(slots)
     assert ctx.cache.lengths.tolist() == ctx.host_lengths == [20, 20, 0]
+
+
+def test_layers_attention_is_called_and_reports_its_scores():
+    """As without pages: hooks on the core attention see each call, and a
+    tracer gets the weights, in 32 bits on the CPU within 1e-5 of those."""
+    _cpu_only()
+    from megatronapp_amd.core.tensor_tracer import (FlagType,
+                                                    enable_tensor_tracers)
+    model = _model(groups=2)
+    tt = enable_tensor_tracers()
+    tt.set_num_layers(2)
+    tt.tt_flags.set_by_configs({"Raw_attention_score": "True"})
+    sp = SamplingParams(num_tokens_to_generate=4, top_k=1)
+    calls, seen = [], {}
+    for layer in model.decoder.layers:
+        layer.self_attention.core_attention.register_forward_hook(
+            lambda *a: calls.append(a[0]))
+    for paged in (False, True):
+        e = _engine(model) if paged else get_dynamic_inference_engine(
+            model, NullTokenizer(127), max_batch_size=3,
+            max_sequence_length=64)
+        seen[paged] = []
+        tt.set_report(lambda r: seen[paged].append(r)
+                      if r["update_type"] == FlagType.RawAttentionScore.value
+                      else None)
+        e.generate([PROMPTS[4]], sp)
+        assert len(calls) == len(seen[paged]) == 2 * 4   # a prompt, 3 steps
+        calls.clear()
+        e.generate(PROMPTS[:2], sp)
+        calls.clear()
+    tt.set_report(None)
+    for a, b in zip(seen[False][:8], seen[True][:8]):
+        assert a["layer_id"] == b["layer_id"]
+        x, y = (torch.tensor(r["result"]).view(r["args"]) for r in (a, b))
+        n = min(x.shape[-1], y.shape[-1])
+        assert (x[..., :n] - y[..., :n]).abs().max() < 1e-5
+        assert (x[..., n:] == 0).all() and (y[..., n:] == 0).all()
+    last = seen[True][-1]       # two rows: 3 and 6 tokens, and 3 more
+    p = torch.tensor(last["result"]).view(last["args"])
+    assert p.shape == (2, 4, 1, 9) and (p[0, ..., 6:] == 0).all()
+    assert (p.sum(-1) - 1).abs().max() < 1e-5
+    destroy()
+
+
+@gpu
+def test_weights_of_a_decode_step_on_the_gpu():
+    """They are the ones that the kernel's output is made with."""
+    ctx = _context(device="cuda")
+    gen = torch.Generator().manual_seed(6)
+
+    def randn(t, b, heads):
+        return torch.randn(t, b, heads, 64, generator=gen).bfloat16().cuda()
+
+    ctx.begin_prompts([0, 2], [20, 33])
+    ctx.attend(1, randn(53, 1, 4), randn(53, 1, 2), randn(53, 1, 2))
+    ctx.set_active([2, 0])
+    q, k, v = randn(1, 2, 4), randn(1, 2, 2), randn(1, 2, 2)
+    out = ctx.attend(1, q, k, v, 0.125).view(2, 4, 64).double()
+    p = ctx.attention_weights(1, q, k, 0.125).double()
+    assert p.shape == (2, 4, 1, 34) and (p[1, ..., 21:] == 0).all()
+    table = ctx.cache.page_tables[[2, 0], :3].clamp(min=0).long()
+    values = ctx.cache.values(0)[table].permute(0, 2, 1, 3, 4).flatten(
+        2, 3)[:, :, :34].double().repeat_interleave(2, 1)
+    want = torch.matmul(p, values)[:, :, 0]
+    # the weights' rounding before V and the output's own, and 5% for what is
+    # in 32 bits
+    h = torch.finfo(torch.bfloat16).eps / 2
+    room = 1.05 * h * (want.abs() + torch.matmul(p, values.abs())[:, :, 0])
+    assert ((out - want).abs() <= room).all()
