@@ -31,10 +31,11 @@ class SharedPrefix:
     Rows ``rows[g]`` to ``rows[g + 1]`` (int32 [groups + 1] on the device,
     ascending) share their first ``lengths[g]`` tokens (int32 [groups]; whole
     pages count, a rest is left to each row): the page tables of these rows
-    name the same pages there, which is not looked at again; the first row's
-    are read for all.  Rows outside every group share nothing.  ``max_rows`` and
-    ``max_length`` are what the host knows about the largest group; they
-    choose how the work is cut, not what is computed.
+    name the same pages there, as far as each row is long, which is not looked
+    at again; one that holds all of them is read for all.  Rows outside every
+    group share nothing.  ``max_rows`` and ``max_length`` are what the host
+    knows about the largest group; they choose how the work is cut, not what
+    is computed.
     """
 
     rows: torch.Tensor

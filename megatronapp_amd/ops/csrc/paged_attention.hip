@@ -115,6 +115,28 @@ __device__ __forceinline__ int shared_at(const Cache& c, const Groups& gr,
                                                       : 0;
 }
 
+// The row of a group whose table is read for all: the first that holds all of
+// what they share, or the longest.  Rows that hold less have nothing in their
+// tables behind that.
+__device__ __forceinline__ int lead_row(const Cache& c, int from, int to,
+                                        int shared, int lane) {
+  int most = -1, at = from;      // the lane's longest
+  for (int base = from; base < to; base += WAVE) {
+    const int row = base + lane;
+    const int len = row < to ? length_at(c, slot_at(c, row)) : -1;
+    const unsigned long long whole = __ballot(len >= shared);
+    if (whole) return base + __builtin_ctzll(whole);
+    if (len > most) most = len, at = row;
+  }
+#pragma unroll
+  for (int off = 1; off < WAVE; off <<= 1) {
+    const int len = __shfl_xor(most, off, WAVE);
+    const int row = __shfl_xor(at, off, WAVE);
+    if (len > most || (len == most && row < at)) most = len, at = row;
+  }
+  return __builtin_amdgcn_readfirstlane(at);
+}
+
 // A lane's worth of a table: 64 page numbers from `base` on, read ahead so
 // that no step waits for its page's number.
 struct Pages {
@@ -451,13 +473,14 @@ __device__ __forceinline__ void shared_keys(
   const Places<D> at_lane(lane);
   const int hk = block % ng, piece = block / ng % gr.pieces;
   const int g = block / ng / gr.pieces % gr.groups;
-  const int first_row = group_row(gr, g);
-  const int queries = (group_row(gr, g + 1) - first_row) * rep;
+  const int first_row = group_row(gr, g), end_row = group_row(gr, g + 1);
+  const int queries = (end_row - first_row) * rep;
   const int shared = shared_of(c, gr, g);
   if (queries <= 0 || shared == 0) return;
   const int per = ((shared + gr.pieces - 1) / gr.pieces + BN - 1) / BN * BN;
   const int from = min(piece * per, shared), to = min(from + per, shared);
-  const int slot = max(0, min(slot_at(c, first_row), c.count - 1));
+  const int lead = lead_row(c, first_row, end_row, shared, lane);
+  const int slot = max(0, min(slot_at(c, lead), c.count - 1));
   const int* table = c.tables + (long)slot * c.width;
   const int turns = (to - from + BN - 1) / BN;
   // no tile lies in two pages: one number is enough

@@ -555,3 +555,37 @@ def test_pages_are_found_by_a_product():
             for x in (k * p - 1, k * p, k * p + 1, top):
                 if 0 <= x <= top:
                     assert x * magic >> shift == x // p, (x, p)
+
+
+# ------------------------------------------------- groups and who leads them
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hold", [
+    {0: 0}, {0: 40, 1: 0}, {i: 7 * i % 90 for i in range(69)},
+    {i: 320 - 16 * (1 + i % 5) - i % 3 for i in range(70)}])
+def test_groups_whose_first_rows_hold_less(hold, d):
+    """Empty and short rows in front, whose tables end with them: the others
+    see all of their prefix.  In the last case no row holds all of it."""
+    q, k, v, tables, lengths = _grouped_state([70], [320], [5] * 70, d=d,
+                                              nh=8)
+    for i, n in hold.items():
+        lengths[i] = n
+        tables[i, -(-n // 16):] = -1
+    g = _groups([0, 70], [320])
+    _near(paged_attention(q, k, v, tables, lengths, shared_prefix=g),
+          oracle(q, k, v, tables, lengths))
+
+
+@gpu
+def test_a_group_that_begins_with_padding():
+    """Rows without a slot in front of those that have one."""
+    q, k, v, tables, lengths = _grouped_state([20], [320], [5] * 20, d=64,
+                                              nh=8)
+    slots = torch.arange(20, dtype=torch.int32, device="cuda")
+    slots[:3] = torch.tensor([-1, 99, -1])
+    tables[0] = tables[0].flip(0)       # what a clamped number would read
+    got = paged_attention(q, k, v, tables, lengths, slots=slots,
+                          shared_prefix=_groups([0, 20], [320]))
+    want, room = oracle(q[3:], k, v, tables, lengths, slots=slots[3:])
+    _near(got[3:], (want, room))
+    assert (got[:3] == 0).all()
