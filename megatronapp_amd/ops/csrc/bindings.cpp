@@ -144,11 +144,12 @@ void launch_cache_write(int*, int*, int*, int*, int, int, int, int, const int*,
                         const void*, int, int, long, long, long, long,
                         hipStream_t);
 void paged_attn_pieces(int, int, int, int, int, int, int, long, int*, int*,
-                       int*);
+                       int*, int*);
 void launch_paged_attn(const void*, long, long, const void*, const void*,
                        const long*, const long*, const int*, const int*,
                        const int*, const int*, const int*, int, int, int, int,
-                       int, int, int, int, int, int, int, int, int, void*,
+                       int, int, int, int, int, int, int, int, int, int,
+                       void*,
                        float*,
                        float*, float, bool, hipStream_t);
 
@@ -1219,7 +1220,7 @@ torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
   TORCH_CHECK_VALUE((float)scale > 0 && std::isfinite((float)scale),
                     "paged_attention: softmax_scale must be positive and "
                     "finite");
-  int groups = 0, own, shared, evenly;
+  int groups = 0, own, shared, evenly, extra;
   if (prefix_rows.has_value()) {
     group_rows = paged_ints(*prefix_rows, q, 1, "shared_prefix.rows");
     group_lengths = paged_ints(*prefix_lengths, q, 1, "shared_prefix.lengths");
@@ -1241,7 +1242,7 @@ torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
                     (int)std::max(std::min(longest, room), 1l),
                     groups, (int)max_rows,
                     std::min(std::max(max_prefix, 0l), 1l << 30), &own,
-                    &shared, &evenly);
+                    &shared, &evenly, &extra);
   const int pieces = own + shared;
   torch::Tensor part;
   if (pieces > 1)
@@ -1257,7 +1258,7 @@ torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
                     groups ? group_rows.data_ptr<int>() : nullptr,
                     groups ? group_lengths.data_ptr<int>() : nullptr, groups,
                     (int)max_rows, b, nh, ng, d, (int)k.size(0), page,
-                    (int)tables.size(1), count, own, shared, evenly,
+                    (int)tables.size(1), count, own, shared, evenly, extra,
                     o.data_ptr(), po,
                     po ? po + (long)b * nh * pieces * d : nullptr,
                     (float)scale, fp16, cur_stream());
@@ -1451,6 +1452,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   mod.def("cache_extend", &cache_extend);
   mod.def("cache_write", &cache_write);
   mod.def("paged_attn", &paged_attn);
+  // how the work is cut: (pieces of a row at most, of a group's beginning, of
+  // a row in general, blocks for those beyond that)
+  mod.def("paged_attn_pieces", [](int b, int nh, int ng, int d, int max_length,
+                                  int groups, int max_rows, long max_prefix) {
+    int own, shared, evenly, extra;
+    paged_attn_pieces(b, nh, ng, d, max_length, groups, max_rows, max_prefix,
+                      &own, &shared, &evenly, &extra);
+    return std::make_tuple(own, shared, evenly, extra);
+  });
   mod.def("attn_bwd", &attn_bwd);
   mod.def("colsum_accum", &colsum_accum);
   mod.def("embedding_bwd_accum", &embedding_bwd_accum);

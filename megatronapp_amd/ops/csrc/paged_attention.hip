@@ -781,18 +781,24 @@ __global__ __launch_bounds__(BLOCK) void paged_join_kernel(Cache c, Groups gr,
 // These pieces have no blocks of their own, which would mostly find nothing to
 // do: 512 blocks share them out.  With a block for every piece that a row may
 // have, 128 rows on 200 tokens beside one on 60000 take 114 us, and 86 so.
+// Unless all rows are of the one group, a row may have `max_length` keys of its
+// own, whatever the others share: one of 20000 beside two that share as many,
+// 32/8 heads of 128, take 49 us, and 303 if the row may have no more keys of
+// its own than those.  Half as many blocks stand by for such rows: four groups
+// of 16 rows, each on 4096 tokens, take 48 us without any, 49 and, with all, 51.
 // ROOM bounds the memory that the pieces take.
 void paged_attn_pieces(int b, int nh, int ng, int d, int max_length,
                        int groups, int max_rows, long max_prefix, int* own,
-                       int* shared, int* evenly) {
+                       int* shared, int* evenly, int* extra) {
   constexpr long SHARE = 96l << 20, FILL = 512, ROOM = 64l << 20;
   const long blocks = (long)b * ng * ((nh / ng + HEADS - 1) / HEADS);
   *shared = 0;
-  long most = max_length;
+  long most = max_length, longest = most;     // own keys, of these and of all
   const long rows = std::min((long)b, (long)groups * max_rows);
   if (rows * max_prefix * ng * d * 4 > SHARE) {
     max_prefix = std::min(max_prefix, most);
     most = std::max(1l, most - max_prefix);
+    if (groups == 1 && max_rows >= b) longest = most;
     const long units =
         (long)groups * ng * (((long)max_rows * (nh / ng) + BM - 1) / BM);
     const long steps = (max_prefix + BN - 1) / BN;
@@ -806,9 +812,12 @@ void paged_attn_pieces(int b, int nh, int ng, int d, int max_length,
   *evenly = 1;
   while (*evenly < 64 && blocks * *evenly < FILL) *evenly *= 2;
   const long part = ROOM / ((long)b * nh * (d + 1) * 4);
-  *own = cuts((int)most, *evenly,
-              (int)std::max((long)*evenly, std::min(part, 64l)));
-  *evenly = std::min(*evenly, *own);
+  const int cap = (int)std::max((long)*evenly, std::min(part, 64l));
+  *evenly = std::min(*evenly, cuts((int)most, *evenly, cap));
+  *own = cuts((int)longest, *evenly, cap);
+  // rows in general may need none of them
+  const bool few = cuts((int)most, *evenly, cap) == *evenly;
+  *extra = (int)std::min(blocks * (*own - *evenly), few ? FILL / 2 : FILL);
 }
 
 void launch_paged_attn(const void* q, long qb, long qh, const void* k,
@@ -817,7 +826,8 @@ void launch_paged_attn(const void* q, long qb, long qh, const void* k,
                        const int* group_rows, const int* group_lengths,
                        int groups, int max_rows, int b, int nh, int ng, int d,
                        int pages, int page, int width, int count, int own,
-                       int shared, int evenly, void* o, float* part, float* lse,
+                       int shared, int evenly, int extra, void* o, float* part,
+                       float* lse,
                        float scale, bool fp16, hipStream_t stream) {
   const unsigned long p16 = page / 16;
   const int shift = 37 + 63 - __builtin_clzl(p16);
@@ -826,7 +836,6 @@ void launch_paged_attn(const void* q, long qb, long qh, const void* k,
                    pages, page, width, count, ((1ul << shift) + p16 - 1) / p16,
                    shift};
   const long units = (long)b * ng * ((nh / ng + HEADS - 1) / HEADS);
-  const int extra = (int)std::min(units * (own - evenly), 512l);
   const Out out = {(unsigned short*)o, part, lse, own + shared, evenly, extra};
   const int tiles =
       (int)std::max(1l, ((long)max_rows * (nh / ng) + BM - 1) / BM);

@@ -589,3 +589,39 @@ def test_a_group_that_begins_with_padding():
     want, room = oracle(q[3:], k, v, tables, lengths, slots=slots[3:])
     _near(got[3:], (want, room))
     assert (got[:3] == 0).all()
+
+
+# --------------------------------------------------------- how work is cut
+def _pieces(*args):
+    from megatronapp_amd import ops
+    if not ops.have_ops():
+        pytest.skip("the extension is not built")
+    return ops.get_ops().paged_attn_pieces(*args)
+
+
+@pytest.mark.parametrize("b,groups,max_rows,most,prefix", [
+    (3, 2, 2, 20050, 20000), (40, 5, 30, 17000, 16384), (9, 1, 8, 9000, 8192)])
+def test_a_long_row_outside_the_group_is_cut(b, groups, max_rows, most,
+                                             prefix):
+    """A row that shares nothing may be as long as the longest of a group:
+    none of its pieces has more than 1024 keys."""
+    own, shared, evenly, extra = _pieces(b, 32, 8, 128, most, groups,
+                                         max_rows, prefix)
+    assert shared > 0 and own * 1024 >= most and evenly <= own
+    assert extra >= min(256, own - evenly)
+    # rows in general go by what they have of their own
+    assert evenly <= max(1, (most - prefix + 255) // 256)
+
+
+def test_rows_of_one_group_are_cut_by_what_is_their_own():
+    for b, own, prefix in ((64, 700, 4096), (256, 1024, 16384)):
+        cut = _pieces(b, 32, 8, 128, prefix + own, 1, b, prefix)
+        assert cut[0] == cut[2] == 1 < cut[1] and cut[3] == 0
+
+
+@gpu
+def test_a_long_row_beside_a_group():
+    own = [3, 70, 20000]
+    s = _grouped_state([2, 1], [20000, 0], own, d=128, nh=32, ng=8, page=32)
+    _near(paged_attention(*s, shared_prefix=_groups(
+        [0, 2, 3], [20000, 0], 2, 20000), max_length=20070), oracle(*s))
