@@ -786,11 +786,14 @@ __global__ __launch_bounds__(BLOCK) void paged_join_kernel(Cache c, Groups gr,
 // 32/8 heads of 128, take 49 us, and 303 if the row may have no more keys of
 // its own than those.  Half as many blocks stand by for such rows: four groups
 // of 16 rows, each on 4096 tokens, take 48 us without any, 49 and, with all, 51.
-// ROOM bounds the memory that the pieces take.
+// ROOM bounds the memory that a row's own pieces take, and four times as much
+// that of all: every row of the batch has room for its group's pieces, in a
+// group or not.  One piece of each is always there.
 void paged_attn_pieces(int b, int nh, int ng, int d, int max_length,
                        int groups, int max_rows, long max_prefix, int* own,
                        int* shared, int* evenly, int* extra) {
   constexpr long SHARE = 96l << 20, FILL = 512, ROOM = 64l << 20;
+  const long part = ROOM / ((long)b * nh * (d + 1) * 4);   // in pieces
   const long blocks = (long)b * ng * ((nh / ng + HEADS - 1) / HEADS);
   *shared = 0;
   long most = max_length, longest = most;     // own keys, of these and of all
@@ -807,11 +810,11 @@ void paged_attn_pieces(int b, int nh, int ng, int d, int max_length,
     const long room = beside * 4 < steps * units / 256 ? 512 : 256;
     const long per = std::max(4l, beside);
     *shared = (int)std::max(
-        1l, std::min(std::min((steps + per - 1) / per, room / units), 64l));
+        1l, std::min(std::min(std::min((steps + per - 1) / per, room / units),
+                              64l), 3 * part));
   }
   *evenly = 1;
   while (*evenly < 64 && blocks * *evenly < FILL) *evenly *= 2;
-  const long part = ROOM / ((long)b * nh * (d + 1) * 4);
   const int cap = (int)std::max((long)*evenly, std::min(part, 64l));
   *evenly = std::min(*evenly, cuts((int)most, *evenly, cap));
   *own = cuts((int)longest, *evenly, cap);

@@ -625,3 +625,18 @@ def test_a_long_row_beside_a_group():
     s = _grouped_state([2, 1], [20000, 0], own, d=128, nh=32, ng=8, page=32)
     _near(paged_attention(*s, shared_prefix=_groups(
         [0, 2, 3], [20000, 0], 2, 20000), max_length=20070), oracle(*s))
+
+
+def test_pieces_take_a_bounded_room():
+    """64 MB for rows' own ones, four times that for all, beyond one of each
+    kind; small groups in large batches above all."""
+    for b in (3, 200, 512, 2048):
+        for nh, ng in ((64, 8), (32, 32), (16, 1)):
+            for d in (64, 128):
+                row = b * nh * (d + 1) * 4      # of one piece, in bytes
+                for groups, rows, prefix in ((0, 1, 0), (1, 4, 32768),
+                                             (b, 1, 16384), (1, b, 100000)):
+                    own, shared, *_ = _pieces(b, nh, ng, d, prefix + 64,
+                                              groups, rows, prefix)
+                    assert own == 1 or own * row <= 64 << 20
+                    assert (own + shared) * row <= max(256 << 20, 2 * row)
