@@ -1445,6 +1445,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   mod.def("attn_fwd", &attn_fwd);
   mod.def("attn_fwd_ablate", &attn_fwd_ablate);
   mod.def("packed_attention", &packed_attention);
+  // how a tile's work for dK and dV is cut: (shares, floats for their sums)
+  mod.def("packed_attn_shares", [](int n, int tq, int tk, int b, int nh,
+                                   int ng, int d) {
+    long floats = 0;
+    const int shares = packed_attn_shares(n, tq, tk, b, nh, ng, d, &floats);
+    return std::make_tuple(shares, floats);
+  });
   mod.def("cache_fork", &cache_fork);
   mod.def("cache_free", &cache_free);
   mod.def("cache_compact", &cache_compact);

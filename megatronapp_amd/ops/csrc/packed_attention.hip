@@ -872,7 +872,7 @@ static constexpr long FOUR_WAVES = 768;
 // the average to do), but none of fewer than two tiles of queries; where every
 // CU has a block already, only long sequences are.  Sequences are taken to be
 // of one length.  The shares' sums are written and read once more, in 32 bits,
-// at most some 130 MB.
+// in at most ROOM floats (134 MB).
 //
 // Backward in one share and so, us: 4096 tokens, 32/8 heads of 128 655 and 502
 // (four shares: 522), of 64 370 and 283; 16384 tokens, 8/2 heads of 128 2540
@@ -882,15 +882,16 @@ static constexpr long FOUR_WAVES = 768;
 // 6921 tokens, 32/8 heads of 64 228 and 256.
 int packed_attn_shares(int n, int tq, int tk, int b, int nh, int ng, int d,
                        long* floats) {
-  constexpr long FILL = 512, LEAST = 2;
+  constexpr long FILL = 512, LEAST = 2, ROOM = 1l << 25;
   const long blocks = tiles_of(n, tk, (long)b * ng);
   const int bq = d == 128 ? Dkv<128, false>::BQ : Dkv<64, false>::BQ;
   const long tiles = (long)(nh / ng) * (tq / std::max(n, 1)) / (2 * bq);
   long fill = (FILL + blocks / 2) / std::max(blocks, 1l);
   if (blocks >= FILL / 2 && tiles < d * 3 / 16) fill = 1;
-  const long shares = std::max(1l, std::min(std::min(fill, tiles / LEAST), 8l));
-  *floats = shares > 1 ? (long)b * ng * ((long)tk / BM + n + 2) * shares * 2 *
-                             BM * d : 0;
+  const long each = (long)b * ng * ((long)tk / BM + n + 2) * 2 * BM * d;
+  const long shares = std::max(
+      1l, std::min(std::min(std::min(fill, tiles / LEAST), 8l), ROOM / each));
+  *floats = shares > 1 ? each * shares : 0;
   return (int)shares;
 }
 

@@ -749,3 +749,23 @@ def test_scores_of_a_packed_stream_are_reported(device):
     p = torch.tensor(seen[0]["result"]).view(4, 16, 16)
     assert (p[:, 10:, :10] == 0).all() and (p.triu(1) == 0).all()
     destroy()
+
+
+def test_shares_take_a_bounded_room():
+    """134 MB at most, also where sequences are short and each has a tile."""
+    from megatronapp_amd import ops
+    if not ops.have_ops():
+        pytest.skip("the extension is not built")
+    shares_of = ops.get_ops().packed_attn_shares
+    assert shares_of(1, 4096, 4096, 1, 32, 8, 128)[0] == 2
+    most = 0
+    for n in (1, 2, 8, 40):
+        for t in (1, 256, 1024, 8192):
+            for rep in (1, 4, 16, 64):
+                for heads in (1, 8, 32, 64, 96, 200):
+                    for d in (64, 128):
+                        shares, floats = shares_of(n, t, t, 1, heads * rep,
+                                                   heads, d)
+                        assert (floats == 0) == (shares == 1)
+                        most = max(most, 4 * floats)
+    assert 100e6 < most < 135e6
