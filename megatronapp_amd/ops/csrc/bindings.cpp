@@ -862,8 +862,11 @@ bool has_tangent(std::initializer_list<const torch::Tensor*> inputs) {
   return false;
 }
 
+// ends behind 32 bits stay behind the stream
 torch::Tensor int32_row(const torch::Tensor& t) {
-  return (t.scalar_type() == torch::kInt32 ? t : t.to(torch::kInt32))
+  return (t.scalar_type() == torch::kInt32
+              ? t
+              : t.clamp(INT32_MIN, INT32_MAX).to(torch::kInt32))
       .contiguous();
 }
 

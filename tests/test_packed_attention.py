@@ -769,3 +769,16 @@ def test_shares_take_a_bounded_room():
                         assert (floats == 0) == (shares == 1)
                         most = max(most, 4 * floats)
     assert 100e6 < most < 135e6
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_ends_behind_32_bits(device):
+    """They run out of the stream like any other that does."""
+    q, k, v, _ = _inputs([40], [40], device=device)
+
+    def run(*cu):
+        return packed_attention(q, k, v, PackedSeqParams(
+            cu_seqlens_q=torch.tensor(cu, device=device)))
+
+    assert torch.equal(run(0, 5, (1 << 32) + 7), run(0, 5, 40))
+    assert torch.equal(run(-(1 << 32) + 3, 5, 9), run(0, 5, 9))
