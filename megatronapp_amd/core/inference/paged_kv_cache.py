@@ -138,13 +138,20 @@ class PagedKVCache:
                     x.device != self.pages.device:
                 raise ValueError(f"PagedKVCache: {name} must be a list or an "
                                  "int32 or int64 [n] on the cache's device")
-            return x.int().contiguous()
+            return self._int32(x)
         x = [int(i) for i in x]
         if any(i < 0 or i >= below for i in x):
             raise ValueError(f"PagedKVCache: {name} out of range: {x}")
         if once and len(set(x)) < len(x):
             raise ValueError(f"PagedKVCache: {name} named twice: {x}")
         return torch.tensor(x, dtype=torch.int32, device=self.pages.device)
+
+    @staticmethod
+    def _int32(x: torch.Tensor) -> torch.Tensor:
+        """What does not fit 32 bits stays out of every range."""
+        if x.dtype != torch.int32:
+            x = x.clamp(-1 << 31, (1 << 31) - 1).int()
+        return x.contiguous()
 
     @property
     def _native(self) -> bool:
@@ -287,7 +294,7 @@ class PagedKVCache:
             raise ValueError("PagedKVCache: write: cu_seqlens must be "
                              "[slots + 1] on the cache's device")
         else:
-            cu_seqlens = cu_seqlens.int().contiguous()
+            cu_seqlens = self._int32(cu_seqlens)
         if self._native:
             _ops.get_ops().cache_write(*self.state, layer, key, value, slots,
                                        cu_seqlens)

@@ -408,3 +408,29 @@ def test_the_cache_holds_values_without_their_derivatives(device):
     page = int(c.page_tables[0, 0])
     assert torch.equal(c.keys(0)[page, :, 0], x[0].detach() * 2)
     assert torch.equal(c.values(0)[page, :, 0], x[0].detach())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_numbers_behind_32_bits_are_out_of_range(device):
+    c = make(device)
+    c.extend([0, 1], [20, 5])
+    kept = [x.clone() for x in c.state[:4]]
+    far = torch.tensor([1 << 32], device=device)
+    zero = torch.tensor([0], device=device)
+    x = torch.ones(1, 2, 8, dtype=torch.bfloat16, device=device)
+    for call, message in (
+            (lambda: c.free(far), "slot out of range"),
+            (lambda: c.free(-far), "slot out of range"),
+            (lambda: c.fork(far, zero + 1), "slot out of range"),
+            (lambda: c.fork(zero, far + 2), "slot out of range"),
+            (lambda: c.extend(far, 1), "slot out of range"),
+            (lambda: c.extend(zero, far + 1), "longer"),
+            (lambda: c.copy_pages(zero, far + 9), "out of the pool"),
+            (lambda: c.write(0, x, x, far), "slot out of range"),
+            (lambda: c.write(0, x, x, zero, torch.cat([zero, far + 1])),
+             "longer")):
+        call()
+        with pytest.raises(RuntimeError, match=message):
+            c.check()
+        for a, b in zip(kept, c.state[:4]):
+            assert torch.equal(a, b)
