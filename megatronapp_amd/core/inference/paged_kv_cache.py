@@ -26,12 +26,13 @@ from ... import ops as _ops
 
 Slots = Union[Sequence[int], torch.Tensor]
 
-BAD_SLOT, NO_PAGE, BAD_PAGE, TOO_LONG = 1, 2, 4, 8
+BAD_SLOT, NO_PAGE, BAD_PAGE, TOO_LONG, SHARED = 1, 2, 4, 8, 16
 _MESSAGES = {
     BAD_SLOT: "a slot out of range, or named twice",
     NO_PAGE: "no free page left",
     BAD_PAGE: "a page out of the pool",
     TOO_LONG: "a sequence longer than its table",
+    SHARED: "a token for a page that several sequences hold",
 }
 
 

@@ -28,7 +28,9 @@ constexpr int PLAN = 1024;    // threads of a planning block
 constexpr int WAVES = PLAN / WAVE;
 constexpr int BLOCK = 256;
 
-enum Status { BAD_SLOT = 1, NO_PAGE = 2, BAD_PAGE = 4, TOO_LONG = 8 };
+enum Status {
+  BAD_SLOT = 1, NO_PAGE = 2, BAD_PAGE = 4, TOO_LONG = 8, SHARED = 16
+};
 
 struct Pool {
   int* refs;
@@ -434,6 +436,11 @@ __global__ __launch_bounds__(BLOCK) void write_kernel(
   const int page = p.tables[(long)s * p.width + at / p.page];
   if (page < 0 || page >= p.pages) {
     atomicOr(p.status, BAD_PAGE);
+    return;
+  }
+  // where an extension found no page, the last place is in an older one
+  if (p.refs[page] > 1) {
+    atomicOr(p.status, SHARED);
     return;
   }
   const long to =

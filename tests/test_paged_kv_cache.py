@@ -434,3 +434,27 @@ def test_numbers_behind_32_bits_are_out_of_range(device):
             c.check()
         for a, b in zip(kept, c.state[:4]):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_shared_pages_are_not_written_where_an_extension_failed(device):
+    """No page is left for the step of a sequence whose last page is full:
+    its token must not go there, where the others would read it."""
+    m = Model(make(device, num_pages=3))
+    m.extend([0], [32])
+    m.fork([0], [1])
+    m.extend([2], [3])
+    before = [x.clone() for x in m.cache.state[:4]]
+    x = torch.ones(2, 2, 8, dtype=torch.bfloat16, device=m.cache.pages.device)
+    m.cache.extend([1, 2], 1)
+    for layer in range(2):
+        m.cache.write(layer, x[:1], x[:1], [1])
+    with pytest.raises(RuntimeError, match="no free page.*several sequences"):
+        m.cache.check()
+    for a, b in zip(before, m.cache.state[:4]):
+        assert torch.equal(a, b)
+    m.free([0])                 # now it is slot 1's alone
+    m.cache.write(0, x[:1], x[:1], [1])
+    m.cache.check()
+    page = int(m.cache.page_tables[1, 1])
+    assert (m.cache.keys(0)[page, :, 15] == 1).all()
