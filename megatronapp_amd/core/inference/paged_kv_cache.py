@@ -10,7 +10,9 @@ captured into a graph.  A call that the host can see to be wrong raises; one
 that only the tables show to be impossible (no page left, a slot out of range
 in a device tensor, a target named twice) changes nothing and is reported by
 the next ``check()``.  Two exceptions: ``write`` leaves out the tokens it has
-no place for, and ``free`` and ``copy_pages`` leave out what is out of range.
+no place for, or only one in a shared page (where an ``extend`` before it could
+not be carried out), and ``free`` and ``copy_pages`` leave out what is out of
+range.
 
 On the GPU this is ``ops/csrc/paged_cache.hip``; on the CPU the same in torch.
 """
@@ -410,6 +412,9 @@ class PagedKVCache:
                 page = int(self.page_tables[s, at // self.page_size])
                 if not 0 <= page < self.num_pages:
                     self._fail(BAD_PAGE)
+                    continue
+                if int(self.ref_counts[page]) > 1:
+                    self._fail(SHARED)
                     continue
                 self.pages[layer, 0, page, :, at % self.page_size] = key[t]
                 self.pages[layer, 1, page, :, at % self.page_size] = value[t]
