@@ -19,6 +19,7 @@ from typing import Optional
 import torch
 from torch.autograd import forward_ad
 
+from .paged_kv_cache import MOST_TOKENS
 from ... import ops as _ops
 
 HEAD_SIZES = (64, 128)
@@ -122,6 +123,9 @@ def _check(query, key_pages, value_pages, page_tables, lengths, slots,
             query.shape[0]:
         raise ValueError("paged_attention: one length for each table, one "
                          "table or slot for each row")
+    if page_tables.shape[1] * page > MOST_TOKENS:
+        raise ValueError("paged_attention: tables of 2^31 tokens, or 8191 "
+                         "fewer, are too long")
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError("paged_attention: softmax_scale must be positive "
                          "and finite")

@@ -29,6 +29,8 @@ from ... import ops as _ops
 Slots = Union[Sequence[int], torch.Tensor]
 
 BAD_SLOT, NO_PAGE, BAD_PAGE, TOO_LONG, SHARED = 1, 2, 4, 8, 16
+# of a sequence: sums of places and a few thousand stay below 2^31
+MOST_TOKENS = (1 << 31) - 8192
 _MESSAGES = {
     BAD_SLOT: "a slot out of range, or named twice",
     NO_PAGE: "no free page left",
@@ -93,9 +95,9 @@ class PagedKVCache:
                 lengths.shape[0] != page_tables.shape[0]:
             raise ValueError("PagedKVCache: the tensors' sizes do not fit "
                              "each other")
-        if page_tables.shape[1] * pages.shape[4] >= 1 << 31:
-            raise ValueError("PagedKVCache: a sequence of 2^31 tokens and "
-                             "more does not fit its length")
+        if page_tables.shape[1] * pages.shape[4] > MOST_TOKENS:
+            raise ValueError("PagedKVCache: a sequence of 2^31 tokens, or "
+                             "8191 fewer, does not fit its length")
         self.pages = pages
         self.ref_counts = ref_counts
         self.page_tables = page_tables

@@ -1000,6 +1000,11 @@ torch::Tensor packed_attention(torch::Tensor q, torch::Tensor k,
 // ------------------------------------------------------------- paged cache
 // pages [layers, 2, P, groups, page, d]; refs [P], tables [slots, W], lengths
 // [slots] and status [1] int32, all on one GPU and contiguous
+
+// of a sequence: the kernels add the keys of a step, and of a piece's rounded
+// share for each of 64 pieces, to a place before they compare it with the end
+constexpr long MOST_TOKENS = (1l << 31) - 8192;
+
 struct CacheRefs {
   int *refs, *tables, *lengths, *status;
   int pages, slots, width, page, planes, groups, token;
@@ -1029,7 +1034,7 @@ CacheRefs cache_refs(const torch::Tensor& pages, const torch::Tensor& refs,
                   lengths.numel() == tables.size(0) && status.numel() > 0 &&
                   token % 16 == 0 && pages.size(2) < (1l << 30) &&
                   tables.size(0) <= (1l << 18) &&
-                  tables.size(1) * (long)pages.size(4) < (1l << 31),
+                  tables.size(1) * (long)pages.size(4) <= MOST_TOKENS,
               "the cache's tensors do not fit each other");
   return {refs.data_ptr<int>(),    tables.data_ptr<int>(),
           lengths.data_ptr<int>(), status.data_ptr<int>(),
@@ -1214,10 +1219,12 @@ torch::Tensor paged_attn(torch::Tensor q, torch::Tensor k, torch::Tensor v,
   if (row_slots.has_value()) slots = paged_ints(*row_slots, q, 1, "slots");
   TORCH_CHECK_VALUE(lengths.numel() == count && count > 0 &&
                         tables.size(1) > 0 &&
-                        tables.size(1) * (long)page < (1l << 31) &&
                         (slots.defined() ? slots.numel() : count) == b,
                     "paged_attention: one length for each table, one table or "
                     "slot for each row");
+  TORCH_CHECK_VALUE(tables.size(1) * (long)page <= MOST_TOKENS,
+                    "paged_attention: tables of 2^31 tokens, or 8191 fewer, "
+                    "are too long");
   const double scale = softmax_scale.has_value() ? *softmax_scale
                                                  : 1.0 / std::sqrt((double)d);
   TORCH_CHECK_VALUE((float)scale > 0 && std::isfinite((float)scale),

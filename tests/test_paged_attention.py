@@ -640,3 +640,12 @@ def test_pieces_take_a_bounded_room():
                                               groups, rows, prefix)
                     assert own == 1 or own * row <= 64 << 20
                     assert (own + shared) * row <= max(256 << 20, 2 * row)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_tables_that_pass_32_bits_are_refused(device):
+    for width in (1 << 22, (1 << 22) - 15):
+        wide = torch.zeros(2, width, dtype=torch.int32, device=device)
+        q, k, v, _, lengths = _state([20, 20], page=512, device=device)
+        with pytest.raises(ValueError, match="too long"):
+            paged_attention(q, k, v, wide, lengths)

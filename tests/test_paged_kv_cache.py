@@ -458,3 +458,16 @@ def test_shared_pages_are_not_written_where_an_extension_failed(device):
     m.cache.check()
     page = int(m.cache.page_tables[1, 1])
     assert (m.cache.keys(0)[page, :, 15] == 1).all()
+
+
+def test_places_next_to_the_longest_stay_in_32_bits():
+    """A kernel's step or piece may end behind the longest sequence."""
+    ints = dict(dtype=torch.int32)
+    for width, fits in (((1 << 22) - 16, True), ((1 << 22) - 15, False)):
+        args = (torch.zeros(1, 2, 1, 1, 512, 8), torch.zeros(1, **ints),
+                torch.zeros(1, width, **ints), torch.zeros(1, **ints))
+        if fits:
+            PagedKVCache.from_state(*args)
+        else:
+            with pytest.raises(ValueError, match="2.31"):
+                PagedKVCache.from_state(*args)
