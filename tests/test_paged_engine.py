@@ -438,3 +438,103 @@ def test_weights_of_a_decode_step_on_the_gpu():
     h = torch.finfo(torch.bfloat16).eps / 2
     room = 1.05 * h * (want.abs() + torch.matmul(p, values.abs())[:, :, 0])
     assert ((out - want).abs() <= room).all()
+
+
+SURELY = 1 << 20      # a host that expects this much shares pages in any case
+
+
+@gpu
+@pytest.mark.parametrize("page", [16, 64])
+def test_shared_pages_after_forks_and_compaction(page):
+    """The group's kernel over tables that forks and a compaction left."""
+    from megatronapp_amd.core.inference import (PagedKVCache, SharedPrefix,
+                                                paged_attention)
+    nh, ng, d, dev = 8, 2, 64, "cuda"
+    gen = torch.Generator().manual_seed(3)
+
+    def randn(*shape):
+        return torch.randn(*shape, generator=gen).bfloat16().to(dev)
+
+    cache = PagedKVCache(1, 64, page, ng, d, 8, 512)
+    lens = [200, 3 * page, 9]
+    held, slots = {}, [0, 3, 4, 5, 1, 2]
+    for s, n in reversed(list(enumerate(lens))):
+        kv = randn(2, n, ng, d)
+        cache.extend([s], n)
+        cache.write(0, kv[0], kv[1], [s],
+                    torch.tensor([0, n], dtype=torch.int32, device=dev))
+        held[s] = kv
+    cache.free([2])
+    cache.fork([0, 0, 0, 1], [3, 4, 5, 2])
+    held.update({3: held[0], 4: held[0], 5: held[0], 2: held[1]})
+    for turn in range(20):
+        new = randn(2, len(slots), ng, d)
+        cache.extend(slots, 1)
+        cache.write(0, new[0], new[1], slots)
+        for i, s in enumerate(slots):
+            held[s] = torch.cat([held[s], new[:, i:i + 1]], 1)
+        if turn == 10:
+            cache.compact()
+    cache.check()
+    ints = dict(dtype=torch.int32, device=dev)
+    shared = 200 // page * page
+    q = randn(len(slots), nh, d)
+    got = paged_attention(
+        q, cache.keys(0), cache.values(0), cache.page_tables, cache.lengths,
+        slots=torch.tensor(slots, **ints),
+        shared_prefix=SharedPrefix(torch.tensor([0, 4, 6], **ints),
+                                   torch.tensor([shared, 3 * page], **ints),
+                                   4, SURELY))
+    h = torch.finfo(torch.bfloat16).eps / 2
+    for i, s in enumerate(slots):
+        k, v = (x.double().repeat_interleave(nh // ng, 1) for x in held[s])
+        w = torch.softmax(torch.einsum("hd,nhd->hn", q[i].double(), k)
+                          / d ** 0.5, -1)
+        o = torch.einsum("hn,nhd->hd", w, v)
+        room = 1.05 * h * (o.abs() + torch.einsum("hn,nhd->hd", w, v.abs()))
+        assert ((got[i].double() - o).abs() <= room).all(), s
+
+
+@gpu
+def test_the_engines_steps_share_pages(monkeypatch):
+    """A family's steps with the pages that it shares read once: the logits
+    of the steps that read them row by row, within the roundings of a model
+    of two layers (80 h of the largest, as above)."""
+    from megatronapp_amd.core.inference.paged_context import (
+        PagedInferenceContext)
+    model = _model(device="cuda", hidden=256, heads=4, groups=2, bf16=True)
+    sp = SamplingParams(num_tokens_to_generate=8, top_k=1)
+    inner = PagedInferenceContext._shared_prefix
+
+    def surely(self, shared):
+        prefix = inner(self, shared)
+        if prefix is not None:
+            prefix.max_length = SURELY
+            forced.append(prefix.lengths.tolist())
+        return prefix
+
+    seen, forced, texts = {}, [], {}
+    for force in (False, True):
+        if force:
+            monkeypatch.setattr(PagedInferenceContext, "_shared_prefix",
+                                surely)
+        e = _engine(model, slots=6)
+        steps = seen[force] = []
+        take = e._logits_last
+        e._logits_last = lambda x: steps.append(take(x)) or steps[-1]
+        ids = e.add_parallel_requests(PROMPTS[4], sp, 4)
+        ids.append(e.add_request(PROMPTS[1], sp))
+        while e.has_unfinished_requests():
+            e.step()
+        texts[force] = [e.finished[i].generated_text for i in ids]
+    assert forced and forced[0] == [32, 0]
+    h = torch.finfo(torch.bfloat16).eps / 2
+    rows = [x for x in seen[False] if x.shape[0] == 5]
+    assert len(rows) == 7
+    for a, b in zip(rows, [x for x in seen[True] if x.shape[0] == 5]):
+        off = (a.float() - b.float()).abs().max()
+        assert off <= 80 * h * a.float().abs().max()
+        if not torch.equal(a.argmax(-1), b.argmax(-1)):
+            break               # from here on they answer different tokens
+    assert len(set(texts[True][:4])) == 1
+    destroy()
