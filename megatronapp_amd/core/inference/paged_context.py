@@ -89,6 +89,9 @@ class PagedInferenceContext:
         """Row i of the active batch continues row indices[i] (a step of beam
         search)."""
         order = indices.tolist()
+        if not all(0 <= i < len(self.active) for i in order):
+            raise ValueError(f"PagedInferenceContext: rows {order} of "
+                             f"{len(self.active)}")
         self.cache.fork([self.active[i] for i in order], self.active)
         lengths = [self.host_lengths[self.active[i]] for i in order]
         for s, n in zip(self.active, lengths):

@@ -538,3 +538,15 @@ def test_the_engines_steps_share_pages(monkeypatch):
             break               # from here on they answer different tokens
     assert len(set(texts[True][:4])) == 1
     destroy()
+
+
+def test_reordering_names_rows_of_the_batch():
+    """A number below zero is no row from the end."""
+    ctx = _context()
+    ctx.begin_prompts([0, 1], [5, 7])
+    for order in ([0, -1], [2, 0], [0]):
+        with pytest.raises(ValueError):
+            ctx.reorder_batch(torch.tensor(order))
+    assert ctx.cache.lengths.tolist() == ctx.host_lengths == [5, 7, 0]
+    ctx.reorder_batch(torch.tensor([1, 0]))
+    assert ctx.cache.lengths.tolist() == ctx.host_lengths == [7, 5, 0]
