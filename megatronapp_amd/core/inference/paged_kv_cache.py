@@ -6,13 +6,14 @@ their full pages (``ref_counts`` says by how many a page is held); a
 part-filled page belongs to one sequence, so nothing shared is ever written.
 
 All state is on the cache's device and no call waits for it, so calls may be
-captured into a graph.  A call that the host can see to be wrong raises; one
-that only the tables show to be impossible (no page left, a slot out of range
-in a device tensor, a target named twice) changes nothing and is reported by
-the next ``check()``.  Two exceptions: ``write`` leaves out the tokens it has
-no place for, or only one in a shared page (where an ``extend`` before it could
-not be carried out), and ``free`` and ``copy_pages`` leave out what is out of
-range.
+captured into a graph where slots, pages and counts are tensors on that device;
+lists are checked by the host and copied there, which waits and cannot be
+captured.  A call that the host can see to be wrong raises; one that only the
+tables show to be impossible (no page left, a slot out of range in a device
+tensor, a target named twice) changes nothing and is reported by the next
+``check()``.  Two exceptions: ``write`` leaves out the tokens it has no place
+for, or only one in a shared page (where an ``extend`` before it could not be
+carried out), and ``free`` and ``copy_pages`` leave out what is out of range.
 
 On the GPU this is ``ops/csrc/paged_cache.hip``; on the CPU the same in torch.
 """

@@ -10,6 +10,16 @@
 //   the gradients of Q and K, 2.8e-3 against 2.4e-3 of them in bf16)
 //   dQ = scale dS K, dK = scale dS^T Q, both sums over the group's heads
 //
+// Rounded to 16 bits are P before its products with V and dO, and dS before its
+// own, because the matrix unit takes nothing wider at this rate; all sums stay
+// in 32 bits.  Against a form that rounds only at the end the output's error is
+// 1.1 times as large and the gradients' 1.45 times (1.8e-3 for 1.6e-3 and 2.4e-3
+// for 1.7e-3 in bf16); two parts of 16 bits each would take it back for three
+// products more of the backward's seven, and one of the forward's two.
+//
+// Times of single kernels below are the shortest of 20 under the profiler, some
+// 5% above what they take in passes without it.
+//
 // The stream's sequences are given on the device, so the grid has as many
 // tiles as could be needed and a block finds its own (sequence, tile) by
 // adding up the sequences' tile counts.  No tile holds rows of two
@@ -77,8 +87,8 @@ __device__ __forceinline__ int wave_sum(int v) {
 // sequences fit a wave's lanes, tiles are handed out by that: level L holds
 // the L-th tile (from the other end for keys) of every sequence that has one,
 // and the highest level goes first, so that the last blocks to start are the
-// shortest.  8 documents of 45 to 2048 tokens, 16 heads of 128: CUs were idle
-// 37% of the forward's time in stream order (94 us).
+// shortest.  8 documents of 45 to 2048 tokens, 16 heads of 128, forward: 94 us
+// in stream order, 82 so, with the CUs busy 76% of the time.
 template <bool KEYS>
 __device__ __forceinline__ bool find_span(const Packing& pk, int slot,
                                           int lane, Span& s) {
@@ -161,18 +171,19 @@ __device__ __forceinline__ int head_of(int x, int ng, int rep) {
 // A wave holds 32 rows of Q as the right operand of S^T = K Q^T, and P^T, which
 // that leaves in its registers, is the right operand of O^T = V^T P^T; the four
 // waves share the tiles of K and V, of which the next one comes into the other
-// of two images while one is used.  Two blocks of 188 registers at D = 128 and
-// four of 123 at 64 run on a CU, each at another place of its loop, so that one
+// of two images while one is used.  Two blocks of 187 registers at D = 128 and
+// four of 122 at 64 run on a CU, each at another place of its loop, so that one
 // does its exponentials beside the other's products.
 //
-// At D = 64 the vector unit bounds it (busy 64% of the time, the matrix unit
-// 28%): an element takes some six of its instructions and two products; 15
-// documents of 1 to 2048 tokens, 32 heads, take 146 us in training, 700
-// TFLOP/s.  At 128 both are near: 8192 + 5003 + 3001 + 188 tokens, 32 heads,
-// fp16 take 830 us, 1000 TFLOP/s, at the 1.8 GHz that the power allows.  Where
+// At D = 64 the vector unit bounds it (active 69% of the time, the matrix unit
+// busy 31%): an element takes some six of its instructions and two products; 15
+// documents of 1 to 2048 tokens, 32 heads, take 161 us, 630 TFLOP/s.  At 128
+// both are near (51% and 48%): 8192 + 5003 + 3001 + 188 tokens, 32 heads, fp16
+// take 890 us without the profiler, 930 TFLOP/s, and under it the clock falls
+// to 1.6 GHz, where shorter work runs at 2.1: that is the power's doing.  Where
 // sequences are few and uneven, the longest tiles are more than a CU's share
-// of the work: ten prompts of 0 to 2048 tokens, 32 heads, 82 us (740), eight
-// documents of 45 to 2048, 16 heads, in training 74 us (710).
+// of the work: ten prompts of 0 to 2048 tokens, 32 heads, 89 us (680; CUs busy
+// 81% of the time), eight documents of 45 to 2048, 16 heads, 82 us (640).
 //
 // Taken back: 64 rows a wave at D = 64 (half the reads of K and V: equal, for
 // short prompts 9.0 us against 7.5), the next tile's scores beside this one's
@@ -362,12 +373,12 @@ __global__ __launch_bounds__(BLOCK * HALVES, 2) void packed_fwd_kernel(
 // order changes results.  Each row's D is found on the way, and left for the
 // other kernel (a kernel of its own: backward 247 us, so 235).
 //
-// Eight documents of 45 to 2048 tokens, 16 heads of 128: 103 us, 760 TFLOP/s;
-// fifteen of 1 to 2048, 32 heads of 64: 198 us, 770.  The matrix unit is busy
-// a third of the time, the vector unit 27% at 128 and 47% at 64; two waves on
-// a SIMD do not cover more of each other's waits.  Eight waves on a tile there
-// keep all of a CU's waves in step: the backward takes 280 us for 244, and 587
-// for 466.
+// Eight documents of 45 to 2048 tokens, 16 heads of 128: 110 us, 710 TFLOP/s;
+// fifteen of 1 to 2048, 32 heads of 64: 215 us, 710.  The matrix unit is busy
+// 33% and 38% of the time, the vector unit active 26% and 51%, and the waves
+// wait 28% and 34% of theirs; two waves on a SIMD do not cover more of each
+// other's waits.  Eight waves on a tile there keep all of a CU's waves in step:
+// the backward takes 280 us for 244, and 587 for 466.
 template <class T, int D, bool CAUSAL, int HALVES>
 __global__ __launch_bounds__(BLOCK * HALVES, 2) void packed_bwd_dq_kernel(
     const unsigned short* __restrict__ q, const unsigned short* __restrict__ k,
@@ -525,9 +536,10 @@ __global__ __launch_bounds__(BLOCK * HALVES, 2) void packed_bwd_dq_kernel(
 // whose sums are added at the end (one wave a SIMD: 228 us for 165 then, and
 // 546 for 361 at D = 64).
 //
-// The same documents as for dQ: 141 us, 740 TFLOP/s, and 245 us, 830.  Both
-// units are busy a third of the time, four tenths of it pass in waits, most
-// for LDS, where each 32 x 32 tile reads Q and dO along both axes.
+// The same documents as for dQ: 153 us, 680 TFLOP/s, and 274 us, 740.  The
+// matrix unit is busy 31% and 37% of the time, the vector unit active 25% and
+// 39%, and the waves wait 40% and 31% of theirs.  Each 32 x 32 tile reads Q and
+// dO along both axes, and at 128 K and V too, from LDS, without conflicts.
 //
 // Eight waves keep in step, which costs time; at D = 64, where K and V are in
 // registers, two blocks of four waves fit a CU instead, and are taken (MANY)
@@ -825,7 +837,11 @@ static long tiles_of(int n, int total, long heads) {
 // blocks, 46 + 46 and 39 + 40; 4096 tokens, 8 heads, 264, 82 + 81 and 67 + 66,
 // 16 heads, 528, 98 + 95 and 85 + 78; two of 2048, 16 heads, 528, 53 + 52 and
 // 51 + 49; 1500 + 900 tokens, 32 heads of 64, 608, 29 + 36 and 32 + 39; five
-// of 310 tokens in all 7.0 and 7.7.
+// of 310 tokens in all 7.0 and 7.7.  At D = 64 a prompt: 2048 tokens, 16 heads,
+// 34 and 28, 4096 tokens, 8 heads, 59 and 48, 16 heads 65 and 55, two of 2048
+// 35 and 33, 1500 + 900 tokens 26 and 21, and a whole pass with gradients 116
+// and 101, 196 and 162, 242 and 219, 137 and 130, 95 and 82; 600 + 600 tokens
+// 13 and 11.5, with gradients 81 in both.
 static bool in_halves(int n, int tq, int tk, int b, int nh) {
   return tiles_of(n, tq, (long)b * nh) <= 576 && tk / std::max(n, 1) >= 512;
 }
@@ -863,8 +879,9 @@ void launch_packed_attn_fwd(const void* q, const void* k, const void* v,
 // Backward with eight and four waves, us, 16 heads: 4096 tokens in two
 // sequences, 528 blocks, 99 and 108, 6144 in three, 800 blocks, 132 and 121;
 // 1024 in each of eight, 1088, 110 and 100; 32 heads, 300 in each of twelve,
-// 1088, 75 and 60; 32/8 heads, 8192 + 5003, 832, 1435 and 1508; the fifteen
-// documents, 1120, 467 and 444.
+// 1088, 75 and 60; the fifteen documents, 1120, 467 and 444.  The rule does not
+// look at lengths, for which few long sequences pay: 32/8 heads, 8192 + 5003
+// tokens, 832 blocks, 1435 and 1508.
 static constexpr long FOUR_WAVES = 768;
 
 // Into how many shares a tile's work for dK and dV is cut, so that there are
@@ -879,7 +896,8 @@ static constexpr long FOUR_WAVES = 768;
 // and 1850; 1024 tokens, 32/8 heads of 128 151 and 84; 8192 tokens, 8/1 heads
 // of 128 1950 and 590; 4096 tokens, 8 heads of 128 233 and 212.  In two shares
 // all the same: 2048 tokens, 16 heads of 128 126 and 130, five sequences of
-// 6921 tokens, 32/8 heads of 64 228 and 256.
+// 6921 tokens, 32/8 heads of 64 228 and 256; these two set the bound on tiles
+// where every CU has a block.
 int packed_attn_shares(int n, int tq, int tk, int b, int nh, int ng, int d,
                        long* floats) {
   constexpr long FILL = 512, LEAST = 2, ROOM = 1l << 25;

@@ -7,7 +7,10 @@
 // piece leaves its own o and log2 of its sum, and a second launch joins them:
 //   o = sum_i 2^(L_i - M) o_i / sum_i 2^(L_i - M),  M = max L_i
 // A row without tokens gives zeros.  A page number out of the pool leaves its
-// tokens out.
+// tokens out.  The weights are rounded to 16 bits before their product with V,
+// which the matrix unit takes nothing wider for at this rate (the output's
+// error is 1.1 times what its last rounding alone leaves); scores, sums and
+// what is joined of pieces stay in 32 bits.
 //
 // Rows of a group begin with the same pages.  Their queries, for all heads of
 // a key head, are the rows of a matrix product over these pages, done once
@@ -457,9 +460,9 @@ __device__ __forceinline__ void rows_block(const unsigned short* q, long qb,
 // queries a wave (rows times the heads of a key head), tiles of 64 keys in two
 // images.  Its products are bound by the matrix and vector units, so that the
 // rows' own keys, read beside them, cost little: 64 rows on 4096 + 33..700
-// tokens, 32/8 heads of 128, take 34 us (113 MB, 4.7 GFLOP) and the join 6;
-// 256 rows on 16384 + 1..1024 170 (611 MB, 71 GFLOP) and 8.  Each row for
-// itself, joined: 97 and 1190.
+// tokens, 32/8 heads of 128, take 34 us (113 MB, 4.7 GFLOP) and the join 5;
+// 256 rows on 16384 + 1..1024 171 (611 MB, 71 GFLOP) and 8; in fp16 the same.
+// Each row for itself, joined: 97 and 1190.
 template <class T, int D>
 __device__ __forceinline__ void shared_keys(
     const unsigned short* q, long qb, long qh, const Cache& c,
