@@ -98,7 +98,17 @@ class PagedInferenceContext:
             self.host_lengths[s] = n
         self._groups = None
 
-    def _check_room(self, slots: List[int], more: List[int]):
+    def _check(self, slots: List[int], more: List[int], empty: bool):
+        """What the host can see to be wrong of tokens to come."""
+        if len(more) != len(slots) or len(set(slots)) < len(slots) or \
+                not all(0 <= s < self.max_slots for s in slots):
+            raise ValueError(f"PagedInferenceContext: slots {slots} of "
+                             f"{self.max_slots}, each once, with a number of "
+                             f"tokens each, got {len(more)}")
+        used = [s for s in slots if empty and self.host_lengths[s]]
+        if used:
+            raise ValueError(f"PagedInferenceContext: slots in use: {used}; "
+                             "release() empties them")
         full = [s for s, n in zip(slots, more)
                 if self.host_lengths[s] + n > self.max_sequence_length]
         if full:
@@ -115,11 +125,7 @@ class PagedInferenceContext:
     def begin_prompts(self, slots: List[int], lengths: List[int]):
         """The next call of the model is one stream of these prompts, in
         slots that hold nothing."""
-        used = [s for s in slots if self.host_lengths[s]]
-        if used:
-            raise ValueError(f"PagedInferenceContext: slots in use: {used}; "
-                             "release() empties them")
-        self._check_room(slots, lengths)
+        self._check(slots, lengths, True)
         self._set_slots(slots)
         self.prefill = True
         self.cache.extend(self._slots, lengths)
@@ -143,7 +149,7 @@ class PagedInferenceContext:
         ``shared`` says how the batch begins, as (rows, tokens) of groups of
         rows that share as many first tokens."""
         assert not prefill, "begin_prompts() admits prompts"
-        self._check_room(slots, [1] * len(slots))
+        self._check(slots, [1] * len(slots), False)
         self._set_slots(slots)
         self.prefill = False
         self.cache.extend(self._slots, 1)

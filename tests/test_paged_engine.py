@@ -550,3 +550,19 @@ def test_reordering_names_rows_of_the_batch():
     assert ctx.cache.lengths.tolist() == ctx.host_lengths == [5, 7, 0]
     ctx.reorder_batch(torch.tensor([1, 0]))
     assert ctx.cache.lengths.tolist() == ctx.host_lengths == [7, 5, 0]
+
+
+def test_calls_name_slots_that_there_are_once():
+    ctx = _context()
+    ctx.begin_prompts([0, 1], [5, 7])
+    for slots in ([2, 2], [3], [-1]):
+        with pytest.raises(ValueError, match="slots"):
+            ctx.begin_prompts(slots, [4] * len(slots))
+    with pytest.raises(ValueError, match="slots"):
+        ctx.begin_prompts([2], [4, 4])
+    for slots in ([0, 0], [0, 3], [-2]):
+        with pytest.raises(ValueError, match="slots"):
+            ctx.set_active(slots)
+    ctx.cache.check()
+    assert ctx.active == [0, 1]
+    assert ctx.cache.lengths.tolist() == ctx.host_lengths == [5, 7, 0]
