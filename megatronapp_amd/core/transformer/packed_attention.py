@@ -10,8 +10,9 @@ On the GPU this is ``ops/csrc/packed_attention.hip`` (bf16 and fp16, head
 sizes 64 and 128), whose gradient cannot be differentiated again, and which
 refuses forward-mode derivatives; on the CPU a plain computation in 32 bits or
 more.  A sequence's values reach no other sequence, whatever they are.  Within
-one, a value of v that is not finite may reach earlier rows of the same 64-key
-tile (nothing times NaN is NaN).
+one, what is not finite may reach rows of the same tile that do not see it
+(nothing times NaN is NaN): from v earlier rows, and in the gradients from k,
+from q and from the output's gradient too.
 """
 
 from __future__ import annotations
